@@ -311,6 +311,67 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
                         float* x_scale, void* h, void* h8, float* h_scale, void* y, void* scratch,
                         size_t scratch_bytes, void* stream);
 
+/* ---- up to 64 tokens on 4-bit weights, and on mixtures of experts (bf16 / fp16 activations) ----
+ * No counterpart in the reference (its module is one dense gated MLP, src/triton_gated_mlp/gated_mlp.py:203-237).
+ *
+ * 4-bit format of a matrix [rows, cols]: w = (q - zero) * scale, q an unsigned nibble, one scale (type `dtype`)
+ * and one zero (a byte, 0..15; only its low four bits are used) per row and group of `group` columns, group 32, 64
+ * or 128, cols a multiple of it.
+ *   w4     rows of cols / 2 bytes: little-endian 32-bit words, word j holding columns 8j .. 8j+7, column 8j + c at
+ *          bit (0, 16, 4, 20, 8, 24, 12, 28)[c]; 16-byte aligned
+ *   scale  [cols / group, rows];  zero [cols / group, rows], or NULL for zero = 8 everywhere
+ * A group's products are summed in fp32 with the integers q - zero and then multiplied by its scale: the weights
+ * are never rounded.
+ *
+ * gmlp_w4_linear: y[m,r] = sum_c x[m,c] w[r,c] (+ bias[r]) (+ residual[m,r]) for 1 <= M <= 64 and any rows >= 1; x
+ *   has row pitch ldx (a multiple of 8), y and residual [M, rows] are contiguous.
+ * gmlp_decode_fwd_w4: gmlp_decode_fwd with three such matrices (K and N multiples of group); two launches.
+ * Both start streaming weights before the preceding kernel on the stream has finished, with the precondition and
+ * the GMLP_TUNE_ORDINARY_LAUNCH way out of gmlp_decode_fwd.
+ *
+ * gmlp_moe_route: the router. logits = x w_router^T ([experts, K]); per token ids[M, top_k] = the experts of the top_k
+ *   largest logits in descending order (equal ones: lower index first; a NaN ranks below every number, so the ids
+ *   are valid and distinct whatever x holds), weights[M, top_k] = softmax over all experts at those ids,
+ *   divided by their sum if `renormalize`. experts <= 512, top_k <= min(32, experts), any M.
+ * gmlp_moe_decode_fwd: y[t] = sum_j weights[t,j] * MLP_{ids[t,j]}(x[t]) (+ residual[t]) with
+ *   MLP_e(x) = (act(x w_gate[e]^T) * (x w_up[e]^T)) w_down[e]^T; w_gate, w_up [experts, N, K], w_down [experts, K, N],
+ *   K and N multiples of 64, M <= 64. Only experts that some token chose are read. An id outside [0, experts) is
+ *   skipped (a padded row: -1 throughout gives y = residual, or 0); the same expert twice in a token adds. The
+ *   weights of the experts that are read must be finite: every token of the call is multiplied with them, by zero
+ *   where it did not choose them. `h`: work buffer of min(experts, M * top_k) * M * N values. Two launches; no
+ *   rule about the preceding kernel (the weights are streamed only once the routing table is there).
+ * gmlp_moe_decode_fwd_w4: the same on 4-bit experts (w4 [experts, rows, cols / 2], scale / zero
+ *   [experts, cols / group, rows]); K and N multiples of group.
+ *
+ * `scratch`: gmlp_few_scratch_bytes(K, N, experts) bytes (gmlp_w4_linear: K = N = rows, experts = 1; mixtures:
+ *   experts = min(experts, M * top_k) or more), 16-byte aligned. What lies behind its first
+ *   gmlp_few_scratch_counters() bytes must be ZERO before the first call; every call leaves it zero, unless
+ *   gmlp_status_read has since returned a non-zero word: then clear it again. Calls of any shapes that it is large
+ *   enough for may use a buffer one after the other; calls that share one must not overlap on the GPU. */
+size_t gmlp_few_scratch_bytes(int64_t K, int64_t N, int32_t experts);
+size_t gmlp_few_scratch_counters(void);
+int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t dtype, const void* x, int64_t ldx,
+                   const void* w4, const void* scale, const void* zero, const void* bias, const void* residual,
+                   void* y, void* scratch, size_t scratch_bytes, uint32_t tuning, void* stream);
+int gmlp_decode_fwd_w4(const gmlp_problem_t* p, int32_t group, const void* x, const void* w_gate4,
+                       const void* w_gate_scale, const void* w_gate_zero, const void* b_gate, const void* w_up4,
+                       const void* w_up_scale, const void* w_up_zero, const void* b_up, const void* w_down4,
+                       const void* w_down_scale, const void* w_down_zero, const void* b_down, const void* residual,
+                       void* h, void* y, void* scratch, size_t scratch_bytes, void* stream);
+int gmlp_moe_route(int64_t M, int64_t K, int32_t experts, int32_t top_k, int32_t renormalize, int32_t dtype,
+                   const void* x, int64_t ldx, const void* w_router, int32_t* ids, float* weights, void* stream);
+int gmlp_moe_decode_fwd(const gmlp_problem_t* p, int32_t experts, int32_t top_k, const void* x, const int32_t* ids,
+                        const float* weights, const void* w_gate, const void* w_up, const void* w_down,
+                        const void* residual, void* h, void* y, void* scratch, size_t scratch_bytes, void* stream);
+int gmlp_moe_decode_fwd_w4(const gmlp_problem_t* p, int32_t group, int32_t experts, int32_t top_k, const void* x,
+                           const int32_t* ids, const float* weights, const void* w_gate4, const void* w_gate_scale,
+                           const void* w_gate_zero, const void* w_up4, const void* w_up_scale, const void* w_up_zero,
+                           const void* w_down4, const void* w_down_scale, const void* w_down_zero,
+                           const void* residual, void* h, void* y, void* scratch, size_t scratch_bytes, void* stream);
+/* *id = 0, or the identity of the graph capture that `stream` is in: a host keys scratch buffers on it, so that
+ * two captured graphs never share one. */
+int gmlp_capture_id(void* stream, uint64_t* id);
+
 /* mask[M,N] (one byte per element, 1 = kept) for the problem's dropout settings:
  * the device side of the bit-exact mask check. */
 int gmlp_dropout_mask(const gmlp_problem_t* p, uint8_t* mask, void* stream);

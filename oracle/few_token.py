@@ -1,0 +1,130 @@
+"""CPU / 64-bit restatement of the few-token operators (4-bit weights, mixtures of experts), with error bounds.
+TEST INFRASTRUCTURE ONLY (tests/): never imported by the package.
+
+Every function returns (value, bound) in float64: the value of the definition and how far a right kernel may be off it.
+The bounds count, term by term,
+  * the rounding of the output, and of the hidden state between the two kernels, to the 16-bit type:
+    eps / 2 of the value, plus half the smallest subnormal;
+  * 32-bit sums: each addition is off by at most 2^-23 of the sum of magnitudes S = sum |w| |x| so far (the tensor
+    core may truncate, hence 2^-23 and not 2^-24); a sum of n columns in groups of G takes at most n / 16 steps of the
+    matrix instruction (16 columns each, counted as 2 additions) and n / G of the group sums, and at most 32 joins;
+  * the gate activation in 32 bits: 2^-19 relative (exp and division of the fast kind, each below 2^-21), and
+    its slope, at most 1.13 for every activation here.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+SHIFTS = (0, 16, 4, 20, 8, 24, 12, 28)
+
+
+def unpack(w4: Tensor, scale: Tensor, zero: Tensor | None) -> Tensor:
+    """float64 [.., rows, cols] of the packed format, nibble by nibble from the bytes."""
+    b = w4.to(torch.int64).unflatten(-1, (-1, 4))
+    word = b[..., 0] + (b[..., 1] << 8) + (b[..., 2] << 16) + (b[..., 3] << 24)
+    q = torch.stack([(word >> s) & 15 for s in SHIFTS], dim=-1).flatten(-2).double()
+    group = q.shape[-1] // scale.shape[-2]
+    s = scale.double().repeat_interleave(group, dim=-2).transpose(-1, -2)
+    z = 8.0 if zero is None else (zero & 15).double().repeat_interleave(group, dim=-2).transpose(-1, -2)
+    return (q - z) * s
+
+
+def _half_step(v: Tensor, dt: torch.dtype) -> Tensor:
+    f = torch.finfo(dt)
+    return v.abs() * (f.eps / 2) + f.smallest_normal * f.eps / 2
+
+
+def product(x: Tensor, w: Tensor, group: int = 64):
+    """x w^T in 64 bits and the bound of its 32-bit sums."""
+    v = x @ w.transpose(-1, -2)
+    n = w.shape[-1]
+    steps = n / 8 + n / group + 32
+    return v, (x.abs() @ w.abs().transpose(-1, -2)) * (steps * 2.0 ** -23)
+
+
+_ACTS = {
+    "silu": torch.nn.functional.silu, "swish": torch.nn.functional.silu, "no_act": lambda v: v, "relu": torch.relu,
+    "gelu": torch.nn.functional.gelu, "sigmoid": torch.sigmoid, "tanh": torch.tanh,
+    "leaky_relu": lambda v: torch.nn.functional.leaky_relu(v, 0.01),
+}
+
+
+def hidden(x: Tensor, wg: Tensor, bg, wu: Tensor, bu, act: str, group: int = 64):
+    """act(x wg^T + bg) * (x wu^T + bu) before its rounding, and the bound."""
+    g, dg = product(x, wg, group)
+    u, du = product(x, wu, group)
+    g = g if bg is None else g + bg
+    u = u if bu is None else u + bu
+    a = _ACTS[act](g)
+    da = 1.13 * dg + a.abs() * 2.0 ** -19 + 2.0 ** -23 * g.abs()
+    return a * u, da * u.abs() + a.abs() * du + da * du + (a * u).abs() * 2.0 ** -22
+
+
+def finish(y: Tensor, dy: Tensor, bias, residual, dt: torch.dtype):
+    for t in (bias, residual):
+        if t is not None:
+            y = y + t
+            dy = dy + (y.abs() + t.abs()) * 2.0 ** -23
+    return y, dy + _half_step(y, dt)
+
+
+def linear(x, w, bias, residual, dt, group: int = 64):
+    y, dy = product(x.double(), w, group)
+    d = lambda t: None if t is None else t.double()
+    return finish(y, dy, d(bias), d(residual), dt)
+
+
+def mlp(x, wg, bg, wu, bu, wd, bd, residual, dt, act="silu", group: int = 64):
+    d = lambda t: None if t is None else t.double()
+    h, dh = hidden(x.double(), wg, d(bg), wu, d(bu), act, group)
+    dh = dh + _half_step(h, dt)
+    y, dy = product(h, wd, group)
+    return finish(y, dy + dh @ wd.abs().t(), d(bd), d(residual), dt)
+
+
+def route(x, w_router, top_k: int, renormalize: bool):
+    """(ids, weights) from 64-bit logits; equal logits: lower index first."""
+    logits = x.double() @ w_router.double().t()
+    p = torch.softmax(logits, -1)
+    ids = torch.sort(logits, dim=-1, descending=True, stable=True)[1][:, :top_k]
+    w = torch.gather(p, 1, ids)
+    return ids.to(torch.int32), (w / w.sum(1, keepdim=True) if renormalize else w)
+
+
+def moe(x, ids, weights, wg, wu, wd, residual, dt, act="silu", group: int = 64):
+    """Experts' weights in float64 ([experts, rows, cols]); ids outside the range skipped."""
+    x = x.double()
+    E, T = wg.shape[0], x.shape[0]
+    valid = (ids >= 0) & (ids < E)
+    share = torch.zeros((T, E), dtype=torch.float64, device=x.device)
+    share.scatter_add_(1, ids.long().clamp(0, E - 1), torch.where(valid, weights.double(), torch.zeros_like(weights).double()))
+    hit = torch.zeros((T, E), dtype=torch.bool, device=x.device)
+    for j in range(ids.shape[1]):
+        rows = torch.nonzero(valid[:, j])[:, 0]
+        hit[rows, ids[rows, j].long()] = True
+    top = torch.where(valid, weights.double().abs(), torch.zeros_like(weights).double()).amax(1, keepdim=True)
+    y, dy = torch.zeros_like(x), torch.zeros_like(x)
+    active = int(hit.any(0).sum())
+    for e in range(E):
+        t = torch.nonzero(hit[:, e])[:, 0]
+        if len(t) == 0:
+            continue
+        h, dh = hidden(x[t], wg[e], None, wu[e], None, act, group)
+        f = torch.where(top[t] > 0, share[t, e][:, None] / top[t], torch.zeros_like(top[t]))
+        h, dh = h * f, dh * f.abs() + (h * f).abs() * 2.0 ** -22
+        dh = dh + _half_step(h, dt)
+        y[t] += top[t] * (h @ wd[e].t())
+        # one sum over all active experts: its steps count for every part
+        steps = active * wd.shape[2] / 8 + active * wd.shape[2] / group + 32
+        dy[t] += top[t] * (dh @ wd[e].abs().t() + (h.abs() @ wd[e].abs().t()) * (steps * 2.0 ** -23))
+    return finish(y, dy + y.abs() * 2.0 ** -22, None, None if residual is None else residual.double(), dt)
+
+
+def check(got: Tensor, want: Tensor, bound: Tensor, what: str) -> None:
+    got, want, bound = got.double().cpu(), want.cpu(), bound.cpu()
+    assert got.shape == want.shape, f"{what}: shape {tuple(got.shape)} != {tuple(want.shape)}"
+    off = (got - want).abs() / bound
+    worst = float(torch.nan_to_num(off, nan=float("inf")).max()) if off.numel() else 0.0
+    assert worst <= 1.0, f"{what}: {worst:.3g} times the bound at {int(off.argmax())} ({float(got.flatten()[off.argmax()])} " \
+                         f"for {float(want.flatten()[off.argmax()])})"

@@ -1,0 +1,395 @@
+// C ABI of the few-token operators on 4-bit weights and on mixtures of experts (declared in include/gmlp.h):
+// argument checks, tensor maps and launches. No torch types, no allocation, no CPU path.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "../../include/gmlp.h"
+#include "host_util.h"
+#include "moe_stream.cuh"
+#include "w4_stream.cuh"
+
+namespace gmlp {
+
+// ----------------------------------------------------------------- scratch --
+// [slots][counters of the first kernel][counters of the second]. The slots take the size of a 64-token call whatever the
+// call is, so that the counters, which have to be zero between calls, lie behind them for every shape and calls of
+// different shapes can follow one another on one buffer.
+static size_t slots_bytes(int ctas) { return static_cast<size_t>(ctas) * 2 * 128 * FEW_MAX_TOKENS * sizeof(float); }
+struct FewLayout {
+  size_t counters1_off, counters2_off, total;
+};
+static FewLayout few_layout(int64_t K, int64_t N, int64_t experts, int ctas) {
+  FewLayout l;
+  l.counters1_off = slots_bytes(ctas);
+  l.counters2_off =
+      l.counters1_off + align_up(static_cast<size_t>((N + 127) / 128) * static_cast<size_t>(experts) * sizeof(int), 256);
+  l.total = l.counters2_off + align_up(static_cast<size_t>((K + 127) / 128) * sizeof(int), 256);
+  return l;
+}
+static int mpad_of(int64_t M) { return M <= 16 ? 16 : (M <= 32 ? 32 : 64); }
+
+// ---------------------------------------------------------------- launching --
+template <typename Kernel, typename Args>
+static int launch_stream(Kernel kfn, int grid, int threads, size_t smem, bool dependent, const CUtensorMap& m0,
+                         const CUtensorMap& m1, const CUtensorMap& mx, const Args& a, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  if (dependent) {
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+  }
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kfn, m0, m1, mx, a);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(GMLP_ERR_LAUNCH, "kernel launch: %s", cudaGetErrorString(e));
+  return GMLP_OK;
+}
+
+// One 4-bit weight matrix (of one or of all experts).
+struct W4Matrix {
+  const void* q;
+  const void* scale;
+  const void* zero;
+};
+
+static int check_w4(const W4Matrix& w) {
+  if (!w.q || !w.scale) return fail(GMLP_ERR_ARG, "NULL 4-bit weight or scale");
+  if (!aligned16(w.q)) return fail(GMLP_ERR_ALIGN, "4-bit weights must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(w.scale) & 1u) != 0) return fail(GMLP_ERR_ALIGN, "scales must be 2-byte aligned");
+  return GMLP_OK;
+}
+static int check_group(int32_t group, int64_t cols) {
+  if (group != 32 && group != 64 && group != 128)
+    return fail(GMLP_ERR_SHAPE, "group size %d: supported are 32, 64 and 128", group);
+  if (cols % group != 0)
+    return fail(GMLP_ERR_SHAPE, "%lld columns are no multiple of the group size %d", static_cast<long long>(cols), group);
+  return GMLP_OK;
+}
+
+template <int MPAD, bool DUAL, typename T>
+static int launch_w4_t(const DeviceInfo* dev, int dtype, int64_t M, int64_t rows, int64_t cols, int64_t experts,
+                       int group, const W4Matrix& w0, const W4Matrix& w1, const void* x, int64_t ldx, int64_t x_rows,
+                       const void* bias0, const void* bias1, const void* residual, void* out, float* slots,
+                       int* counters, int act, bool dependent, bool early, const MoeTable& moe, int64_t grid_units,
+                       cudaStream_t stream) {
+  CUtensorMap m0, m1, mx;
+  int rc;
+  if ((rc = encode_map(&m0, w0.q, cols / 2, experts * rows, cols / 2, 128, 128, DTYPE_U8))) return rc;
+  m1 = m0;
+  if (DUAL && (rc = encode_map(&m1, w1.q, cols / 2, experts * rows, cols / 2, 128, 128, DTYPE_U8))) return rc;
+  if ((rc = encode_map(&mx, x, cols, x_rows, ldx, 64, MPAD, dtype))) return rc;
+  W4Args a;
+  memset(&a, 0, sizeof(a));
+  a.M = static_cast<int>(M);
+  a.rows = static_cast<int>(rows);
+  a.kbt = static_cast<int>((cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
+  a.groups = static_cast<int>(cols / group);
+  a.gshift = group == 32 ? 0 : (group == 64 ? 1 : 2);
+  a.idesc = make_idesc_f16(128, MPAD, dtype == GMLP_BF16 ? 1 : 0, false, false);
+  a.status = dev->status_ptr;
+  a.scale0 = w0.scale;
+  a.scale1 = w1.scale;
+  a.zero0 = static_cast<const uint8_t*>(w0.zero);
+  a.zero1 = static_cast<const uint8_t*>(w1.zero);
+  a.bias0 = bias0;
+  a.bias1 = bias1;
+  a.residual = residual;
+  a.out = out;
+  a.slots = slots;
+  a.counters = counters;
+  a.act = act;
+  a.dependent = dependent ? 1 : 0;
+  a.early = early ? 1 : 0;
+  a.moe = moe;
+  const int grid = static_cast<int>(grid_units < dev->sm_count ? grid_units : dev->sm_count);
+  auto kfn = w4_stream_kernel<MPAD, DUAL, T>;
+  static std::atomic<uint64_t> attr_done{0};
+  if ((rc = ensure_smem_attr(kfn, w4_smem_bytes<MPAD>(), attr_done))) return rc;
+  return launch_stream(kfn, grid, w4_threads<MPAD>(), w4_smem_bytes<MPAD>(), dependent, m0, m1, mx, a, stream);
+}
+template <bool DUAL, typename... Args>
+static int launch_w4(int mpad, int dtype, const DeviceInfo* dev, Args... args) {
+  const bool bf = dtype == GMLP_BF16;
+  if (mpad == 16)
+    return bf ? launch_w4_t<16, DUAL, __nv_bfloat16>(dev, dtype, args...)
+              : launch_w4_t<16, DUAL, __half>(dev, dtype, args...);
+  if (mpad == 32)
+    return bf ? launch_w4_t<32, DUAL, __nv_bfloat16>(dev, dtype, args...)
+              : launch_w4_t<32, DUAL, __half>(dev, dtype, args...);
+  return bf ? launch_w4_t<64, DUAL, __nv_bfloat16>(dev, dtype, args...)
+            : launch_w4_t<64, DUAL, __half>(dev, dtype, args...);
+}
+
+template <int MPAD, bool DUAL, typename T>
+static int launch_moe_t(const DeviceInfo* dev, int dtype, int64_t M, int64_t rows, int64_t cols, int64_t experts,
+                        const void* w0, const void* w1, const void* x, int64_t ldx, int64_t x_rows,
+                        const void* residual, void* out, float* slots, int* counters, int act, bool early,
+                        const MoeTable& moe, int64_t grid_units, cudaStream_t stream) {
+  CUtensorMap m0, m1, mx;
+  int rc;
+  if ((rc = encode_map(&m0, w0, cols, experts * rows, cols, 64, 128, dtype))) return rc;
+  m1 = m0;
+  if (DUAL && (rc = encode_map(&m1, w1, cols, experts * rows, cols, 64, 128, dtype))) return rc;
+  if ((rc = encode_map(&mx, x, cols, x_rows, ldx, 64, MPAD, dtype))) return rc;
+  MoeArgs a;
+  memset(&a, 0, sizeof(a));
+  a.M = static_cast<int>(M);
+  a.rows = static_cast<int>(rows);
+  a.kbt = static_cast<int>(cols / 64);
+  a.idesc = make_idesc_f16(128, MPAD, dtype == GMLP_BF16 ? 1 : 0, false, false);
+  a.status = dev->status_ptr;
+  a.residual = residual;
+  a.out = out;
+  a.slots = slots;
+  a.counters = counters;
+  a.act = act;
+  a.early = early ? 1 : 0;
+  a.moe = moe;
+  const int grid = static_cast<int>(grid_units < dev->sm_count ? grid_units : dev->sm_count);
+  auto kfn = moe_stream_kernel<MPAD, DUAL, T>;
+  constexpr size_t smem = moe_smem_bytes<MPAD, DUAL>();
+  static std::atomic<uint64_t> attr_done{0};
+  if ((rc = ensure_smem_attr(kfn, smem, attr_done))) return rc;
+  return launch_stream(kfn, grid, MOE_THREADS, smem, true, m0, m1, mx, a, stream);
+}
+template <bool DUAL, typename... Args>
+static int launch_moe(int mpad, int dtype, const DeviceInfo* dev, Args... args) {
+  const bool bf = dtype == GMLP_BF16;
+  if (mpad == 16)
+    return bf ? launch_moe_t<16, DUAL, __nv_bfloat16>(dev, dtype, args...)
+              : launch_moe_t<16, DUAL, __half>(dev, dtype, args...);
+  if (mpad == 32)
+    return bf ? launch_moe_t<32, DUAL, __nv_bfloat16>(dev, dtype, args...)
+              : launch_moe_t<32, DUAL, __half>(dev, dtype, args...);
+  return bf ? launch_moe_t<64, DUAL, __nv_bfloat16>(dev, dtype, args...)
+            : launch_moe_t<64, DUAL, __half>(dev, dtype, args...);
+}
+
+static int check_few(const gmlp_problem_t* p, const char* what) {
+  int rc;
+  if ((rc = check_problem(p))) return rc;
+  if (p->dtype != GMLP_BF16 && p->dtype != GMLP_FP16) return fail(GMLP_ERR_DTYPE, "%s takes bf16 or fp16", what);
+  if (p->M > FEW_MAX_TOKENS)
+    return fail(GMLP_ERR_SHAPE, "%s takes at most 64 tokens, got %lld", what, static_cast<long long>(p->M));
+  if (p->dropout_p != 0.0f) return fail(GMLP_ERR_ARG, "%s is inference only: dropout_p must be 0", what);
+  return GMLP_OK;
+}
+static int check_experts(const gmlp_problem_t* p, int32_t experts, int32_t top_k, const void* ids, const void* weights) {
+  if (experts < 1 || experts > MOE_MAX_EXPERTS)
+    return fail(GMLP_ERR_SHAPE, "%d experts: 1 to %d are supported", experts, MOE_MAX_EXPERTS);
+  if (top_k < 1 || top_k > MOE_MAX_TOPK || top_k > experts)
+    return fail(GMLP_ERR_SHAPE, "top_k=%d: 1 to min(%d, experts) are supported", top_k, MOE_MAX_TOPK);
+  if (static_cast<int64_t>(experts) * p->N > 0x7ffffe00LL || static_cast<int64_t>(experts) * p->K > 0x7ffffe00LL)
+    return fail(GMLP_ERR_SHAPE, "experts * rows exceeds 32-bit tile coordinates");
+  if (!ids || !weights) return fail(GMLP_ERR_ARG, "NULL routing table");
+  if ((reinterpret_cast<uintptr_t>(ids) & 3u) != 0 || (reinterpret_cast<uintptr_t>(weights) & 3u) != 0)
+    return fail(GMLP_ERR_ALIGN, "the routing table must be 4-byte aligned");
+  return GMLP_OK;
+}
+static int64_t max_active(const gmlp_problem_t* p, int32_t experts, int32_t top_k) {
+  return std::min<int64_t>(experts, p->M * top_k);
+}
+
+}  // namespace gmlp
+
+using namespace gmlp;
+
+extern "C" {
+
+static int scratch_ctas() {
+  const DeviceInfo* dev;
+  return device_info(&dev) == GMLP_OK ? dev->sm_count : 256;  // without a device: an upper bound on the SM count
+}
+size_t gmlp_few_scratch_bytes(int64_t K, int64_t N, int32_t experts) {
+  if (K <= 0 || N <= 0 || experts <= 0 || experts > MOE_MAX_EXPERTS) return 0;
+  return few_layout(K, N, experts, scratch_ctas()).total;
+}
+size_t gmlp_few_scratch_counters(void) { return slots_bytes(scratch_ctas()); }
+
+int gmlp_capture_id(void* stream, uint64_t* id) {
+  if (!id) return fail(GMLP_ERR_ARG, "NULL id");
+  *id = 0;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long v = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &v);
+  if (e != cudaSuccess) return fail(GMLP_ERR_LAUNCH, "cudaStreamGetCaptureInfo: %s", cudaGetErrorString(e));
+  if (status != cudaStreamCaptureStatusNone) *id = v;
+  return GMLP_OK;
+}
+
+int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t dtype, const void* x, int64_t ldx,
+                   const void* w4, const void* scale, const void* zero, const void* bias, const void* residual,
+                   void* y, void* scratch, size_t scratch_bytes, uint32_t tuning, void* stream) {
+  int rc;
+  if (dtype != GMLP_BF16 && dtype != GMLP_FP16) return fail(GMLP_ERR_DTYPE, "the 4-bit product takes bf16 or fp16");
+  if (M < 1 || M > FEW_MAX_TOKENS)
+    return fail(GMLP_ERR_SHAPE, "the 4-bit product takes 1 to 64 tokens, got %lld", static_cast<long long>(M));
+  if (rows < 1 || cols < 1 || rows > 0x7ffffe00LL || cols > 0x7ffffe00LL)
+    return fail(GMLP_ERR_SHAPE, "rows=%lld cols=%lld out of range", static_cast<long long>(rows),
+                static_cast<long long>(cols));
+  if ((rc = check_group(group, cols))) return rc;
+  const W4Matrix w{w4, scale, zero};
+  if ((rc = check_w4(w))) return rc;
+  if ((rc = check_ptrs({x, y, scratch}))) return rc;
+  if (ldx < cols || (ldx % 8) != 0) return fail(GMLP_ERR_ALIGN, "row pitch of x must be a multiple of 8 and >= cols");
+  const DeviceInfo* dev;
+  if ((rc = device_info(&dev))) return rc;
+  const FewLayout l = few_layout(rows, rows, 1, dev->sm_count);
+  if (scratch_bytes < l.total)
+    return fail(GMLP_ERR_SCRATCH, "scratch holds %zu bytes, %zu needed", scratch_bytes, l.total);
+  char* sc = static_cast<char*>(scratch);
+  const bool dep = (tuning & (1u << 26)) == 0;  // GMLP_TUNE_ORDINARY_LAUNCH
+  const int64_t units = ((rows + 255) / 256) * ((cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
+  return launch_w4<false>(mpad_of(M), dtype, dev, M, rows, cols, int64_t{1}, group, w, w, x, ldx, M, bias,
+                          static_cast<const void*>(nullptr), residual, y, reinterpret_cast<float*>(sc),
+                          reinterpret_cast<int*>(sc + l.counters1_off), 0, dep, true, MoeTable{nullptr, nullptr, 0, 0}, units,
+                          static_cast<cudaStream_t>(stream));
+}
+
+// Both halves of a gated MLP on 4-bit weights, dense (ids == NULL) or over experts.
+static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const MoeTable& moe, int64_t active,
+                  const void* x, const W4Matrix& g, const void* b_gate, const W4Matrix& u, const void* b_up,
+                  const W4Matrix& d, const void* b_down, const void* residual, void* h, void* y, void* scratch,
+                  size_t scratch_bytes, void* stream) {
+  int rc;
+  if ((rc = check_group(group, p->K))) return rc;
+  if ((rc = check_group(group, p->N))) return rc;
+  if ((rc = check_w4(g)) || (rc = check_w4(u)) || (rc = check_w4(d))) return rc;
+  if ((rc = check_ptrs({x, h, y, scratch}))) return rc;
+  const DeviceInfo* dev;
+  if ((rc = device_info(&dev))) return rc;
+  const FewLayout l = few_layout(p->K, p->N, active, dev->sm_count);
+  if (scratch_bytes < l.total)
+    return fail(GMLP_ERR_SCRATCH, "scratch holds %zu bytes, %zu needed", scratch_bytes, l.total);
+  char* sc = static_cast<char*>(scratch);
+  float* slots = reinterpret_cast<float*>(sc);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool sparse = moe.ids != nullptr;
+  const bool dep = sparse || (p->tuning & (1u << 26)) == 0;  // GMLP_TUNE_ORDINARY_LAUNCH
+  const int64_t k_units = (p->K + W4_UNIT_COLS - 1) / W4_UNIT_COLS, n_units = (p->N + W4_UNIT_COLS - 1) / W4_UNIT_COLS;
+  rc = launch_w4<true>(mpad_of(p->M), p->dtype, dev, p->M, p->N, p->K, experts, group, g, u, x, p->K, p->M, b_gate, b_up,
+                       static_cast<const void*>(nullptr), h, slots, reinterpret_cast<int*>(sc + l.counters1_off), p->act, dep, !sparse,
+                       moe, active * ((p->N + 127) / 128) * k_units, st);
+  if (rc) return rc;
+  return launch_w4<false>(mpad_of(p->M), p->dtype, dev, p->M, p->K, p->N, experts, group, d, d,
+                          static_cast<const void*>(h), p->N, active * p->M, b_down, static_cast<const void*>(nullptr),
+                          residual, y, slots, reinterpret_cast<int*>(sc + l.counters2_off), 0, true, true, moe,
+                          active * ((p->K + 255) / 256) * n_units, st);
+}
+
+int gmlp_decode_fwd_w4(const gmlp_problem_t* p, int32_t group, const void* x, const void* w_gate4,
+                       const void* w_gate_scale, const void* w_gate_zero, const void* b_gate, const void* w_up4,
+                       const void* w_up_scale, const void* w_up_zero, const void* b_up, const void* w_down4,
+                       const void* w_down_scale, const void* w_down_zero, const void* b_down, const void* residual,
+                       void* h, void* y, void* scratch, size_t scratch_bytes, void* stream) {
+  int rc;
+  if ((rc = check_few(p, "the 4-bit decode path"))) return rc;
+  return mlp_w4(p, group, 1, MoeTable{nullptr, nullptr, 0, 0}, 1, x, {w_gate4, w_gate_scale, w_gate_zero}, b_gate,
+                {w_up4, w_up_scale, w_up_zero}, b_up, {w_down4, w_down_scale, w_down_zero}, b_down, residual, h, y,
+                scratch, scratch_bytes, stream);
+}
+
+int gmlp_moe_decode_fwd_w4(const gmlp_problem_t* p, int32_t group, int32_t experts, int32_t top_k, const void* x,
+                           const int32_t* ids, const float* weights, const void* w_gate4, const void* w_gate_scale,
+                           const void* w_gate_zero, const void* w_up4, const void* w_up_scale, const void* w_up_zero,
+                           const void* w_down4, const void* w_down_scale, const void* w_down_zero,
+                           const void* residual, void* h, void* y, void* scratch, size_t scratch_bytes, void* stream) {
+  int rc;
+  if ((rc = check_few(p, "the mixture-of-experts decode path"))) return rc;
+  if ((rc = check_experts(p, experts, top_k, ids, weights))) return rc;
+  return mlp_w4(p, group, experts, MoeTable{ids, weights, top_k, experts}, max_active(p, experts, top_k), x,
+                {w_gate4, w_gate_scale, w_gate_zero}, nullptr, {w_up4, w_up_scale, w_up_zero}, nullptr,
+                {w_down4, w_down_scale, w_down_zero}, nullptr, residual, h, y, scratch, scratch_bytes, stream);
+}
+
+int gmlp_moe_decode_fwd(const gmlp_problem_t* p, int32_t experts, int32_t top_k, const void* x, const int32_t* ids,
+                        const float* weights, const void* w_gate, const void* w_up, const void* w_down,
+                        const void* residual, void* h, void* y, void* scratch, size_t scratch_bytes, void* stream) {
+  int rc;
+  if ((rc = check_few(p, "the mixture-of-experts decode path"))) return rc;
+  if ((p->K % 64) != 0 || (p->N % 64) != 0)
+    return fail(GMLP_ERR_SHAPE, "the mixture-of-experts decode path needs K and N multiples of 64");
+  if ((rc = check_experts(p, experts, top_k, ids, weights))) return rc;
+  if ((rc = check_ptrs({x, w_gate, w_up, w_down, h, y, scratch}))) return rc;
+  const DeviceInfo* dev;
+  if ((rc = device_info(&dev))) return rc;
+  const int64_t active = max_active(p, experts, top_k);
+  const FewLayout l = few_layout(p->K, p->N, active, dev->sm_count);
+  if (scratch_bytes < l.total)
+    return fail(GMLP_ERR_SCRATCH, "scratch holds %zu bytes, %zu needed", scratch_bytes, l.total);
+  char* sc = static_cast<char*>(scratch);
+  float* slots = reinterpret_cast<float*>(sc);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const MoeTable moe{ids, weights, top_k, experts};
+  rc = launch_moe<true>(mpad_of(p->M), p->dtype, dev, p->M, p->N, p->K, static_cast<int64_t>(experts), w_gate, w_up, x, p->K,
+                        p->M, static_cast<const void*>(nullptr), h, slots, reinterpret_cast<int*>(sc + l.counters1_off), p->act, false,
+                        moe, active * ((p->N + 127) / 128) * (p->K / 64), st);
+  if (rc) return rc;
+  return launch_moe<false>(mpad_of(p->M), p->dtype, dev, p->M, p->K, p->N, static_cast<int64_t>(experts), w_down,
+                           static_cast<const void*>(nullptr), static_cast<const void*>(h), p->N, active * p->M,
+                           residual, y, slots, reinterpret_cast<int*>(sc + l.counters2_off), p->act, true, moe,
+                           active * ((p->K + 127) / 128) * (p->N / 64), st);
+}
+
+int gmlp_moe_route(int64_t M, int64_t K, int32_t experts, int32_t top_k, int32_t renormalize, int32_t dtype,
+                   const void* x, int64_t ldx, const void* w_router, int32_t* ids, float* weights, void* stream) {
+  int rc;
+  if (dtype != GMLP_BF16 && dtype != GMLP_FP16) return fail(GMLP_ERR_DTYPE, "the router takes bf16 or fp16");
+  if (M < 1 || M > 0xffffffLL || K < 1 || K > 0x7ffffff0LL || (K % 8) != 0)
+    return fail(GMLP_ERR_SHAPE, "the router needs 1 <= M < 2^24 and K a positive multiple of 8; got M=%lld K=%lld",
+                static_cast<long long>(M), static_cast<long long>(K));
+  if (experts < 1 || experts > MOE_MAX_EXPERTS)
+    return fail(GMLP_ERR_SHAPE, "%d experts: 1 to %d are supported", experts, MOE_MAX_EXPERTS);
+  if (top_k < 1 || top_k > MOE_MAX_TOPK || top_k > experts)
+    return fail(GMLP_ERR_SHAPE, "top_k=%d: 1 to min(%d, experts) are supported", top_k, MOE_MAX_TOPK);
+  if ((rc = check_ptrs({x, w_router}))) return rc;
+  if (ldx < K || (ldx % 8) != 0) return fail(GMLP_ERR_ALIGN, "row pitch of x must be a multiple of 8 and >= K");
+  if (!ids || !weights) return fail(GMLP_ERR_ARG, "NULL routing table");
+  if ((reinterpret_cast<uintptr_t>(ids) & 3u) != 0 || (reinterpret_cast<uintptr_t>(weights) & 3u) != 0)
+    return fail(GMLP_ERR_ALIGN, "the routing table must be 4-byte aligned");
+  const DeviceInfo* dev;
+  if ((rc = device_info(&dev))) return rc;
+  RouteArgs a;
+  a.x = x;
+  a.w = w_router;
+  a.ldx = ldx;
+  a.K = static_cast<int>(K);
+  a.E = experts;
+  a.top_k = top_k;
+  a.renormalize = renormalize ? 1 : 0;
+  a.ids = ids;
+  a.weights = weights;
+  // one warp per expert at a time; up to eight blocks a token
+  int cluster = 1;
+  while (cluster < 8 && cluster * (ROUTE_THREADS / 32) < experts) cluster *= 2;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(M * cluster));
+  cfg.blockDim = dim3(ROUTE_THREADS);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = dtype == GMLP_BF16 ? cudaLaunchKernelEx(&cfg, moe_route_kernel<__nv_bfloat16>, a)
+                                     : cudaLaunchKernelEx(&cfg, moe_route_kernel<__half>, a);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(GMLP_ERR_LAUNCH, "kernel launch: %s", cudaGetErrorString(e));
+  return GMLP_OK;
+}
+
+}  // extern "C"

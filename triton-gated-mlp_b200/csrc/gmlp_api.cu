@@ -15,13 +15,14 @@
 #include "decode_fused.cuh"
 #include "elementwise.cuh"
 #include "gemm_tcgen05.cuh"
+#include "host_util.h"
 #include "peer_reduce.cuh"
 
 namespace gmlp {
 
 // ------------------------------------------------------------------ errors --
 static thread_local char g_err[512] = "";
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -32,12 +33,6 @@ static int fail(int code, const char* fmt, ...) {
 // Per-device status word written by kernels that give up a bounded wait.
 __device__ int g_dev_status;
 
-struct DeviceInfo {
-  std::atomic<bool> ready{false};
-  int sm_count = 0;
-  int cc_major = 0;
-  int* status_ptr = nullptr;
-};
 static DeviceInfo g_dev[64];
 static std::mutex g_mu;
 
@@ -47,7 +42,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 static EncodeTiledFn g_encode = nullptr;
 
-static int device_info(const DeviceInfo** out) {
+int device_info(const DeviceInfo** out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return fail(GMLP_ERR_LAUNCH, "cudaGetDevice: %s", cudaGetErrorString(e));
@@ -128,15 +123,14 @@ static uint32_t map_hash(const MapKey& k) {
   return static_cast<uint32_t>(h >> 40) % MAP_CACHE_SLOTS;
 }
 
-constexpr int DTYPE_U8 = 100;  // internal: one-byte elements (e4m3 operands of the 8-bit decode path)
 static unsigned dtype_bytes(int dtype) { return dtype == DTYPE_U8 ? 1u : dtype == GMLP_F32 ? 4u : 2u; }
 
 // 2-D row-major matrix [outer, inner] of 16-bit (DTYPE_U8: 8-bit, GMLP_F32: 32-bit) elements, swizzled rows of
 // `swizzle_bytes` (32 / 64 / 128), out-of-bounds elements read as zero and are not
 // written by stores.
-static int encode_map(CUtensorMap* m, const void* base, int64_t inner, int64_t outer,
-                      int64_t pitch_elems, uint32_t box_inner, uint32_t box_outer, int dtype,
-                      int swizzle_bytes = 128) {
+int encode_map(CUtensorMap* m, const void* base, int64_t inner, int64_t outer,
+               int64_t pitch_elems, uint32_t box_inner, uint32_t box_outer, int dtype,
+               int swizzle_bytes) {
   const MapKey key{base, inner, outer, pitch_elems, box_inner, box_outer, dtype, swizzle_bytes};
   MapSlot& slot = g_map_cache[map_hash(key)];
   if (slot.used && slot.key == key) {
@@ -168,8 +162,6 @@ static int encode_map(CUtensorMap* m, const void* base, int64_t inner, int64_t o
   slot.used = true;
   return GMLP_OK;
 }
-
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // One operand of C = A B^T as it lies in memory.
 struct Operand {
@@ -245,22 +237,6 @@ static Tuning resolve_tuning(uint32_t word) {
 static int64_t gemm_cta_budget(int sm_count, int sm_limit) {
   int64_t b = (sm_limit > 0 && sm_limit < sm_count) ? sm_limit : sm_count;
   return b < 2 ? 2 : b;
-}
-
-// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per (kernel, device) instead of
-// before every launch.
-template <typename K>
-static int ensure_smem_attr(K kfn, size_t smem, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (done.load(std::memory_order_acquire) & bit) return GMLP_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
-  if (e != cudaSuccess)
-    return fail(GMLP_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  done.fetch_or(bit, std::memory_order_release);
-  return GMLP_OK;
 }
 
 template <int BN, bool A_MN, bool B_MN, int EPI, typename T, bool ASUM>
@@ -435,7 +411,7 @@ static int launch_gemm(const DeviceInfo* dev, int dtype, int64_t M, int64_t N, c
                                                           ep, tuning_word, stream);
 }
 
-static int check_problem(const gmlp_problem_t* p) {
+int check_problem(const gmlp_problem_t* p) {
   if (!p) return fail(GMLP_ERR_ARG, "NULL problem descriptor");
   if (p->dtype != GMLP_BF16 && p->dtype != GMLP_FP16 && p->dtype != GMLP_F32)
     return fail(GMLP_ERR_DTYPE, "dtype %d is not a gmlp_dtype_t", p->dtype);
@@ -481,7 +457,7 @@ static DropoutParams make_dropout(const gmlp_problem_t* p) {
   return d;
 }
 
-static int check_ptrs(std::initializer_list<const void*> ps) {
+int check_ptrs(std::initializer_list<const void*> ps) {
   for (const void* q : ps) {
     if (!q) return fail(GMLP_ERR_ARG, "NULL pointer argument");
     if (!aligned16(q)) return fail(GMLP_ERR_ALIGN, "pointer %p is not 16-byte aligned", q);
@@ -1044,8 +1020,6 @@ int gmlp_colsum(int64_t rows, int64_t cols, int32_t dtype, const void* src, int6
 }  // extern "C"
 
 // ------------------------------------------------------------------ decode --
-static size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
-
 struct DecodeLayout {
   int mpad;
   size_t counters1_off, counters2_off, sync_off, slots_off, total;

@@ -1,0 +1,421 @@
+// The experts of a mixture layer for up to 64 tokens on 16-bit weights: gate/up (DUAL = true) and down (DUAL = false).
+// The scheme (active experts, zero-padded hidden rows, one long reduction) is in few_token.cuh; the weight path is the
+// one of the dense decode kernel (decode_stream.cuh): 128 weight rows x 64 columns per tile through a deep TMA ring,
+// tokens as the N dimension of tcgen05.mma, stream-K over units. HBM-bound: every byte of the active experts once.
+//   DUAL   units = (active expert, row tile of N, 64 columns of K), two tiles (gate, up) a unit; all M tokens are
+//          multiplied (the tensor pipe has the time, see MPAD there) and the epilogue keeps the chosen ones
+//   !DUAL  units = (row tile of the hidden size, (active expert, 64 columns of N)): one accumulator for all experts
+#pragma once
+#include "few_token.cuh"
+
+namespace gmlp {
+
+struct MoeArgs {
+  int M;
+  int rows;  // weight rows per expert: N for DUAL, K (hidden) otherwise
+  int kbt;   // 64-wide reduction blocks per expert
+  uint32_t idesc;
+  int* status;
+  const void* residual;  // [M][rows] or null (DUAL = false)
+  void* out;             // DUAL: H[active][M][rows]; else Y[M][rows]
+  float* slots;
+  int* counters;
+  int act;
+  int early;  // weights may be streamed before the preceding kernel has finished (the down kernel)
+  MoeTable moe;
+};
+
+constexpr int MOE_THREADS = 192;
+template <int MPAD, bool DUAL>
+__host__ __device__ constexpr int moe_stage_bytes() {
+  return (DUAL ? 2 : 1) * 16384 + MPAD * 128;
+}
+template <int MPAD, bool DUAL>
+__host__ __device__ constexpr int moe_stages() {
+  constexpr int fit = (232448 - 1024 - 4096) / moe_stage_bytes<MPAD, DUAL>();
+  return fit > 12 ? 12 : fit;
+}
+template <int MPAD, bool DUAL>
+constexpr size_t moe_smem_bytes() {
+  return static_cast<size_t>(moe_stages<MPAD, DUAL>()) * moe_stage_bytes<MPAD, DUAL>() + 1024;
+}
+
+template <int MPAD, bool DUAL, typename T>
+__global__ void __launch_bounds__(MOE_THREADS, 1)
+moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant__ CUtensorMap tmW1,
+                  const __grid_constant__ CUtensorMap tmX, const MoeArgs args) {
+  constexpr int NACC = DUAL ? 2 : 1;
+  constexpr int STAGES = moe_stages<MPAD, DUAL>();
+  constexpr uint32_t W_BYTES = 16384;
+  constexpr uint32_t X_OFF = NACC * W_BYTES;
+  constexpr uint32_t STAGE_BYTES = moe_stage_bytes<MPAD, DUAL>();
+  constexpr uint32_t ACC_COLS = NACC * MPAD;
+  constexpr uint32_t TMEM_COLS = 2 * ACC_COLS <= 32 ? 32 : 2 * ACC_COLS <= 64 ? 64 : 2 * ACC_COLS <= 128 ? 128 : 256;
+
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[2 * STAGES + 5];
+  __shared__ uint32_t tmem_base_holder;
+  __shared__ int abort_flag;
+  __shared__ MoeShared moe;
+
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bar_base = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+  auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
+  auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };
+  const uint32_t drain_bar = bar_base + 8u * (2 * STAGES + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), 4);
+    }
+    mbar_init(drain_bar, 1);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(&tmW0);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_base_holder), TMEM_COLS);
+    tmem_relinquish();
+  }
+  // The routing table comes from an earlier kernel. The gate/up kernel waits for that kernel before it lets its own
+  // dependent start, so the down kernel may read the table (and stream weights) at once.
+  if (!args.early) pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  tc_fence_before_sync();
+  moe_collect(args.moe, args.M, moe);  // ends with a block barrier
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_base_holder;
+  volatile int* abortp = &abort_flag;
+
+  const int row_tiles = (args.rows + 127) / 128;
+  const long long per_tile = DUAL ? args.kbt : static_cast<long long>(moe.n) * args.kbt;
+  const long long total = per_tile * (DUAL ? static_cast<long long>(moe.n) * row_tiles : row_tiles);
+  const long long ctas = total < gridDim.x ? total : gridDim.x;
+  const long long u_begin = blockIdx.x < ctas ? unit_start(blockIdx.x, total, ctas) : 0;
+  const long long u_end = blockIdx.x < ctas ? unit_start(blockIdx.x + 1, total, ctas) : 0;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA --
+    if (lane == 0 && u_begin < u_end) {
+      const uint64_t pol_w = l2_policy_evict_first();
+      const uint64_t pol_x = l2_policy_evict_last();
+      struct Pos {
+        int a, rt, kb;
+      };
+      auto pos_at = [&](long long u) {
+        Pos p;
+        const long long tile = u / per_tile, r = u - tile * per_tile;
+        if (DUAL) {
+          p.a = static_cast<int>(tile / row_tiles);
+          p.rt = static_cast<int>(tile - static_cast<long long>(p.a) * row_tiles);
+          p.kb = static_cast<int>(r);
+        } else {
+          p.rt = static_cast<int>(tile);
+          p.a = static_cast<int>(r / args.kbt);
+          p.kb = static_cast<int>(r - static_cast<long long>(p.a) * args.kbt);
+        }
+        return p;
+      };
+      auto step = [&](Pos& p) {  // unit by unit: no 64-bit division in the issuing thread's loop
+        if (++p.kb < args.kbt) return;
+        p.kb = 0;
+        if (DUAL) {
+          if (++p.rt == row_tiles) {
+            p.rt = 0;
+            ++p.a;
+          }
+        } else {
+          if (++p.a == moe.n) {
+            p.a = 0;
+            ++p.rt;
+          }
+        }
+      };
+      Pos pw = pos_at(u_begin), px = pw;
+      auto load_w = [&](int st) {
+        const int y = moe.list[pw.a] * args.rows + pw.rt * 128;
+        const uint32_t sw = smem_base + st * STAGE_BYTES;
+        mbar_expect_tx(full_bar(st), STAGE_BYTES);
+        tma_load_2d_hint(sw, &tmW0, full_bar(st), pw.kb * 64, y, pol_w);
+        if (DUAL) tma_load_2d_hint(sw + W_BYTES, &tmW1, full_bar(st), pw.kb * 64, y, pol_w);
+        step(pw);
+      };
+      auto load_x = [&](int st) {
+        tma_load_2d_hint(smem_base + st * STAGE_BYTES + X_OFF, &tmX, full_bar(st), px.kb * 64,
+                         DUAL ? 0 : px.a * args.M, pol_x);
+        step(px);
+      };
+      long long u = u_begin;
+      if (args.early) {
+        const long long n0 = (u_end - u_begin) < STAGES ? (u_end - u_begin) : STAGES;
+        for (int i = 0; i < n0; ++i) load_w(i);
+        pdl_wait();
+        for (int i = 0; i < n0; ++i) load_x(i);
+        u += n0;
+      }
+      int st = static_cast<int>((u - u_begin) % STAGES);
+      uint32_t ph = static_cast<uint32_t>((u - u_begin) / STAGES) & 1u;
+      bool ok = true;
+      for (; u < u_end; ++u) {
+        if (!mbar_wait(empty_bar(st), ph ^ 1u, abortp)) {
+          ok = false;
+          break;
+        }
+        load_w(st);
+        load_x(st);
+        if (++st == STAGES) {
+          st = 0;
+          ph ^= 1u;
+        }
+      }
+      if (!ok) {
+        abort_flag = 1;
+        atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_PRODUCER);
+        const long long done = u - u_begin;  // see the copies in flight land before the block leaves
+        for (long long i = done > STAGES ? done - STAGES : 0; i < done; ++i)
+          drain_wait(full_bar(static_cast<int>(i % STAGES)), static_cast<uint32_t>(i / STAGES) & 1u);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA --
+    if (lane == 0) {
+      int st = 0, seg = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      long long u = u_begin;
+      while (u < u_end && ok) {
+        const Segment s = segment_at(u, u_end, per_tile);
+        const int acc = seg & 1;
+        if (!(ok = mbar_wait(tempty_bar(acc), ((seg >> 1) & 1u) ^ 1u, abortp))) break;
+        tc_fence_after_sync();
+        const uint32_t d = tmem_base + acc * ACC_COLS;
+        uint32_t accum = 0u;
+        for (; u < s.end; ++u) {
+          if (!(ok = mbar_wait(full_bar(st), ph, abortp))) break;
+          tc_fence_after_sync();
+          const uint32_t sw = smem_base + st * STAGE_BYTES;
+          const uint64_t xd = make_smem_desc(sw + X_OFF, 16, 1024);
+          const uint64_t w0 = make_smem_desc(sw, 16, 1024), w1 = make_smem_desc(sw + W_BYTES, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            umma_f16(d, w0 + static_cast<uint64_t>(2 * k), xd + static_cast<uint64_t>(2 * k), args.idesc, accum);
+            if (DUAL)
+              umma_f16(d + MPAD, w1 + static_cast<uint64_t>(2 * k), xd + static_cast<uint64_t>(2 * k), args.idesc, accum);
+            accum = 1u;
+          }
+          umma_commit(empty_bar(st));
+          if (++st == STAGES) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) umma_commit(tfull_bar(acc));
+        ++seg;
+      }
+      if (!ok) {
+        abort_flag = 1;
+        atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_MMA);
+        umma_commit(drain_bar);
+        drain_wait(drain_bar, 0);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue --
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const int ep_tid = threadIdx.x - 64;
+    if (args.early) pdl_wait();  // slots, counters and outputs may still be in use by the preceding grid
+    T* const out = static_cast<T*>(args.out);
+    const T* const res = static_cast<const T*>(args.residual);
+    const long long ld = args.rows;
+    if (!DUAL && total == 0) {
+      // no token chose any expert: the outputs are the residual, or zero
+      const long long all = static_cast<long long>(args.M) * args.rows;
+      for (long long i = blockIdx.x * 128LL + ep_tid; i < all; i += gridDim.x * 128LL)
+        out[i] = res ? res[i] : static_cast<T>(0.f);
+    }
+    int seg = 0;
+    long long u = u_begin;
+    while (u < u_end) {
+      const Segment s = segment_at(u, u_end, per_tile);
+      const int acc = seg & 1;
+      const int a = DUAL ? static_cast<int>(s.tile / row_tiles) : 0;
+      const int rt = static_cast<int>(DUAL ? s.tile - static_cast<long long>(a) * row_tiles : s.tile);
+      if (DUAL) moe_factors(args.moe, args.M, moe.list[a], ep_tid, moe);  // seen behind the next barrier
+      if (!mbar_wait_warp(tfull_bar(acc), (seg >> 1) & 1u, abortp, lane) && lane == 0) {
+        abort_flag = 1;
+        atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_EPILOGUE);
+      }
+      tc_fence_after_sync();
+      float v[NACC][MPAD];
+#pragma unroll
+      for (int t = 0; t < NACC; ++t)
+#pragma unroll
+        for (int c = 0; c < MPAD / 16; ++c) {
+          uint32_t r[16];
+          tmem_ld_32x16(tmem_base + acc * ACC_COLS + lane_addr + t * MPAD + c * 16, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[t][c * 16 + i] = __uint_as_float(r[i]);
+        }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty_bar(acc));
+      const Split sp{total,       ctas,   args.slots, args.counters,
+                     args.status, abortp, smem_base,  static_cast<int>(STAGES * STAGE_BYTES / (128 * 16))};
+      const int what = settle_segment<NACC, MPAD, MPAD, 128>(v, s, sp, args.M, 0, row, ep_tid);
+      if (what == SETTLE_ABORT) break;
+      const int wrow = rt * 128 + row;
+      if (what == SETTLE_EMIT && wrow < args.rows) {
+        if (DUAL)
+          store_hidden<MPAD>(args.act, out + static_cast<long long>(a) * args.M * ld + wrow, ld, args.M, 0, v[0],
+                             v[NACC - 1], 0.f, 0.f, &moe);
+        else
+          store_product<MPAD>(out + wrow, res ? res + wrow : nullptr, ld, args.M, 0, v[0], 0.f, &moe);
+      }
+      if (DUAL) named_bar_sync(1, 128);  // f and hit are overwritten for the next tile
+      u = s.end;
+      ++seg;
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---- router ----
+// logits l[t][e] = x_t . Wr_e; p = softmax(l); the top_k largest (equal ones: lowest index first; NaN ranks lowest) with
+// weights p, or p divided by their sum. A cluster of C blocks per token: each takes E / C experts, a warp per expert
+// and pass, products exact in fp32, eight of them summed in fp32 and added to an fp64 sum, so that the order of the
+// logits (a choice next to a border) is that of the exact sums but for a relative 1e-7. The logits go to the first
+// block's shared memory (distributed shared memory), whose first warp selects. Latency-bound: C spreads the 2 E K bytes
+// of a token over SMs, since one SM draws about 100 GB/s per resident warp group.
+constexpr int ROUTE_THREADS = 256;
+struct RouteArgs {
+  const void* x;
+  const void* w;
+  long long ldx;
+  int K, E, top_k, renormalize;
+  int* ids;
+  float* weights;
+};
+__device__ __forceinline__ unsigned long long sort_key(double v) {
+  if (v != v) return 1ull;  // NaN: above a removed entry (0), below -inf
+  const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
+  return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+}
+template <typename T>
+__global__ void __launch_bounds__(ROUTE_THREADS)
+moe_route_kernel(const RouteArgs args) {
+  __shared__ double logits[MOE_MAX_EXPERTS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t rank, size;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+  const long long token = blockIdx.x / size;
+  pdl_launch_dependents();
+  pdl_wait();
+  const T* const x = static_cast<const T*>(args.x) + token * args.ldx;
+  const int e0 = static_cast<int>(static_cast<long long>(args.E) * rank / size);
+  const int e1 = static_cast<int>(static_cast<long long>(args.E) * (rank + 1) / size);
+  const uint32_t dst0 = mapa_shared(smem_u32(logits), 0);
+  for (int e = e0 + warp; e < e1; e += ROUTE_THREADS / 32) {
+    const T* const w = static_cast<const T*>(args.w) + static_cast<long long>(e) * args.K;
+    double sum = 0.0;
+#pragma unroll 8
+    for (int k = lane * 8; k < args.K; k += 256) {
+      float a[8], b[8];
+      load8(x + k, a);
+      load8(w + k, b);
+      float s = a[0] * b[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) s = fmaf(a[i], b[i], s);
+      sum += static_cast<double>(s);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0)
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst0 + 8u * e), "d"(sum) : "memory");
+  }
+  __syncwarp();
+  cluster_sync_all();
+  if (rank != 0 || warp != 0) return;
+  constexpr int PER = MOE_MAX_EXPERTS / 32;
+  unsigned long long key[PER];
+  float ex[PER];
+  double top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = i * 32 + lane;
+    const double l = e < args.E ? logits[e] : 0.0;
+    key[i] = e < args.E ? sort_key(l) : 0ull;
+    if (e < args.E && !(l <= top)) top = l;  // a NaN becomes the maximum and makes every weight of the token NaN
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double v = __shfl_xor_sync(0xffffffffu, top, o);
+    if (v > top || v != v) top = v;
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = i * 32 + lane;
+    ex[i] = e < args.E ? expf(static_cast<float>(logits[e] - top)) : 0.f;
+    sum += ex[i];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  float mine = 0.f, chosen = 0.f;  // lane j keeps choice j
+  int id = 0;
+  for (int j = 0; j < args.top_k; ++j) {
+    unsigned long long best = 0ull;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] > best) {  // ascending index inside a lane: the first of equals stays
+        best = key[i];
+        at = i;
+      }
+    const uint32_t hi = static_cast<uint32_t>(best >> 32), lo = static_cast<uint32_t>(best);
+    const uint32_t mhi = __reduce_max_sync(0xffffffffu, hi);
+    const uint32_t mlo = __reduce_max_sync(0xffffffffu, hi == mhi ? lo : 0u);
+    const uint32_t e = __reduce_min_sync(
+        0xffffffffu, (hi == mhi && lo == mlo) ? static_cast<uint32_t>(at * 32 + lane) : 0xffffffffu);
+    float w = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (static_cast<uint32_t>(i * 32 + lane) == e) {
+        w = ex[i];
+        key[i] = 0ull;
+      }
+    w = __shfl_sync(0xffffffffu, w, e & 31u);
+    chosen += w;
+    if (lane == j) {
+      mine = w;
+      id = static_cast<int>(e);
+    }
+  }
+  if (lane < args.top_k) {
+    args.ids[token * args.top_k + lane] = id;
+    args.weights[token * args.top_k + lane] = mine / (args.renormalize ? chosen : sum);
+  }
+}
+
+}  // namespace gmlp

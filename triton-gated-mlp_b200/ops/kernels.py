@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
@@ -524,6 +525,343 @@ def decode_fwd_fp8(x: Tensor, w_gate8: Tensor, w_gate_scale: Tensor, b_gate: Ten
                                          ptr(w_up_scale), ptr(b_up), ptr(w_down8), ptr(w_down_scale), ptr(b_down),
                                          ptr(residual), ptr(x8), ptr(xs), ptr(h), ptr(h8), ptr(hs), ptr(y), ptr(scratch),
                                          scratch.numel() * scratch.element_size(), stream_of(x)))
+    return y
+
+
+# ---- up to 64 tokens on 4-bit weights, and on mixtures of experts ----
+
+INT4_SHIFTS = (0, 16, 4, 20, 8, 24, 12, 28)   # bit of column 8j + c in 32-bit word j of a row
+INT4_GROUPS = (32, 64, 128)
+
+
+class Int4Weight(NamedTuple):
+    """A matrix [.., rows, cols] in the library's 4-bit format (include/gmlp.h): w = (q - zero) * scale.
+
+    w4     uint8 [.., rows, cols / 2]: little-endian 32-bit words, column 8j + c of word j at bit INT4_SHIFTS[c]
+    scale  [.., cols / group, rows] in the activations' type; the group size (32, 64 or 128) follows from the shapes
+    zero   uint8 [.., cols / group, rows], values 0..15, or None for 8 everywhere"""
+
+    w4: Tensor
+    scale: Tensor
+    zero: Tensor | None = None
+
+
+def quantize_weight_int4(w: Tensor, group: int = 128, symmetric: bool = False) -> Int4Weight:
+    """One-off preparation of a 16-bit weight matrix [.., rows, cols] for the 4-bit paths: per row and group of `group`
+    columns the range of its values is divided into 16 steps (symmetric=True: steps around zero, no zero points).
+    Plain torch ops: this runs when weights are loaded, not per step."""
+    if group not in INT4_GROUPS:
+        raise ValueError(f"group size {group}: supported are {INT4_GROUPS}")
+    if w.shape[-1] % group:
+        raise ValueError(f"{w.shape[-1]} columns are no multiple of the group size {group}")
+    if w.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"4-bit weights are made from bfloat16 or float16 matrices, got {w.dtype}")
+    v = w.detach().float().unflatten(-1, (-1, group))
+    if symmetric:
+        scale = (v.abs().amax(-1) / 7.5).clamp_min(2.0 ** -24).to(w.dtype)
+        zero = None
+    else:
+        lo, hi = v.amin(-1).clamp_max(0), v.amax(-1).clamp_min(0)
+        scale = ((hi - lo) / 15).clamp_min(2.0 ** -24).to(w.dtype)
+        zero = (-lo / scale.float()).round().clamp(0, 15)
+    q = (v / scale.float()[..., None]).round()
+    q = (q + (8 if zero is None else zero[..., None])).clamp_(0, 15).to(torch.int32).flatten(-2)
+    shifts = torch.tensor(INT4_SHIFTS, dtype=torch.int32, device=w.device)
+    words = (q.unflatten(-1, (-1, 8)) << shifts).sum(-1).to(torch.int32)
+    return Int4Weight(words.view(torch.uint8), scale.transpose(-1, -2).contiguous(),
+                      None if zero is None else zero.to(torch.uint8).transpose(-1, -2).contiguous())
+
+
+def dequantize_weight_int4(w: Int4Weight) -> Tensor:
+    """The float32 matrix [.., rows, cols] that `w` stands for (exact)."""
+    shifts = torch.tensor(INT4_SHIFTS, dtype=torch.int32, device=w.w4.device)
+    q = ((w.w4.view(torch.int32)[..., None] >> shifts) & 15).flatten(-2).float()
+    scale = w.scale.transpose(-1, -2).float()
+    zero = 8.0 if w.zero is None else (w.zero & 15).transpose(-1, -2).float()[..., None]
+    return ((q.unflatten(-1, (scale.shape[-1], -1)) - zero) * scale[..., None]).flatten(-2)
+
+
+def _int4_group(w: Int4Weight, lead: tuple, rows: int, cols: int, dt: torch.dtype, dev: torch.device) -> int:
+    """Checks a 4-bit weight against the shape it must have; returns its group size."""
+    q, s, z = w
+    groups = s.shape[-2] if s.dim() >= 2 else 0
+    if (q.dtype is not torch.uint8 or q.shape != (*lead, rows, cols // 2) or q.device != dev or not q.is_contiguous()
+            or cols % 8):
+        raise ValueError(f"4-bit weights must be contiguous uint8 of shape {(*lead, rows, cols // 2)} on {dev}; got "
+                         f"{q.dtype} {tuple(q.shape)} on {q.device}")
+    group = cols // groups if groups else 0
+    if group not in INT4_GROUPS or groups * group != cols:
+        raise ValueError(f"4-bit weights of {cols} columns need cols / group scales per row with group in "
+                         f"{INT4_GROUPS}; got scales of shape {tuple(s.shape)}")
+    if s.dtype is not dt or s.shape != (*lead, groups, rows) or s.device != dev or not s.is_contiguous():
+        raise ValueError(f"scales must be contiguous {dt} of shape {(*lead, groups, rows)} on {dev}; got {s.dtype} "
+                         f"{tuple(s.shape)} on {s.device}")
+    if z is not None and (z.dtype is not torch.uint8 or z.shape != s.shape or z.device != dev
+                          or not z.is_contiguous()):
+        raise ValueError(f"zeros must be contiguous uint8 of shape {tuple(s.shape)} on {dev}")
+    return group
+
+
+_few_scratch: dict = {}
+
+
+def few_scratch(K: int, N: int, experts: int, device: torch.device) -> Tensor:
+    """Zero-initialised scratch for the 4-bit and mixture-of-experts calls, for callers that keep their own."""
+    with torch.cuda.device(device):
+        nbytes = load().gmlp_few_scratch_bytes(K, N, experts)
+    return torch.zeros((nbytes,), dtype=torch.uint8, device=device)
+
+
+def _scratch_for(K: int, N: int, experts: int, dev: torch.device, stream: int) -> Tensor:
+    """The scratch of calls without one of their own: one buffer per (device, stream), since calls on a stream are
+    ordered, and one per graph capture, cleared inside the graph: no two graphs, and no graph and an eager call, ever
+    share counters. A new buffer is made when a kernel has given up a wait since (its counters may be dirty)."""
+    cap = 0
+    if torch.cuda.is_current_stream_capturing():
+        v = C.c_uint64(0)
+        check(load().gmlp_capture_id(stream, C.byref(v)))
+        cap = v.value
+    key = (dev.index, stream, cap != 0)
+    tag = (cap, _lib.scratch_epoch())
+    need = (-(-N // 128)) * experts * 4 + (-(-K // 128)) * 4 + 512
+    have = _few_scratch.get(key)
+    if have is None or have[0] != tag or have[1] < need:
+        if len(_few_scratch) > 32:
+            _few_scratch.clear()
+        lib = load()
+        room = need if cap else max(need, 1 << 16)   # eager buffers serve calls of many shapes
+        slots = lib.gmlp_few_scratch_counters()
+        buf = torch.empty((slots + room,), dtype=torch.uint8, device=dev)
+        buf[slots:].zero_()
+        have = _few_scratch[key] = (tag, room, buf)
+    return have[2]
+
+
+def _rows_of(x: Tensor) -> Tensor:
+    """x with contiguous rows on 16-byte boundaries (a copy where the caller's view has neither)."""
+    x = _c(x)
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def _few_common(x: Tensor, dt: torch.dtype, what: str) -> None:
+    if x.dim() != 2:
+        raise ValueError(f"{what} takes x of shape [tokens, columns], got {tuple(x.shape)}")
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise NotImplementedError(f"{what} computes in bfloat16 or float16; got {dt}")
+    if x.shape[0] > DECODE_MAX_TOKENS:
+        raise ValueError(f"{what} takes at most {DECODE_MAX_TOKENS} tokens, got {x.shape[0]}")
+
+
+def _vector(b: Tensor | None, n: int, name: str) -> Tensor | None:
+    if b is None:
+        return None
+    if b.shape != (n,):
+        raise ValueError(f"{name} must have shape ({n},), got {tuple(b.shape)}")
+    return _c(b)
+
+
+def _like(r: Tensor | None, shape: tuple, name: str) -> Tensor | None:
+    if r is None:
+        return None
+    if r.shape != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(r.shape)}")
+    return _c(r)
+
+
+def linear_w4(x: Tensor, w: Int4Weight, bias: Tensor | None = None, residual: Tensor | None = None,
+              scratch: Tensor | None = None, ordinary_launch: bool = False) -> Tensor:
+    """y = x W^T (+ bias) (+ residual) for at most 64 tokens on 4-bit weights with group scales (Int4Weight
+    [rows, cols]; any number of rows). The kernel normally starts streaming weights while the preceding kernel on the
+    stream is still running; ordinary_launch=True makes it wait first (for the call that follows a kernel which
+    writes the weights)."""
+    dev = require_cuda(x, w[0], w[1], w[2], bias, residual)
+    dt = _same_dtype(x, bias, residual)
+    _few_common(x, dt, "linear_w4")
+    M, K = x.shape
+    if w[0].dim() != 2:
+        raise ValueError(f"linear_w4 takes one matrix [rows, cols], got 4-bit weights of shape {tuple(w[0].shape)}")
+    N = w[0].shape[0]
+    group = _int4_group(w, (), N, K, dt, dev)
+    bias, residual = _vector(bias, N, "bias"), _like(residual, (M, N), "residual")
+    y = torch.empty((M, N), dtype=dt, device=dev)
+    if M == 0 or N == 0:
+        return y
+    ldx = K
+    if M > 1 and x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= K and x.data_ptr() % 16 == 0:
+        ldx = x.stride(0)
+    else:
+        x = _rows_of(x)
+    with _on(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if scratch is None:
+            scratch = _scratch_for(N, N, 1, dev, stream)
+        check(load().gmlp_w4_linear(M, N, K, group, dtype_code(dt), x.data_ptr(), ldx, w[0].data_ptr(),
+                                    w[1].data_ptr(), ptr(w[2]), ptr(bias), ptr(residual), y.data_ptr(),
+                                    scratch.data_ptr(), scratch.numel() * scratch.element_size(),
+                                    (1 << 26) if ordinary_launch else 0, stream))
+    return y
+
+
+def decode_w4_supported(M: int, K: int, N: int, group: int) -> bool:
+    return 0 < M <= DECODE_MAX_TOKENS and group in INT4_GROUPS and K % group == 0 and N % group == 0
+
+
+def decode_fwd_w4(x: Tensor, w_gate: Int4Weight, b_gate: Tensor | None, w_up: Int4Weight, b_up: Tensor | None,
+                  w_down: Int4Weight, b_down: Tensor | None, scratch: Tensor | None = None, act: str = "silu",
+                  residual: Tensor | None = None, ordinary_launch: bool = False) -> Tensor:
+    """decode_fwd on 4-bit weights with group scales (quantize_weight_int4); x, biases, residual and the result stay
+    16-bit, the hidden state is rounded to 16 bits between the two kernels as in decode_fwd. All three matrices share
+    one group size."""
+    dev = require_cuda(x, *w_gate, b_gate, *w_up, b_up, *w_down, b_down, residual)
+    dt = _same_dtype(x, b_gate, b_up, b_down, residual)
+    _few_common(x, dt, "decode_fwd_w4")
+    M, K = x.shape
+    N = w_gate[0].shape[0]
+    group = _int4_group(w_gate, (), N, K, dt, dev)
+    if _int4_group(w_up, (), N, K, dt, dev) != group or _int4_group(w_down, (), K, N, dt, dev) != group:
+        raise ValueError("gate, up and down weights must have one group size")
+    b_gate, b_up, b_down = _vector(b_gate, N, "b_gate"), _vector(b_up, N, "b_up"), _vector(b_down, K, "b_down")
+    residual = _like(residual, (M, K), "residual")
+    y = torch.empty((M, K), dtype=dt, device=dev)
+    if M == 0:
+        return y
+    x = _rows_of(x)
+    h = torch.empty((M, N), dtype=dt, device=dev)
+    prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act, (1 << 26) if ordinary_launch else 0)
+    with _on(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if scratch is None:
+            scratch = _scratch_for(K, N, 1, dev, stream)
+        check(load().gmlp_decode_fwd_w4(
+            C.byref(prob), group, x.data_ptr(), w_gate[0].data_ptr(), w_gate[1].data_ptr(), ptr(w_gate[2]), ptr(b_gate),
+            w_up[0].data_ptr(), w_up[1].data_ptr(), ptr(w_up[2]), ptr(b_up), w_down[0].data_ptr(), w_down[1].data_ptr(),
+            ptr(w_down[2]), ptr(b_down), ptr(residual), h.data_ptr(), y.data_ptr(), scratch.data_ptr(),
+            scratch.numel() * scratch.element_size(), stream))
+    return y
+
+
+MOE_MAX_EXPERTS = 512
+MOE_MAX_TOP_K = 32
+
+
+def moe_route(x: Tensor, w_router: Tensor, top_k: int, renormalize: bool = True):
+    """The router of a mixture of experts: (ids int32 [M, top_k], weights float32 [M, top_k]) with ids the experts of
+    the top_k largest logits x w_router^T ([experts, K]) in descending order (equal ones: lower index first) and
+    weights their softmax probabilities, divided by their sum when `renormalize`. Any number of tokens."""
+    dev = require_cuda(x, w_router)
+    dt = _same_dtype(x, w_router)
+    if x.dim() != 2 or w_router.dim() != 2 or x.shape[1] != w_router.shape[1]:
+        raise ValueError(f"moe_route takes x [tokens, K] and w_router [experts, K]; got {tuple(x.shape)} and "
+                         f"{tuple(w_router.shape)}")
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise NotImplementedError(f"moe_route computes in bfloat16 or float16; got {dt}")
+    M, K = x.shape
+    E = w_router.shape[0]
+    if not 1 <= E <= MOE_MAX_EXPERTS:
+        raise ValueError(f"{E} experts: 1 to {MOE_MAX_EXPERTS} are supported")
+    if not 1 <= top_k <= min(E, MOE_MAX_TOP_K):
+        raise ValueError(f"top_k={top_k}: 1 to {min(E, MOE_MAX_TOP_K)} are supported for {E} experts")
+    ids = torch.empty((M, top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((M, top_k), dtype=torch.float32, device=dev)
+    if M == 0:
+        return ids, weights
+    x, w_router = _rows_of(x), _rows_of(w_router)
+    with _on(dev):
+        check(load().gmlp_moe_route(M, K, E, top_k, 1 if renormalize else 0, dtype_code(dt), x.data_ptr(), K,
+                                    w_router.data_ptr(), ids.data_ptr(), weights.data_ptr(),
+                                    torch.cuda.current_stream(dev).cuda_stream))
+    return ids, weights
+
+
+def _moe_table(x: Tensor, ids: Tensor, weights: Tensor, experts: int):
+    M = x.shape[0]
+    if ids.dim() != 2 or ids.shape[0] != M or ids.dtype is not torch.int32:
+        raise ValueError(f"ids must be int32 of shape [{M}, top_k], got {ids.dtype} {tuple(ids.shape)}")
+    if weights.shape != ids.shape or weights.dtype is not torch.float32:
+        raise ValueError(f"weights must be float32 of shape {tuple(ids.shape)}, got {weights.dtype} "
+                         f"{tuple(weights.shape)}")
+    if not 1 <= experts <= MOE_MAX_EXPERTS:
+        raise ValueError(f"{experts} experts: 1 to {MOE_MAX_EXPERTS} are supported")
+    k = ids.shape[1]
+    if not 1 <= k <= min(experts, MOE_MAX_TOP_K):
+        raise ValueError(f"top_k={k}: 1 to {min(experts, MOE_MAX_TOP_K)} are supported for {experts} experts")
+    return _c(ids), _c(weights), k
+
+
+def moe_decode_supported(M: int, K: int, N: int, experts: int) -> bool:
+    return 0 < M <= DECODE_MAX_TOKENS and K % 64 == 0 and N % 64 == 0 and 0 < experts <= MOE_MAX_EXPERTS
+
+
+def moe_decode_fwd(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
+                   act: str = "silu", residual: Tensor | None = None, scratch: Tensor | None = None) -> Tensor:
+    """y[t] = sum_j weights[t, j] * MLP_e(x[t]) (+ residual[t]), e = ids[t, j], for at most 64 tokens, with
+    MLP_e(x) = (act(x w_gate[e]^T) * (x w_up[e]^T)) w_down[e]^T; w_gate / w_up [experts, N, K], w_down [experts, K, N].
+    ids and weights come from moe_route or from a router of the caller's: an id outside [0, experts) is skipped (-1
+    marks padding), a repeated one adds. Only the experts that some token chose are read."""
+    dev = require_cuda(x, ids, weights, w_gate, w_up, w_down, residual)
+    dt = _same_dtype(x, w_gate, w_up, w_down, residual)
+    _few_common(x, dt, "moe_decode_fwd")
+    M, K = x.shape
+    if w_gate.dim() != 3:
+        raise ValueError(f"w_gate must have shape [experts, N, K], got {tuple(w_gate.shape)}")
+    E, N = w_gate.shape[0], w_gate.shape[1]
+    if w_gate.shape != (E, N, K) or w_up.shape != (E, N, K) or w_down.shape != (E, K, N):
+        raise ValueError(f"w_gate, w_up must be [experts, N, {K}] and w_down [experts, {K}, N]; got "
+                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
+    ids, weights, k = _moe_table(x, ids, weights, E)
+    residual = _like(residual, (M, K), "residual")
+    y = torch.empty((M, K), dtype=dt, device=dev)
+    if M == 0:
+        return y
+    if not moe_decode_supported(M, K, N, E):
+        raise ValueError(f"the mixture-of-experts decode path needs K and N multiples of 64; got K={K} N={N}")
+    x, w_gate, w_up, w_down = _rows_of(x), _c(w_gate), _c(w_up), _c(w_down)
+    active = min(E, M * k)
+    h = torch.empty((active, M, N), dtype=dt, device=dev)
+    prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act)
+    with _on(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if scratch is None:
+            scratch = _scratch_for(K, N, active, dev, stream)
+        check(load().gmlp_moe_decode_fwd(
+            C.byref(prob), E, k, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+            w_down.data_ptr(), ptr(residual), h.data_ptr(), y.data_ptr(), scratch.data_ptr(),
+            scratch.numel() * scratch.element_size(), stream))
+    return y
+
+
+def moe_decode_fwd_w4(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Int4Weight, w_up: Int4Weight,
+                      w_down: Int4Weight, act: str = "silu", residual: Tensor | None = None,
+                      scratch: Tensor | None = None) -> Tensor:
+    """moe_decode_fwd on 4-bit experts: Int4Weight matrices with a leading [experts] dimension, one group size."""
+    dev = require_cuda(x, ids, weights, *w_gate, *w_up, *w_down, residual)
+    dt = _same_dtype(x, residual)
+    _few_common(x, dt, "moe_decode_fwd_w4")
+    M, K = x.shape
+    if w_gate[0].dim() != 3:
+        raise ValueError(f"4-bit experts must have shape [experts, N, K / 2], got {tuple(w_gate[0].shape)}")
+    E, N = w_gate[0].shape[0], w_gate[0].shape[1]
+    group = _int4_group(w_gate, (E,), N, K, dt, dev)
+    if _int4_group(w_up, (E,), N, K, dt, dev) != group or _int4_group(w_down, (E,), K, N, dt, dev) != group:
+        raise ValueError("gate, up and down weights must have one group size")
+    ids, weights, k = _moe_table(x, ids, weights, E)
+    residual = _like(residual, (M, K), "residual")
+    y = torch.empty((M, K), dtype=dt, device=dev)
+    if M == 0:
+        return y
+    x = _rows_of(x)
+    active = min(E, M * k)
+    h = torch.empty((active, M, N), dtype=dt, device=dev)
+    prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act)
+    with _on(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if scratch is None:
+            scratch = _scratch_for(K, N, active, dev, stream)
+        check(load().gmlp_moe_decode_fwd_w4(
+            C.byref(prob), group, E, k, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate[0].data_ptr(),
+            w_gate[1].data_ptr(), ptr(w_gate[2]), w_up[0].data_ptr(), w_up[1].data_ptr(), ptr(w_up[2]),
+            w_down[0].data_ptr(), w_down[1].data_ptr(), ptr(w_down[2]), ptr(residual), h.data_ptr(), y.data_ptr(),
+            scratch.data_ptr(), scratch.numel() * scratch.element_size(), stream))
     return y
 
 
