@@ -320,12 +320,14 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
  *   w4     rows of cols / 2 bytes: little-endian 32-bit words, word j holding columns 8j .. 8j+7, column 8j + c at
  *          bit (0, 16, 4, 20, 8, 24, 12, 28)[c]; 16-byte aligned
  *   scale  [cols / group, rows];  zero [cols / group, rows], or NULL for zero = 8 everywhere
- * A group's products are summed in fp32 with the integers q - zero and then multiplied by its scale: the weights
- * are never rounded.
+ * The weights are never rounded: a group's products with the integers q are summed in fp32 and then take zero and scale.
+ * Activations enter as sums of two (bf16) or three (fp16) e4m3 numbers under a power of two per token and group,
+ * which is off by at most 2^-17 of the group's largest activation, and not at all for those within 2^-9 (bf16) or
+ * 2^-6 (fp16) of it. A NaN or infinite activation makes its token's outputs NaN, and no other token's.
  *
  * gmlp_w4_linear: y[m,r] = sum_c x[m,c] w[r,c] (+ bias[r]) (+ residual[m,r]) for 1 <= M <= 64 and any rows >= 1; x
  *   has row pitch ldx (a multiple of 8), y and residual [M, rows] are contiguous.
- * gmlp_decode_fwd_w4: gmlp_decode_fwd with three such matrices (K and N multiples of group); two launches.
+ * gmlp_decode_fwd_w4: gmlp_decode_fwd with three such matrices (K and N multiples of group).
  * Both start streaming weights before the preceding kernel on the stream has finished, with the precondition and
  * the GMLP_TUNE_ORDINARY_LAUNCH way out of gmlp_decode_fwd.
  *
@@ -343,6 +345,8 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
  * gmlp_moe_decode_fwd_w4: the same on 4-bit experts (w4 [experts, rows, cols / 2], scale / zero
  *   [experts, cols / group, rows]); K and N multiples of group.
  *
+ * `work` (4-bit calls): gmlp_w4_work_bytes(M, K, N, experts, group, dtype) bytes of any content, 16-byte aligned, for the
+ *   hidden state and the activations' terms (gmlp_w4_linear: K = cols, N = 0, experts = 1).
  * `scratch`: gmlp_few_scratch_bytes(K, N, experts) bytes (gmlp_w4_linear: K = N = rows, experts = 1; mixtures:
  *   experts = min(experts, M * top_k) or more), 16-byte aligned. What lies behind its first
  *   gmlp_few_scratch_counters() bytes must be ZERO before the first call; every call leaves it zero, unless
@@ -350,14 +354,16 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
  *   enough for may use a buffer one after the other; calls that share one must not overlap on the GPU. */
 size_t gmlp_few_scratch_bytes(int64_t K, int64_t N, int32_t experts);
 size_t gmlp_few_scratch_counters(void);
+size_t gmlp_w4_work_bytes(int64_t M, int64_t K, int64_t N, int32_t experts, int32_t group, int32_t dtype);
 int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t dtype, const void* x, int64_t ldx,
                    const void* w4, const void* scale, const void* zero, const void* bias, const void* residual,
-                   void* y, void* scratch, size_t scratch_bytes, uint32_t tuning, void* stream);
+                   void* y, void* work, size_t work_bytes, void* scratch, size_t scratch_bytes, uint32_t tuning,
+                   void* stream);
 int gmlp_decode_fwd_w4(const gmlp_problem_t* p, int32_t group, const void* x, const void* w_gate4,
                        const void* w_gate_scale, const void* w_gate_zero, const void* b_gate, const void* w_up4,
                        const void* w_up_scale, const void* w_up_zero, const void* b_up, const void* w_down4,
                        const void* w_down_scale, const void* w_down_zero, const void* b_down, const void* residual,
-                       void* h, void* y, void* scratch, size_t scratch_bytes, void* stream);
+                       void* y, void* work, size_t work_bytes, void* scratch, size_t scratch_bytes, void* stream);
 int gmlp_moe_route(int64_t M, int64_t K, int32_t experts, int32_t top_k, int32_t renormalize, int32_t dtype,
                    const void* x, int64_t ldx, const void* w_router, int32_t* ids, float* weights, void* stream);
 int gmlp_moe_decode_fwd(const gmlp_problem_t* p, int32_t experts, int32_t top_k, const void* x, const int32_t* ids,
@@ -367,7 +373,8 @@ int gmlp_moe_decode_fwd_w4(const gmlp_problem_t* p, int32_t group, int32_t exper
                            const int32_t* ids, const float* weights, const void* w_gate4, const void* w_gate_scale,
                            const void* w_gate_zero, const void* w_up4, const void* w_up_scale, const void* w_up_zero,
                            const void* w_down4, const void* w_down_scale, const void* w_down_zero,
-                           const void* residual, void* h, void* y, void* scratch, size_t scratch_bytes, void* stream);
+                           const void* residual, void* y, void* work, size_t work_bytes, void* scratch,
+                           size_t scratch_bytes, void* stream);
 /* *id = 0, or the identity of the graph capture that `stream` is in: a host keys scratch buffers on it, so that
  * two captured graphs never share one. */
 int gmlp_capture_id(void* stream, uint64_t* id);

@@ -8,6 +8,8 @@ The bounds count, term by term,
   * 32-bit sums: each addition is off by at most 2^-23 of the sum of magnitudes S = sum |w| |x| so far (the tensor
     core may truncate, hence 2^-23 and not 2^-24); a sum of n columns in groups of G takes at most n / 16 steps of the
     matrix instruction (16 columns each, counted as 2 additions) and n / G of the group sums, and at most 32 joins;
+  * 4-bit products only: an activation enters as a sum of e4m3 numbers that is off by at most 2^-17 of the largest
+    activation of its token and group;
   * the gate activation in 32 bits: 2^-19 relative (exp and division of the fast kind, each below 2^-21), and
     its slope, at most 1.13 for every activation here.
 """
@@ -35,12 +37,23 @@ def _half_step(v: Tensor, dt: torch.dtype) -> Tensor:
     return v.abs() * (f.eps / 2) + f.smallest_normal * f.eps / 2
 
 
-def product(x: Tensor, w: Tensor, group: int = 64):
-    """x w^T in 64 bits and the bound of its 32-bit sums."""
+def _largest(x: Tensor, group: int) -> Tensor:
+    """|x| of every element replaced by the largest of its group of columns."""
+    return x.abs().unflatten(-1, (-1, group)).amax(-1, keepdim=True).expand(*x.shape[:-1], -1, group).flatten(-2)
+
+
+def product(x: Tensor, w: Tensor, group: int = 0):
+    """x w^T in 64 bits and the bound of its 32-bit sums (group > 0: on 4-bit weights with that group size). A 4-bit
+    product adds up q and takes the zero point off at the end: its magnitudes are up to (15 + 15) scale, where the
+    group's largest |w| is at least 7.5 scale (weights made by a quantiser that uses the range): 4 times that."""
     v = x @ w.transpose(-1, -2)
     n = w.shape[-1]
-    steps = n / 8 + n / group + 32
-    return v, (x.abs() @ w.abs().transpose(-1, -2)) * (steps * 2.0 ** -23)
+    steps = n / 8 + (n / group if group else 0) + 32
+    if not group:
+        return v, (x.abs() @ w.abs().transpose(-1, -2)) * (steps * 2.0 ** -23)
+    size = 4 * _largest(w, group)
+    return v, (x.abs() @ size.transpose(-1, -2)) * (steps * 2.0 ** -23) + \
+        (_largest(x, group) @ w.abs().transpose(-1, -2)) * 2.0 ** -17
 
 
 _ACTS = {
@@ -50,7 +63,7 @@ _ACTS = {
 }
 
 
-def hidden(x: Tensor, wg: Tensor, bg, wu: Tensor, bu, act: str, group: int = 64):
+def hidden(x: Tensor, wg: Tensor, bg, wu: Tensor, bu, act: str, group: int = 0):
     """act(x wg^T + bg) * (x wu^T + bu) before its rounding, and the bound."""
     g, dg = product(x, wg, group)
     u, du = product(x, wu, group)
@@ -69,13 +82,13 @@ def finish(y: Tensor, dy: Tensor, bias, residual, dt: torch.dtype):
     return y, dy + _half_step(y, dt)
 
 
-def linear(x, w, bias, residual, dt, group: int = 64):
+def linear(x, w, bias, residual, dt, group: int = 0):
     y, dy = product(x.double(), w, group)
     d = lambda t: None if t is None else t.double()
     return finish(y, dy, d(bias), d(residual), dt)
 
 
-def mlp(x, wg, bg, wu, bu, wd, bd, residual, dt, act="silu", group: int = 64):
+def mlp(x, wg, bg, wu, bu, wd, bd, residual, dt, act="silu", group: int = 0):
     d = lambda t: None if t is None else t.double()
     h, dh = hidden(x.double(), wg, d(bg), wu, d(bu), act, group)
     dh = dh + _half_step(h, dt)
@@ -92,7 +105,7 @@ def route(x, w_router, top_k: int, renormalize: bool):
     return ids.to(torch.int32), (w / w.sum(1, keepdim=True) if renormalize else w)
 
 
-def moe(x, ids, weights, wg, wu, wd, residual, dt, act="silu", group: int = 64):
+def moe(x, ids, weights, wg, wu, wd, residual, dt, act="silu", group: int = 0):
     """Experts' weights in float64 ([experts, rows, cols]); ids outside the range skipped."""
     x = x.double()
     E, T = wg.shape[0], x.shape[0]
@@ -116,8 +129,8 @@ def moe(x, ids, weights, wg, wu, wd, residual, dt, act="silu", group: int = 64):
         dh = dh + _half_step(h, dt)
         y[t] += top[t] * (h @ wd[e].t())
         # one sum over all active experts: its steps count for every part
-        steps = active * wd.shape[2] / 8 + active * wd.shape[2] / group + 32
-        dy[t] += top[t] * (dh @ wd[e].abs().t() + (h.abs() @ wd[e].abs().t()) * (steps * 2.0 ** -23))
+        own = product(h, wd[e], group)[1]
+        dy[t] += top[t] * (dh @ wd[e].abs().t() + own * active)
     return finish(y, dy + y.abs() * 2.0 ** -22, None, None if residual is None else residual.double(), dt)
 
 

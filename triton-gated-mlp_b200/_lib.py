@@ -25,7 +25,7 @@ EXPORTS = (
     "gmlp_down_fwd", "gmlp_mlp_fwd", "gmlp_mlp_bwd", "gmlp_bwd_dhidden", "gmlp_bwd_dact", "gmlp_bwd_dx",
     "gmlp_bwd_dw_gate_up", "gmlp_bwd_dw_down", "gmlp_bias_grad_scratch_bytes", "gmlp_bwd_dw_gate_up_bias",
     "gmlp_bwd_dw_down_bias", "gmlp_colsum_scratch_bytes", "gmlp_colsum", "gmlp_colsum_static",
-    "gmlp_few_scratch_bytes", "gmlp_few_scratch_counters", "gmlp_w4_linear", "gmlp_decode_fwd_w4", "gmlp_moe_route",
+    "gmlp_few_scratch_bytes", "gmlp_few_scratch_counters", "gmlp_w4_work_bytes", "gmlp_w4_linear", "gmlp_decode_fwd_w4", "gmlp_moe_route",
     "gmlp_moe_decode_fwd", "gmlp_moe_decode_fwd_w4", "gmlp_capture_id",
     "gmlp_dropout_mask", "gmlp_gemm", "gmlp_decode_scratch_bytes", "gmlp_decode_fwd", "gmlp_set_cta_pair_mode", "gmlp_set_raster_group", "gmlp_set_sm_limit",
     "gmlp_peer_region_bytes", "gmlp_set_peer_two_shot_bytes", "gmlp_peer_alloc", "gmlp_peer_open", "gmlp_peer_close", "gmlp_peer_free",
@@ -83,12 +83,14 @@ def _declare(lib: C.CDLL) -> None:
     lib.gmlp_few_scratch_bytes.restype = C.c_size_t
     lib.gmlp_few_scratch_counters.argtypes = []
     lib.gmlp_few_scratch_counters.restype = C.c_size_t
-    lib.gmlp_w4_linear.argtypes = [i64, i64, i64, i32, i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, C.c_uint32,
-                                   vp]
-    lib.gmlp_decode_fwd_w4.argtypes = [pp, i32] + [vp] * 17 + [C.c_size_t, vp]
+    lib.gmlp_w4_linear.argtypes = [i64, i64, i64, i32, i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp,
+                                   C.c_size_t, C.c_uint32, vp]
+    lib.gmlp_w4_work_bytes.argtypes = [i64, i64, i64, i32, i32, i32]
+    lib.gmlp_w4_work_bytes.restype = C.c_size_t
+    lib.gmlp_decode_fwd_w4.argtypes = [pp, i32] + [vp] * 16 + [C.c_size_t, vp, C.c_size_t, vp]
     lib.gmlp_moe_route.argtypes = [i64, i64, i32, i32, i32, i32, vp, i64, vp, vp, vp, vp]
     lib.gmlp_moe_decode_fwd.argtypes = [pp, i32, i32] + [vp] * 10 + [C.c_size_t, vp]
-    lib.gmlp_moe_decode_fwd_w4.argtypes = [pp, i32, i32, i32] + [vp] * 16 + [C.c_size_t, vp]
+    lib.gmlp_moe_decode_fwd_w4.argtypes = [pp, i32, i32, i32] + [vp] * 15 + [C.c_size_t, vp, C.c_size_t, vp]
     lib.gmlp_capture_id.argtypes = [vp, C.POINTER(C.c_uint64)]
     lib.gmlp_dropout_mask.argtypes = [pp, u8p, vp]
     lib.gmlp_gemm.argtypes = [i32, i32, i32, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp, vp]

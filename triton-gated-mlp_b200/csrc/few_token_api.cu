@@ -64,7 +64,8 @@ struct W4Matrix {
 static int check_w4(const W4Matrix& w) {
   if (!w.q || !w.scale) return fail(GMLP_ERR_ARG, "NULL 4-bit weight or scale");
   if (!aligned16(w.q)) return fail(GMLP_ERR_ALIGN, "4-bit weights must be 16-byte aligned");
-  if ((reinterpret_cast<uintptr_t>(w.scale) & 1u) != 0) return fail(GMLP_ERR_ALIGN, "scales must be 2-byte aligned");
+  if (((reinterpret_cast<uintptr_t>(w.scale) | reinterpret_cast<uintptr_t>(w.zero)) & 3u) != 0)
+    return fail(GMLP_ERR_ALIGN, "scales and zeros must be 4-byte aligned");
   return GMLP_OK;
 }
 static int check_group(int32_t group, int64_t cols) {
@@ -75,58 +76,130 @@ static int check_group(int32_t group, int64_t cols) {
   return GMLP_OK;
 }
 
-template <int MPAD, bool DUAL, typename T>
-static int launch_w4_t(const DeviceInfo* dev, int dtype, int64_t M, int64_t rows, int64_t cols, int64_t experts,
-                       int group, const W4Matrix& w0, const W4Matrix& w1, const void* x, int64_t ldx, int64_t x_rows,
-                       const void* bias0, const void* bias1, const void* residual, void* out, float* slots,
-                       int* counters, int act, bool dependent, bool early, const MoeTable& moe, int64_t grid_units,
-                       cudaStream_t stream) {
+// Work buffer of a 4-bit call: [hidden state][activation terms][their meta data]. The terms of x and, later, of the
+// hidden state take turns in one place.
+static int w4_mt(int64_t M) { return M <= 8 ? 8 : (M <= 16 ? 16 : (M <= 32 ? 32 : 64)); }
+struct W4Work {
+  size_t t8_off, meta_off, total;
+};
+static size_t w4_t8_bytes(int64_t rows, int64_t cols, int dtype) {
+  return static_cast<size_t>(dtype == GMLP_BF16 ? w4_terms<__nv_bfloat16>() : w4_terms<__half>()) * rows * cols;
+}
+// K columns of x (M rows); N columns of h (active * M rows), N = 0 for a plain product
+static W4Work w4_work(int64_t M, int64_t K, int64_t N, int64_t active, int group, int dtype) {
+  W4Work w;
+  w.t8_off = align_up(static_cast<size_t>(active * M * N) * 2, 256);
+  w.meta_off = w.t8_off + align_up(std::max(w4_t8_bytes(M, K, dtype), w4_t8_bytes(active * M, N, dtype)), 256);
+  w.total = w.meta_off + static_cast<size_t>(std::max(K / group, active * (N / group))) * 2 * w4_mt(M) * sizeof(float);
+  return w;
+}
+
+// Activations as e4m3 terms (see w4_stream.cuh).
+static int launch_split(int64_t M, int64_t R, int64_t cols, int64_t ldx, int group, int dtype, const void* x, void* t8,
+                        void* meta, bool dependent, cudaStream_t stream) {
+  W4SplitArgs a;
+  a.x = x;
+  a.ldx = ldx;
+  a.R = R;
+  a.M = static_cast<int>(M);
+  a.MT = w4_mt(M);
+  a.cols = static_cast<int>(cols);
+  a.gshift = group == 32 ? 0 : (group == 64 ? 1 : 2);
+  a.t8 = static_cast<uint8_t*>(t8);
+  a.meta = static_cast<float*>(meta);
+  a.dependent = dependent ? 1 : 0;
+  const int64_t items = R * ((cols + W4_HALF_COLS - 1) / W4_HALF_COLS);
+  const int64_t per_block = W4_SPLIT_THREADS / 16;
+  const int64_t blocks = (items + per_block - 1) / per_block;
+  if (blocks > 0x7fffffffLL) return fail(GMLP_ERR_SHAPE, "too many activations");
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(W4_SPLIT_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  if (dependent) {
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+  }
+  cudaError_t e = dtype == GMLP_BF16 ? cudaLaunchKernelEx(&cfg, w4_split_kernel<__nv_bfloat16>, a)
+                                     : cudaLaunchKernelEx(&cfg, w4_split_kernel<__half>, a);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(GMLP_ERR_LAUNCH, "kernel launch: %s", cudaGetErrorString(e));
+  return GMLP_OK;
+}
+
+// What every instantiation of the stream kernel is launched with.
+struct W4Call {
+  int dtype;
+  int64_t M, rows, cols, experts, R;
+  int group;
+  W4Matrix w0, w1;
+  const void *t8, *meta;
+  const void *bias0, *bias1, *residual;
+  void* out;
+  float* slots;
+  int* counters;
+  int act;
+  bool early;
+  MoeTable moe;
+  int64_t max_units;
+  cudaStream_t stream;
+};
+template <int MT, bool DUAL, typename T>
+static int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
+  using Conf = W4Conf<MT, w4_terms<T>()>;
   CUtensorMap m0, m1, mx;
   int rc;
-  if ((rc = encode_map(&m0, w0.q, cols / 2, experts * rows, cols / 2, 128, 128, DTYPE_U8))) return rc;
+  if ((rc = encode_map(&m0, c.w0.q, c.cols / 2, c.experts * c.rows, c.cols / 2, 128, 128, DTYPE_U8))) return rc;
   m1 = m0;
-  if (DUAL && (rc = encode_map(&m1, w1.q, cols / 2, experts * rows, cols / 2, 128, 128, DTYPE_U8))) return rc;
-  if ((rc = encode_map(&mx, x, cols, x_rows, ldx, 64, MPAD, dtype))) return rc;
+  if (DUAL && (rc = encode_map(&m1, c.w1.q, c.cols / 2, c.experts * c.rows, c.cols / 2, 128, 128, DTYPE_U8))) return rc;
+  if ((rc = encode_map(&mx, c.t8, c.cols, w4_terms<T>() * c.R, c.cols, 128, MT, DTYPE_U8))) return rc;
   W4Args a;
   memset(&a, 0, sizeof(a));
-  a.M = static_cast<int>(M);
-  a.rows = static_cast<int>(rows);
-  a.kbt = static_cast<int>((cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
-  a.groups = static_cast<int>(cols / group);
-  a.gshift = group == 32 ? 0 : (group == 64 ? 1 : 2);
-  a.idesc = make_idesc_f16(128, MPAD, dtype == GMLP_BF16 ? 1 : 0, false, false);
+  a.M = static_cast<int>(c.M);
+  a.rows = static_cast<int>(c.rows);
+  a.kbt = static_cast<int>((c.cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
+  a.groups = static_cast<int>(c.cols / c.group);
+  a.gshift = c.group == 32 ? 0 : (c.group == 64 ? 1 : 2);
+  // an accumulator buffer holds as many groups of a half unit as leave room for a second buffer
+  a.gpg = 4 >> a.gshift;
+  while (a.gpg > 1 && a.gpg * Conf::N > 128) a.gpg >>= 1;
+  a.acc_bufs = std::min(Conf::MAX_ACC_BUFS, Conf::C_COLS / (a.gpg * Conf::N));
+  a.R = c.R;
+  a.idesc = make_idesc_f8(128, Conf::N);
   a.status = dev->status_ptr;
-  a.scale0 = w0.scale;
-  a.scale1 = w1.scale;
-  a.zero0 = static_cast<const uint8_t*>(w0.zero);
-  a.zero1 = static_cast<const uint8_t*>(w1.zero);
-  a.bias0 = bias0;
-  a.bias1 = bias1;
-  a.residual = residual;
-  a.out = out;
-  a.slots = slots;
-  a.counters = counters;
-  a.act = act;
-  a.dependent = dependent ? 1 : 0;
-  a.early = early ? 1 : 0;
-  a.moe = moe;
-  const int grid = static_cast<int>(grid_units < dev->sm_count ? grid_units : dev->sm_count);
-  auto kfn = w4_stream_kernel<MPAD, DUAL, T>;
+  a.meta = static_cast<const float*>(c.meta);
+  a.scale0 = static_cast<const uint16_t*>(c.w0.scale);
+  a.scale1 = static_cast<const uint16_t*>(c.w1.scale);
+  a.zero0 = static_cast<const uint8_t*>(c.w0.zero);
+  a.zero1 = static_cast<const uint8_t*>(c.w1.zero);
+  a.bias0 = c.bias0;
+  a.bias1 = c.bias1;
+  a.residual = c.residual;
+  a.out = c.out;
+  a.slots = c.slots;
+  a.counters = c.counters;
+  a.act = c.act;
+  a.early = c.early ? 1 : 0;
+  a.moe = c.moe;
+  const int grid = static_cast<int>(c.max_units < dev->sm_count ? c.max_units : dev->sm_count);
+  auto kfn = w4_stream_kernel<MT, DUAL, T>;
   static std::atomic<uint64_t> attr_done{0};
-  if ((rc = ensure_smem_attr(kfn, w4_smem_bytes<MPAD>(), attr_done))) return rc;
-  return launch_stream(kfn, grid, w4_threads<MPAD>(), w4_smem_bytes<MPAD>(), dependent, m0, m1, mx, a, stream);
+  if ((rc = ensure_smem_attr(kfn, Conf::SMEM, attr_done))) return rc;
+  return launch_stream(kfn, grid, Conf::THREADS, Conf::SMEM, true, m0, m1, mx, a, c.stream);
 }
-template <bool DUAL, typename... Args>
-static int launch_w4(int mpad, int dtype, const DeviceInfo* dev, Args... args) {
-  const bool bf = dtype == GMLP_BF16;
-  if (mpad == 16)
-    return bf ? launch_w4_t<16, DUAL, __nv_bfloat16>(dev, dtype, args...)
-              : launch_w4_t<16, DUAL, __half>(dev, dtype, args...);
-  if (mpad == 32)
-    return bf ? launch_w4_t<32, DUAL, __nv_bfloat16>(dev, dtype, args...)
-              : launch_w4_t<32, DUAL, __half>(dev, dtype, args...);
-  return bf ? launch_w4_t<64, DUAL, __nv_bfloat16>(dev, dtype, args...)
-            : launch_w4_t<64, DUAL, __half>(dev, dtype, args...);
+template <bool DUAL>
+static int launch_w4(const DeviceInfo* dev, const W4Call& c) {
+  const bool bf = c.dtype == GMLP_BF16;
+  switch (w4_mt(c.M)) {
+    case 8: return bf ? launch_w4_t<8, DUAL, __nv_bfloat16>(dev, c) : launch_w4_t<8, DUAL, __half>(dev, c);
+    case 16: return bf ? launch_w4_t<16, DUAL, __nv_bfloat16>(dev, c) : launch_w4_t<16, DUAL, __half>(dev, c);
+    case 32: return bf ? launch_w4_t<32, DUAL, __nv_bfloat16>(dev, c) : launch_w4_t<32, DUAL, __half>(dev, c);
+    default: return bf ? launch_w4_t<64, DUAL, __nv_bfloat16>(dev, c) : launch_w4_t<64, DUAL, __half>(dev, c);
+  }
 }
 
 template <int MPAD, bool DUAL, typename T>
@@ -226,9 +299,16 @@ int gmlp_capture_id(void* stream, uint64_t* id) {
   return GMLP_OK;
 }
 
+size_t gmlp_w4_work_bytes(int64_t M, int64_t K, int64_t N, int32_t experts, int32_t group, int32_t dtype) {
+  if (M <= 0 || M > FEW_MAX_TOKENS || K <= 0 || N < 0 || experts <= 0 || (group != 32 && group != 64 && group != 128))
+    return 0;
+  return w4_work(M, K, N, experts, group, dtype).total;
+}
+
 int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t dtype, const void* x, int64_t ldx,
                    const void* w4, const void* scale, const void* zero, const void* bias, const void* residual,
-                   void* y, void* scratch, size_t scratch_bytes, uint32_t tuning, void* stream) {
+                   void* y, void* work, size_t work_bytes, void* scratch, size_t scratch_bytes, uint32_t tuning,
+                   void* stream) {
   int rc;
   if (dtype != GMLP_BF16 && dtype != GMLP_FP16) return fail(GMLP_ERR_DTYPE, "the 4-bit product takes bf16 or fp16");
   if (M < 1 || M > FEW_MAX_TOKENS)
@@ -239,76 +319,134 @@ int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t
   if ((rc = check_group(group, cols))) return rc;
   const W4Matrix w{w4, scale, zero};
   if ((rc = check_w4(w))) return rc;
-  if ((rc = check_ptrs({x, y, scratch}))) return rc;
+  if ((rc = check_ptrs({x, y, work, scratch}))) return rc;
   if (ldx < cols || (ldx % 8) != 0) return fail(GMLP_ERR_ALIGN, "row pitch of x must be a multiple of 8 and >= cols");
   const DeviceInfo* dev;
   if ((rc = device_info(&dev))) return rc;
   const FewLayout l = few_layout(rows, rows, 1, dev->sm_count);
   if (scratch_bytes < l.total)
     return fail(GMLP_ERR_SCRATCH, "scratch holds %zu bytes, %zu needed", scratch_bytes, l.total);
-  char* sc = static_cast<char*>(scratch);
+  const W4Work ww = w4_work(M, cols, 0, 1, group, dtype);
+  if (work_bytes < ww.total) return fail(GMLP_ERR_SCRATCH, "work holds %zu bytes, %zu needed", work_bytes, ww.total);
+  char* const wk = static_cast<char*>(work);
+  char* const sc = static_cast<char*>(scratch);
   const bool dep = (tuning & (1u << 26)) == 0;  // GMLP_TUNE_ORDINARY_LAUNCH
-  const int64_t units = ((rows + 255) / 256) * ((cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
-  return launch_w4<false>(mpad_of(M), dtype, dev, M, rows, cols, int64_t{1}, group, w, w, x, ldx, M, bias,
-                          static_cast<const void*>(nullptr), residual, y, reinterpret_cast<float*>(sc),
-                          reinterpret_cast<int*>(sc + l.counters1_off), 0, dep, true, MoeTable{nullptr, nullptr, 0, 0}, units,
-                          static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = launch_split(M, M, cols, ldx, group, dtype, x, wk + ww.t8_off, wk + ww.meta_off, dep, st))) return rc;
+  W4Call c;
+  memset(&c, 0, sizeof(c));
+  c.dtype = dtype;
+  c.M = M;
+  c.rows = rows;
+  c.cols = cols;
+  c.experts = 1;
+  c.R = M;
+  c.group = group;
+  c.w0 = c.w1 = w;
+  c.t8 = wk + ww.t8_off;
+  c.meta = wk + ww.meta_off;
+  c.bias0 = bias;
+  c.residual = residual;
+  c.out = y;
+  c.slots = reinterpret_cast<float*>(sc);
+  c.counters = reinterpret_cast<int*>(sc + l.counters1_off);
+  c.early = true;
+  c.max_units = ((rows + 255) / 256) * ((cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
+  c.stream = st;
+  return launch_w4<false>(dev, c);
 }
 
-// Both halves of a gated MLP on 4-bit weights, dense (ids == NULL) or over experts.
+// Both halves of a gated MLP on 4-bit weights, dense (moe.ids == NULL) or over experts.
 static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const MoeTable& moe, int64_t active,
                   const void* x, const W4Matrix& g, const void* b_gate, const W4Matrix& u, const void* b_up,
-                  const W4Matrix& d, const void* b_down, const void* residual, void* h, void* y, void* scratch,
-                  size_t scratch_bytes, void* stream) {
+                  const W4Matrix& d, const void* b_down, const void* residual, void* y, void* work, size_t work_bytes,
+                  void* scratch, size_t scratch_bytes, void* stream) {
   int rc;
   if ((rc = check_group(group, p->K))) return rc;
   if ((rc = check_group(group, p->N))) return rc;
   if ((rc = check_w4(g)) || (rc = check_w4(u)) || (rc = check_w4(d))) return rc;
-  if ((rc = check_ptrs({x, h, y, scratch}))) return rc;
+  if ((rc = check_ptrs({x, y, work, scratch}))) return rc;
   const DeviceInfo* dev;
   if ((rc = device_info(&dev))) return rc;
   const FewLayout l = few_layout(p->K, p->N, active, dev->sm_count);
   if (scratch_bytes < l.total)
     return fail(GMLP_ERR_SCRATCH, "scratch holds %zu bytes, %zu needed", scratch_bytes, l.total);
-  char* sc = static_cast<char*>(scratch);
-  float* slots = reinterpret_cast<float*>(sc);
+  const W4Work ww = w4_work(p->M, p->K, p->N, active, group, p->dtype);
+  if (work_bytes < ww.total) return fail(GMLP_ERR_SCRATCH, "work holds %zu bytes, %zu needed", work_bytes, ww.total);
+  char* const wk = static_cast<char*>(work);
+  char* const sc = static_cast<char*>(scratch);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool sparse = moe.ids != nullptr;
   const bool dep = sparse || (p->tuning & (1u << 26)) == 0;  // GMLP_TUNE_ORDINARY_LAUNCH
   const int64_t k_units = (p->K + W4_UNIT_COLS - 1) / W4_UNIT_COLS, n_units = (p->N + W4_UNIT_COLS - 1) / W4_UNIT_COLS;
-  rc = launch_w4<true>(mpad_of(p->M), p->dtype, dev, p->M, p->N, p->K, experts, group, g, u, x, p->K, p->M, b_gate, b_up,
-                       static_cast<const void*>(nullptr), h, slots, reinterpret_cast<int*>(sc + l.counters1_off), p->act, dep, !sparse,
-                       moe, active * ((p->N + 127) / 128) * k_units, st);
-  if (rc) return rc;
-  return launch_w4<false>(mpad_of(p->M), p->dtype, dev, p->M, p->K, p->N, experts, group, d, d,
-                          static_cast<const void*>(h), p->N, active * p->M, b_down, static_cast<const void*>(nullptr),
-                          residual, y, slots, reinterpret_cast<int*>(sc + l.counters2_off), 0, true, true, moe,
-                          active * ((p->K + 255) / 256) * n_units, st);
+  if ((rc = launch_split(p->M, p->M, p->K, p->K, group, p->dtype, x, wk + ww.t8_off, wk + ww.meta_off, dep, st)))
+    return rc;
+  W4Call c;
+  memset(&c, 0, sizeof(c));
+  c.dtype = p->dtype;
+  c.M = p->M;
+  c.experts = experts;
+  c.group = group;
+  c.t8 = wk + ww.t8_off;
+  c.meta = wk + ww.meta_off;
+  c.slots = reinterpret_cast<float*>(sc);
+  c.act = p->act;
+  c.moe = moe;
+  c.stream = st;
+  c.rows = p->N;
+  c.cols = p->K;
+  c.R = p->M;
+  c.w0 = g;
+  c.w1 = u;
+  c.bias0 = b_gate;
+  c.bias1 = b_up;
+  c.out = wk;
+  c.counters = reinterpret_cast<int*>(sc + l.counters1_off);
+  c.early = !sparse;
+  c.max_units = active * ((p->N + 127) / 128) * k_units;
+  if ((rc = launch_w4<true>(dev, c))) return rc;
+  if ((rc = launch_split(p->M, active * p->M, p->N, p->N, group, p->dtype, wk, wk + ww.t8_off, wk + ww.meta_off, true,
+                         st)))
+    return rc;
+  c.rows = p->K;
+  c.cols = p->N;
+  c.R = active * p->M;
+  c.w0 = c.w1 = d;
+  c.bias0 = b_down;
+  c.bias1 = nullptr;
+  c.residual = residual;
+  c.out = y;
+  c.counters = reinterpret_cast<int*>(sc + l.counters2_off);
+  c.early = true;
+  c.max_units = active * ((p->K + 255) / 256) * n_units;
+  return launch_w4<false>(dev, c);
 }
 
 int gmlp_decode_fwd_w4(const gmlp_problem_t* p, int32_t group, const void* x, const void* w_gate4,
                        const void* w_gate_scale, const void* w_gate_zero, const void* b_gate, const void* w_up4,
                        const void* w_up_scale, const void* w_up_zero, const void* b_up, const void* w_down4,
                        const void* w_down_scale, const void* w_down_zero, const void* b_down, const void* residual,
-                       void* h, void* y, void* scratch, size_t scratch_bytes, void* stream) {
+                       void* y, void* work, size_t work_bytes, void* scratch, size_t scratch_bytes, void* stream) {
   int rc;
   if ((rc = check_few(p, "the 4-bit decode path"))) return rc;
   return mlp_w4(p, group, 1, MoeTable{nullptr, nullptr, 0, 0}, 1, x, {w_gate4, w_gate_scale, w_gate_zero}, b_gate,
-                {w_up4, w_up_scale, w_up_zero}, b_up, {w_down4, w_down_scale, w_down_zero}, b_down, residual, h, y,
-                scratch, scratch_bytes, stream);
+                {w_up4, w_up_scale, w_up_zero}, b_up, {w_down4, w_down_scale, w_down_zero}, b_down, residual, y, work,
+                work_bytes, scratch, scratch_bytes, stream);
 }
 
 int gmlp_moe_decode_fwd_w4(const gmlp_problem_t* p, int32_t group, int32_t experts, int32_t top_k, const void* x,
                            const int32_t* ids, const float* weights, const void* w_gate4, const void* w_gate_scale,
                            const void* w_gate_zero, const void* w_up4, const void* w_up_scale, const void* w_up_zero,
                            const void* w_down4, const void* w_down_scale, const void* w_down_zero,
-                           const void* residual, void* h, void* y, void* scratch, size_t scratch_bytes, void* stream) {
+                           const void* residual, void* y, void* work, size_t work_bytes, void* scratch,
+                           size_t scratch_bytes, void* stream) {
   int rc;
   if ((rc = check_few(p, "the mixture-of-experts decode path"))) return rc;
   if ((rc = check_experts(p, experts, top_k, ids, weights))) return rc;
   return mlp_w4(p, group, experts, MoeTable{ids, weights, top_k, experts}, max_active(p, experts, top_k), x,
                 {w_gate4, w_gate_scale, w_gate_zero}, nullptr, {w_up4, w_up_scale, w_up_zero}, nullptr,
-                {w_down4, w_down_scale, w_down_zero}, nullptr, residual, h, y, scratch, scratch_bytes, stream);
+                {w_down4, w_down_scale, w_down_zero}, nullptr, residual, y, work, work_bytes, scratch, scratch_bytes,
+                stream);
 }
 
 int gmlp_moe_decode_fwd(const gmlp_problem_t* p, int32_t experts, int32_t top_k, const void* x, const int32_t* ids,

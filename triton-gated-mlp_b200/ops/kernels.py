@@ -637,6 +637,12 @@ def _scratch_for(K: int, N: int, experts: int, dev: torch.device, stream: int) -
     return have[2]
 
 
+def _w4_work(M: int, K: int, N: int, experts: int, group: int, dt: torch.dtype, dev: torch.device) -> Tensor:
+    """Work buffer of one 4-bit call (gmlp_w4_work_bytes)."""
+    return torch.empty((load().gmlp_w4_work_bytes(M, K, N, experts, group, dtype_code(dt)),), dtype=torch.uint8,
+                       device=dev)
+
+
 def _rows_of(x: Tensor) -> Tensor:
     """x with contiguous rows on 16-byte boundaries (a copy where the caller's view has neither)."""
     x = _c(x)
@@ -695,9 +701,10 @@ def linear_w4(x: Tensor, w: Int4Weight, bias: Tensor | None = None, residual: Te
         stream = torch.cuda.current_stream(dev).cuda_stream
         if scratch is None:
             scratch = _scratch_for(N, N, 1, dev, stream)
+        work = _w4_work(M, K, 0, 1, group, dt, dev)
         check(load().gmlp_w4_linear(M, N, K, group, dtype_code(dt), x.data_ptr(), ldx, w[0].data_ptr(),
                                     w[1].data_ptr(), ptr(w[2]), ptr(bias), ptr(residual), y.data_ptr(),
-                                    scratch.data_ptr(), scratch.numel() * scratch.element_size(),
+                                    work.data_ptr(), work.numel(), scratch.data_ptr(), scratch.numel() * scratch.element_size(),
                                     (1 << 26) if ordinary_launch else 0, stream))
     return y
 
@@ -726,7 +733,7 @@ def decode_fwd_w4(x: Tensor, w_gate: Int4Weight, b_gate: Tensor | None, w_up: In
     if M == 0:
         return y
     x = _rows_of(x)
-    h = torch.empty((M, N), dtype=dt, device=dev)
+    work = _w4_work(M, K, N, 1, group, dt, dev)
     prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act, (1 << 26) if ordinary_launch else 0)
     with _on(dev):
         stream = torch.cuda.current_stream(dev).cuda_stream
@@ -735,7 +742,7 @@ def decode_fwd_w4(x: Tensor, w_gate: Int4Weight, b_gate: Tensor | None, w_up: In
         check(load().gmlp_decode_fwd_w4(
             C.byref(prob), group, x.data_ptr(), w_gate[0].data_ptr(), w_gate[1].data_ptr(), ptr(w_gate[2]), ptr(b_gate),
             w_up[0].data_ptr(), w_up[1].data_ptr(), ptr(w_up[2]), ptr(b_up), w_down[0].data_ptr(), w_down[1].data_ptr(),
-            ptr(w_down[2]), ptr(b_down), ptr(residual), h.data_ptr(), y.data_ptr(), scratch.data_ptr(),
+            ptr(w_down[2]), ptr(b_down), ptr(residual), y.data_ptr(), work.data_ptr(), work.numel(), scratch.data_ptr(),
             scratch.numel() * scratch.element_size(), stream))
     return y
 
@@ -851,7 +858,7 @@ def moe_decode_fwd_w4(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Int4Weigh
         return y
     x = _rows_of(x)
     active = min(E, M * k)
-    h = torch.empty((active, M, N), dtype=dt, device=dev)
+    work = _w4_work(M, K, N, active, group, dt, dev)
     prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act)
     with _on(dev):
         stream = torch.cuda.current_stream(dev).cuda_stream
@@ -860,8 +867,8 @@ def moe_decode_fwd_w4(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Int4Weigh
         check(load().gmlp_moe_decode_fwd_w4(
             C.byref(prob), group, E, k, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate[0].data_ptr(),
             w_gate[1].data_ptr(), ptr(w_gate[2]), w_up[0].data_ptr(), w_up[1].data_ptr(), ptr(w_up[2]),
-            w_down[0].data_ptr(), w_down[1].data_ptr(), ptr(w_down[2]), ptr(residual), h.data_ptr(), y.data_ptr(),
-            scratch.data_ptr(), scratch.numel() * scratch.element_size(), stream))
+            w_down[0].data_ptr(), w_down[1].data_ptr(), ptr(w_down[2]), ptr(residual), y.data_ptr(), work.data_ptr(),
+            work.numel(), scratch.data_ptr(), scratch.numel() * scratch.element_size(), stream))
     return y
 
 
