@@ -97,8 +97,152 @@ __device__ __forceinline__ void moe_factors(const MoeTable& t, int M, int e, int
   s.hit[ep_tid] = hit;
 }
 
+// ---- stream-K: the launch's units in row-tile-major order, cut into one contiguous range per CTA; a range is cut at row
+// tile borders into segments. All in 32 bits (the host refuses larger calls): a 64-bit division is a hundred
+// instructions, and a single warp at the start of a kernel takes a microsecond for four of them. ----
+struct Cut {
+  int total;      // units of the launch
+  int ctas;       // CTAs that have units (at most one per unit)
+  int each, odd;  // units per CTA; the first `odd` CTAs have one more
+};
+__device__ __forceinline__ Cut make_cut(int total, int grid) {
+  Cut c;
+  c.total = total;
+  c.ctas = total < grid ? total : grid;
+  c.each = c.ctas > 0 ? total / c.ctas : 0;
+  c.odd = total - c.each * c.ctas;
+  return c;
+}
+__device__ __forceinline__ int cut_start(const Cut& c, int cta) {
+  return cta >= c.ctas ? c.total : cta * c.each + (cta < c.odd ? cta : c.odd);
+}
+__device__ __forceinline__ int cut_owner(const Cut& c, int unit) {  // the CTA that has the unit
+  const int big = c.odd * (c.each + 1);
+  return unit < big ? unit / (c.each + 1) : c.odd + (unit - big) / c.each;
+}
+
+struct Segment {
+  int tile, begin, end;  // row tile, and this CTA's units of it
+  int tile_begin, tile_end;
+};
+__device__ __forceinline__ Segment segment_at(int u, int u_end, int per_tile) {
+  Segment s;
+  s.tile = u / per_tile;
+  s.begin = u;
+  s.tile_begin = s.tile * per_tile;
+  s.tile_end = s.tile_begin + per_tile;
+  s.end = s.tile_end < u_end ? s.tile_end : u_end;
+  return s;
+}
+
+// ---- end of a segment: sums to a slot, from there to the output ----
+// A CTA's sums of a row tile go to a slot in global memory (L2), [NT][COLS_ALL / 4][128] float4 = four tokens of one
+// weight row, and from there through the epilogue to the output, in a loop of a few hundred instructions. (Straight
+// from the registers the epilogue is unrolled over all of a thread's tokens, 10 KB of code that run once per tile:
+// fetching it took 9,500 clocks at 64 tokens.) A tile whose units lie in several CTAs is finished by all of them together:
+// each publishes its part as soon as it has it, and when it is through with its units it waits (bounded) for the
+// others' parts and finishes an equal share of the tile's rows and tokens, adding the parts in CTA order (the result does
+// not depend on arrival). (With one owner per tile that fetched all parts, 64 tokens and 9 CTAs per tile, the owner
+// alone took 26,000 clocks.) A CTA waits only after it has published everything it owes, for CTAs that come to
+// their last unit when it does; one that has not started yet waits for an SM that some other kernel or a CTA that
+// will not wait for it still holds.
+// Only the float4 columns below M travel: with one token that is a quarter of a 16-column tile.
+// Counter word of a tile: parts published in the low half, CTAs that have seen all of them in the high half; the last of
+// those clears it.
+struct Split {
+  Cut cut;
+  int M;
+  float4* slots;  // [2 * CTAs]: slot 2c holds CTA c's part of the tile it starts in the middle of, 2c + 1 any other
+  int* counters;  // [row tiles]; zero before and after the launch
+  int* status;
+  volatile int* abortp;
+};
+__device__ __forceinline__ int ld_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void red_release(int* p, int v) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+__device__ __forceinline__ int slot_of(const Cut& c, int cta, int tile_begin) {
+  return 2 * cta + (cut_start(c, cta) > tile_begin ? 0 : 1);
+}
+
+// All THREADS epilogue threads: thread = weight row `row` of NT tiles, COLS of the COLS_ALL token columns from col0 on.
+template <int NT, int COLS, int COLS_ALL, int THREADS>
+__device__ __forceinline__ void publish_segment(const float (&v)[NT][COLS], const Segment& s, const Split& sp, int col0,
+                                                int row, int ep_tid) {
+  const int left = sp.M - col0;
+  const int nq = left <= 0 ? 0 : ((left < COLS ? left : COLS) + 3) / 4;
+  float4* const slot = sp.slots + static_cast<long long>(slot_of(sp.cut, blockIdx.x, s.tile_begin)) * (NT * COLS_ALL / 4 * 128);
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < COLS / 4; ++i)
+      if (i < nq)
+        slot[(t * (COLS_ALL / 4) + col0 / 4 + i) * 128 + row] =
+            make_float4(v[t][4 * i], v[t][4 * i + 1], v[t][4 * i + 2], v[t][4 * i + 3]);
+  named_bar_sync(1, THREADS);
+  if (s.begin != s.tile_begin || s.end != s.tile_end) {
+    // one thread's release covers the block's stores, which the barrier put before it (256 threads that each
+    // waited for their own held up the sums behind them for 2,000 to 9,000 clocks while HBM was busy)
+    if (ep_tid == 0) red_release(sp.counters + s.tile, 1);
+  }
+}
+
+// This CTA's share of a tile whose parts are in the slots: emit(t, row, i, sums) for four tokens 4i .. 4i + 3 of a row, with
+// JOINT over both tiles at once (emit(0, row, i, gate, up)). The first part of the next item is on its way while an item
+// is finished.
+template <int NT, bool JOINT, int COLS_ALL, int THREADS, typename Emit>
+__device__ __forceinline__ void finish_tile(int tile_begin, int first, int last, const Split& sp, int ep_tid, Emit emit) {
+  constexpr int SLOT4 = NT * COLS_ALL / 4 * 128;
+  const int nq = (sp.M + 3) / 4, parts = last - first + 1, mine = blockIdx.x - first;
+  const int items = (JOINT ? 1 : NT) * nq * 128;
+  const int lo = items * mine / parts, hi = items * (mine + 1) / parts;  // at most 2 * 16 * 128 * 1024
+  const float4* const s0 = sp.slots + static_cast<long long>(slot_of(sp.cut, first, tile_begin)) * SLOT4;
+  const float4* const s1 = sp.slots + (2LL * first + 2) * SLOT4;  // the others start in the middle of the tile
+  float4 next_a = make_float4(0.f, 0.f, 0.f, 0.f), next_b = next_a;
+  int t = 0, row = 0, i = 0;
+  auto place = [&](int it) {
+    t = JOINT ? 0 : it / (nq * 128);
+    const int rest = it - t * nq * 128;
+    i = rest >> 7;
+    row = rest & 127;
+    return (t * (COLS_ALL / 4) + i) * 128 + row;
+  };
+  auto fetch = [&](int it) {
+    const int at = place(it);
+    next_a = __ldcg(s0 + at);
+    if (JOINT) next_b = __ldcg(s0 + at + COLS_ALL / 4 * 128);
+  };
+  if (lo + ep_tid < hi) fetch(lo + ep_tid);
+#pragma unroll 1
+  for (int it = lo + ep_tid; it < hi; it += THREADS) {
+    float4 a = next_a, b = next_b;
+    if (it + THREADS < hi) fetch(it + THREADS);
+    const float4* s = s1 + place(it);
+#pragma unroll 4
+    for (int c = 1; c < parts; ++c, s += 2 * SLOT4) {
+      const float4 q = __ldcg(s);
+      a.x += q.x;
+      a.y += q.y;
+      a.z += q.z;
+      a.w += q.w;
+      if (JOINT) {
+        const float4 r = __ldcg(s + COLS_ALL / 4 * 128);
+        b.x += r.x;
+        b.y += r.y;
+        b.z += r.z;
+        b.w += r.w;
+      }
+    }
+    emit(t, row, i, a, b);
+  }
+}
+
 // Gate activations at fp32 accuracy (the GEMM epilogues use tanh.approx, whose 2^-11 is as large as fp16's own
-// rounding; here the epilogue runs once per 128 x 64 outputs and costs nothing).
+// rounding; here the epilogue is a small part of the work).
 template <int ACT>
 __device__ __forceinline__ float act_fine(float x) {
   if (ACT == ACT_SILU) return __fdividef(x, 1.0f + __expf(-x));
@@ -109,158 +253,101 @@ __device__ __forceinline__ float act_fine(float x) {
   if (ACT == ACT_LEAKY_RELU) return x > 0.0f ? x : 0.01f * x;
   return x;
 }
-
-// One weight row of the gate/up kernel: hidden values of tokens col0 .. col0 + COLS - 1 (those below M).
-template <int ACT, int COLS, typename T>
-__device__ __forceinline__ void store_hidden_act(T* po, long long ld, int M, int col0, const float* gate,
-                                                 const float* up, float b0, float b1, const MoeShared* moe) {
+template <int ACT>
+__device__ __forceinline__ void hidden4(float (&h)[4], const float4& g, const float4& u, float bg, float bu) {
+  h[0] = act_fine<ACT>(g.x + bg) * (u.x + bu);
+  h[1] = act_fine<ACT>(g.y + bg) * (u.y + bu);
+  h[2] = act_fine<ACT>(g.z + bg) * (u.z + bu);
+  h[3] = act_fine<ACT>(g.w + bg) * (u.w + bu);
+}
+// Four tokens of a hidden row: act(gate + bg) * (up + bu), on experts times the token's factor, or 0.
+template <typename T>
+__device__ __forceinline__ void emit_hidden(T* po, long long ld, int M, int i, const float4& gate, const float4& up,
+                                            float bg, float bu, int act, const MoeShared* moe) {
+  float h[4];
+  switch (act) {
+    case ACT_SILU: hidden4<ACT_SILU>(h, gate, up, bg, bu); break;
+    case ACT_NONE: hidden4<ACT_NONE>(h, gate, up, bg, bu); break;
+    case ACT_RELU: hidden4<ACT_RELU>(h, gate, up, bg, bu); break;
+    case ACT_GELU: hidden4<ACT_GELU>(h, gate, up, bg, bu); break;
+    case ACT_SIGMOID: hidden4<ACT_SIGMOID>(h, gate, up, bg, bu); break;
+    case ACT_TANH: hidden4<ACT_TANH>(h, gate, up, bg, bu); break;
+    default: hidden4<ACT_LEAKY_RELU>(h, gate, up, bg, bu); break;
+  }
+  po += static_cast<long long>(4 * i) * ld;
 #pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    const int m = col0 + c;
+  for (int k = 0; k < 4; ++k, po += ld) {
+    const int m = 4 * i + k;
     if (m < M) {
-      float h = act_fine<ACT>(gate[c] + b0) * (up[c] + b1);
-      if (moe != nullptr) h = moe->hit[m] ? h * moe->f[m] : 0.f;
-      po[static_cast<long long>(m) * ld] = static_cast<T>(h);
+      if (moe != nullptr) h[k] = moe->hit[m] ? h[k] * moe->f[m] : 0.f;
+      *po = static_cast<T>(h[k]);
     }
   }
 }
-template <int COLS, typename T>
-__device__ __forceinline__ void store_hidden(int act, T* po, long long ld, int M, int col0, const float* gate,
-                                             const float* up, float b0, float b1, const MoeShared* moe) {
-  switch (act) {  // outside the unrolled token loop: one body per activation, not COLS switches
-    case ACT_SILU: store_hidden_act<ACT_SILU, COLS>(po, ld, M, col0, gate, up, b0, b1, moe); break;
-    case ACT_NONE: store_hidden_act<ACT_NONE, COLS>(po, ld, M, col0, gate, up, b0, b1, moe); break;
-    case ACT_RELU: store_hidden_act<ACT_RELU, COLS>(po, ld, M, col0, gate, up, b0, b1, moe); break;
-    case ACT_GELU: store_hidden_act<ACT_GELU, COLS>(po, ld, M, col0, gate, up, b0, b1, moe); break;
-    case ACT_SIGMOID: store_hidden_act<ACT_SIGMOID, COLS>(po, ld, M, col0, gate, up, b0, b1, moe); break;
-    case ACT_TANH: store_hidden_act<ACT_TANH, COLS>(po, ld, M, col0, gate, up, b0, b1, moe); break;
-    default: store_hidden_act<ACT_LEAKY_RELU, COLS>(po, ld, M, col0, gate, up, b0, b1, moe); break;
-  }
-}
-// One weight row of a plain product: out[m] = v[m] (* wmax[m]) + bias + residual[m].
-template <int COLS, typename T>
-__device__ __forceinline__ void store_product(T* po, const T* pr, long long ld, int M, int col0, const float* v,
-                                              float bias, const MoeShared* moe) {
+// Four tokens of an output row: v (* wmax) + bias + residual.
+template <typename T>
+__device__ __forceinline__ void emit_product(T* po, const T* pr, long long ld, int M, int i, const float4& v, float bias,
+                                             const MoeShared* moe) {
+  const float a[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    const int m = col0 + c;
+  for (int k = 0; k < 4; ++k) {
+    const int m = 4 * i + k;
     if (m < M) {
-      float o = (moe != nullptr ? v[c] * moe->wmax[m] : v[c]) + bias;
+      float o = (moe != nullptr ? a[k] * moe->wmax[m] : a[k]) + bias;
       if (pr) o += static_cast<float>(pr[static_cast<long long>(m) * ld]);
       po[static_cast<long long>(m) * ld] = static_cast<T>(o);
     }
   }
 }
 
-// ---- stream-K: the units [u_begin, u_end) of a CTA, cut at row tile borders into segments ----
-struct Segment {
-  long long tile, begin, end;  // row tile, and this CTA's units of it
-  long long tile_begin, tile_end;
+// The end of a segment and of a CTA's units, shared by the stream kernels. `emit_tile(tile, tile_begin, first, last)` finishes
+// this CTA's share of a tile from the slots of CTAs first .. last.
+struct Pending {
+  int tile[2];
+  int n = 0;
 };
-__device__ __forceinline__ Segment segment_at(long long u, long long u_end, long long per_tile) {
-  Segment s;
-  s.tile = u / per_tile;
-  s.begin = u;
-  s.tile_begin = s.tile * per_tile;
-  s.tile_end = s.tile_begin + per_tile;
-  s.end = s.tile_end < u_end ? s.tile_end : u_end;
-  return s;
-}
-
-struct Split {
-  long long total;  // units of the launch
-  long long ctas;   // CTAs that have units (at most one per unit)
-  float* slots;     // [ctas][NT][COLS_ALL / 4][128] float4: a CTA's partial row tile
-  int* counters;    // [row tiles]: units whose partial sums are in the slots; zero before and after the launch
-  int* status;
-  volatile int* abortp;
-  uint32_t ring;    // shared memory free for staging while a CTA finishes its last segment
-  int ring_pieces;  // 16-byte pieces per thread that the ring holds
-};
-
-enum : int { SETTLE_ABORT = 0, SETTLE_EMIT = 1, SETTLE_SENT = 2 };
-
-// Joins a row tile's partial sums. Called by all THREADS epilogue threads (a multiple of 128: thread = weight row
-// `row` of the tile, column group of COLS tokens starting at col0) with this CTA's sums of segment `s`.
-// A tile that was not cut is complete. Of a cut tile the CTA that holds the first units is the owner: for it
-// the tile is the last thing it works on, while the others met it first and published their part before. It
-// waits (bounded) until all other units are counted, adds the parts in CTA order (the result does not depend
-// on arrival) and clears the counter. Only the float4 columns below M travel: with one token that is a
-// quarter of a 16-column tile.
-template <int NT, int COLS, int COLS_ALL, int THREADS>
-__device__ __forceinline__ int settle_segment(float (&v)[NT][COLS], const Segment& s, const Split& sp, int M,
-                                              int col0, int row, int ep_tid) {
+template <int NT, int COLS, int COLS_ALL, int THREADS, typename EmitTile>
+__device__ __forceinline__ bool end_segment(const float (&v)[NT][COLS], const Segment& s, const Split& sp, int col0, int row,
+                                            int ep_tid, Pending& pending, EmitTile emit_tile) {
   // vote: all epilogue threads leave the same way even if the abort flag flips between their reads
-  if (named_bar_or(1, THREADS, *sp.abortp != 0)) return SETTLE_ABORT;
-  const bool first = s.begin == s.tile_begin;
-  if (first && s.end == s.tile_end) return SETTLE_EMIT;
-  constexpr long long SLOT4 = static_cast<long long>(NT) * (COLS_ALL / 4) * 128;
-  const int left = M - col0;
-  const int nq = left <= 0 ? 0 : ((left < COLS ? left : COLS) + 3) / 4;
-  if (!first) {
-    float4* const slot = reinterpret_cast<float4*>(sp.slots) + blockIdx.x * SLOT4;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < COLS / 4; ++i)
-        if (i < nq)
-          slot[(t * (COLS_ALL / 4) + col0 / 4 + i) * 128 + row] =
-              make_float4(v[t][4 * i], v[t][4 * i + 1], v[t][4 * i + 2], v[t][4 * i + 3]);
-    __threadfence();
-    named_bar_sync(1, THREADS);
-    if (ep_tid == 0) atomicAdd(sp.counters + s.tile, static_cast<int>(s.end - s.begin));
-    return SETTLE_SENT;
-  }
-  if (ep_tid == 0) {
-    const int need = static_cast<int>(s.tile_end - s.end);
-    const volatile int* cnt = sp.counters + s.tile;
+  if (named_bar_or(1, THREADS, *sp.abortp != 0)) return false;
+  publish_segment<NT, COLS, COLS_ALL, THREADS>(v, s, sp, col0, row, ep_tid);
+  if (s.begin == s.tile_begin && s.end == s.tile_end)
+    emit_tile(s.tile, s.tile_begin, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.x));
+  else
+    pending.tile[pending.n++] = s.tile;
+  return true;
+}
+template <int THREADS, typename EmitTile>
+__device__ __forceinline__ void end_units(const Pending& pending, int per_tile, const Split& sp, int ep_tid,
+                                          EmitTile emit_tile) {
+  if (pending.n == 0) return;
+  // thread 0 waits for the parts of the first tile, thread 32 for those of the second
+  const int k = ep_tid >> 5;
+  const bool waiter = (ep_tid & 31) == 0 && k < pending.n;
+  int my_tile = 0, my_parts = 0;
+  if (waiter) {
+    my_tile = k == 0 ? pending.tile[0] : pending.tile[1];
+    const int begin = my_tile * per_tile;
+    my_parts = cut_owner(sp.cut, begin + per_tile - 1) - cut_owner(sp.cut, begin) + 1;
     const long long t0 = clock64();
-    while (*cnt != need) {
+    while ((ld_acquire(sp.counters + my_tile) & 0xffff) != my_parts) {
       if (*sp.abortp != 0 || clock64() - t0 > WAIT_LIMIT_CYCLES) {
         *sp.abortp = 1;
         atomicCAS(sp.status, 0, GMLP_DEV_TIMEOUT_EPILOGUE);
         break;
       }
-      __nanosleep(32);
-    }
-    __threadfence();
-  }
-  if (named_bar_or(1, THREADS, *sp.abortp != 0)) return SETTLE_ABORT;
-  const long long c_first = ((s.tile_begin + 1) * sp.ctas - 1) / sp.total;
-  const long long c_last = (s.tile_end * sp.ctas - 1) / sp.total;
-  const int per = NT * nq;  // pieces of one contributor and thread
-  if (per > 0) {
-    const int batch = sp.ring_pieces / per;  // contributors fetched per round trip
-    auto stage = [&](int k) { return sp.ring + static_cast<uint32_t>(k * THREADS + ep_tid) * 16u; };
-    for (long long cb = c_first + 1; cb <= c_last; cb += batch) {
-      const long long ce = cb + batch - 1 < c_last ? cb + batch - 1 : c_last;
-      int k = 0;
-      for (long long c = cb; c <= ce; ++c) {
-        const float4* slot = reinterpret_cast<const float4*>(sp.slots) + c * SLOT4;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          for (int i = 0; i < nq; ++i, ++k)
-            cp_async_16(stage(k), slot + (t * (COLS_ALL / 4) + col0 / 4 + i) * 128 + row);
-      }
-      cp_async_wait_all();
-      k = 0;
-      for (long long c = cb; c <= ce; ++c) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < COLS / 4; ++i)
-            if (i < nq) {
-              const float4 q = ld_shared_f4(stage(k++));
-              v[t][4 * i] += q.x;
-              v[t][4 * i + 1] += q.y;
-              v[t][4 * i + 2] += q.z;
-              v[t][4 * i + 3] += q.w;
-            }
-      }
     }
   }
-  if (ep_tid == 0) sp.counters[s.tile] = 0;  // ready for the next call
-  return SETTLE_EMIT;
+  if (named_bar_or(1, THREADS, *sp.abortp != 0)) return;
+#pragma unroll 1
+  for (int p = 0; p < pending.n; ++p) {
+    const int tile = p == 0 ? pending.tile[0] : pending.tile[1];
+    const int begin = tile * per_tile;
+    emit_tile(tile, begin, cut_owner(sp.cut, begin), cut_owner(sp.cut, begin + per_tile - 1));
+  }
+  // the last CTA to have seen all parts leaves the counter ready for the next call
+  if (waiter && (atomicAdd(sp.counters + my_tile, 0x10000) >> 16) == my_parts - 1) sp.counters[my_tile] = 0;
 }
 
 // Bounded wait that looks at no abort flag: a thread that gives up uses it to see its own copies in flight land

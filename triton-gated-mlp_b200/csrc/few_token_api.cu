@@ -8,8 +8,8 @@
 
 #include "../../include/gmlp.h"
 #include "host_util.h"
+#include "few_token_host.cuh"
 #include "moe_stream.cuh"
-#include "w4_stream.cuh"
 
 namespace gmlp {
 
@@ -17,7 +17,8 @@ namespace gmlp {
 // [slots][counters of the first kernel][counters of the second]. The slots take the size of a 64-token call whatever the
 // call is, so that the counters, which have to be zero between calls, lie behind them for every shape and calls of
 // different shapes can follow one another on one buffer.
-static size_t slots_bytes(int ctas) { return static_cast<size_t>(ctas) * 2 * 128 * FEW_MAX_TOKENS * sizeof(float); }
+// two slots per CTA, each two tiles of 128 rows
+static size_t slots_bytes(int ctas) { return static_cast<size_t>(ctas) * 2 * 2 * 128 * FEW_MAX_TOKENS * sizeof(float); }
 struct FewLayout {
   size_t counters1_off, counters2_off, total;
 };
@@ -30,36 +31,6 @@ static FewLayout few_layout(int64_t K, int64_t N, int64_t experts, int ctas) {
   return l;
 }
 static int mpad_of(int64_t M) { return M <= 16 ? 16 : (M <= 32 ? 32 : 64); }
-
-// ---------------------------------------------------------------- launching --
-template <typename Kernel, typename Args>
-static int launch_stream(Kernel kfn, int grid, int threads, size_t smem, bool dependent, const CUtensorMap& m0,
-                         const CUtensorMap& m1, const CUtensorMap& mx, const Args& a, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  if (dependent) {
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-  }
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kfn, m0, m1, mx, a);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(GMLP_ERR_LAUNCH, "kernel launch: %s", cudaGetErrorString(e));
-  return GMLP_OK;
-}
-
-// One 4-bit weight matrix (of one or of all experts).
-struct W4Matrix {
-  const void* q;
-  const void* scale;
-  const void* zero;
-};
 
 static int check_w4(const W4Matrix& w) {
   if (!w.q || !w.scale) return fail(GMLP_ERR_ARG, "NULL 4-bit weight or scale");
@@ -78,7 +49,6 @@ static int check_group(int32_t group, int64_t cols) {
 
 // Work buffer of a 4-bit call: [hidden state][activation terms][their meta data]. The terms of x and, later, of the
 // hidden state take turns in one place.
-static int w4_mt(int64_t M) { return M <= 8 ? 8 : (M <= 16 ? 16 : (M <= 32 ? 32 : 64)); }
 struct W4Work {
   size_t t8_off, meta_off, total;
 };
@@ -90,7 +60,9 @@ static W4Work w4_work(int64_t M, int64_t K, int64_t N, int64_t active, int group
   W4Work w;
   w.t8_off = align_up(static_cast<size_t>(active * M * N) * 2, 256);
   w.meta_off = w.t8_off + align_up(std::max(w4_t8_bytes(M, K, dtype), w4_t8_bytes(active * M, N, dtype)), 256);
-  w.total = w.meta_off + static_cast<size_t>(std::max(K / group, active * (N / group))) * 2 * w4_mt(M) * sizeof(float);
+  const int64_t k_units = (K + W4_UNIT_COLS - 1) / W4_UNIT_COLS, n_units = (N + W4_UNIT_COLS - 1) / W4_UNIT_COLS;
+  w.total = w.meta_off + static_cast<size_t>(std::max(k_units, active * n_units)) * (W4_UNIT_COLS / group) * 2 * w4_mt(M) *
+                             sizeof(float);
   return w;
 }
 
@@ -108,98 +80,19 @@ static int launch_split(int64_t M, int64_t R, int64_t cols, int64_t ldx, int gro
   a.t8 = static_cast<uint8_t*>(t8);
   a.meta = static_cast<float*>(meta);
   a.dependent = dependent ? 1 : 0;
-  const int64_t items = R * ((cols + W4_HALF_COLS - 1) / W4_HALF_COLS);
+  const int64_t items = R * ((cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS) * 2;
   const int64_t per_block = W4_SPLIT_THREADS / 16;
   const int64_t blocks = (items + per_block - 1) / per_block;
   if (blocks > 0x7fffffffLL) return fail(GMLP_ERR_SHAPE, "too many activations");
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(W4_SPLIT_THREADS);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  if (dependent) {
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-  }
-  cudaError_t e = dtype == GMLP_BF16 ? cudaLaunchKernelEx(&cfg, w4_split_kernel<__nv_bfloat16>, a)
-                                     : cudaLaunchKernelEx(&cfg, w4_split_kernel<__half>, a);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(GMLP_ERR_LAUNCH, "kernel launch: %s", cudaGetErrorString(e));
-  return GMLP_OK;
+  return dtype == GMLP_BF16 ? launch_few(w4_split_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks),
+                                         W4_SPLIT_THREADS, 0, dependent, stream, a)
+                            : launch_few(w4_split_kernel<__half>, static_cast<unsigned>(blocks), W4_SPLIT_THREADS, 0,
+                                         dependent, stream, a);
 }
 
-// What every instantiation of the stream kernel is launched with.
-struct W4Call {
-  int dtype;
-  int64_t M, rows, cols, experts, R;
-  int group;
-  W4Matrix w0, w1;
-  const void *t8, *meta;
-  const void *bias0, *bias1, *residual;
-  void* out;
-  float* slots;
-  int* counters;
-  int act;
-  bool early;
-  MoeTable moe;
-  int64_t max_units;
-  cudaStream_t stream;
-};
-template <int MT, bool DUAL, typename T>
-static int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
-  using Conf = W4Conf<MT, w4_terms<T>()>;
-  CUtensorMap m0, m1, mx;
-  int rc;
-  if ((rc = encode_map(&m0, c.w0.q, c.cols / 2, c.experts * c.rows, c.cols / 2, 128, 128, DTYPE_U8))) return rc;
-  m1 = m0;
-  if (DUAL && (rc = encode_map(&m1, c.w1.q, c.cols / 2, c.experts * c.rows, c.cols / 2, 128, 128, DTYPE_U8))) return rc;
-  if ((rc = encode_map(&mx, c.t8, c.cols, w4_terms<T>() * c.R, c.cols, 128, MT, DTYPE_U8))) return rc;
-  W4Args a;
-  memset(&a, 0, sizeof(a));
-  a.M = static_cast<int>(c.M);
-  a.rows = static_cast<int>(c.rows);
-  a.kbt = static_cast<int>((c.cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
-  a.groups = static_cast<int>(c.cols / c.group);
-  a.gshift = c.group == 32 ? 0 : (c.group == 64 ? 1 : 2);
-  // an accumulator buffer holds as many groups of a half unit as leave room for a second buffer
-  a.gpg = 4 >> a.gshift;
-  while (a.gpg > 1 && a.gpg * Conf::N > 128) a.gpg >>= 1;
-  a.acc_bufs = std::min(Conf::MAX_ACC_BUFS, Conf::C_COLS / (a.gpg * Conf::N));
-  a.R = c.R;
-  a.idesc = make_idesc_f8(128, Conf::N);
-  a.status = dev->status_ptr;
-  a.meta = static_cast<const float*>(c.meta);
-  a.scale0 = static_cast<const uint16_t*>(c.w0.scale);
-  a.scale1 = static_cast<const uint16_t*>(c.w1.scale);
-  a.zero0 = static_cast<const uint8_t*>(c.w0.zero);
-  a.zero1 = static_cast<const uint8_t*>(c.w1.zero);
-  a.bias0 = c.bias0;
-  a.bias1 = c.bias1;
-  a.residual = c.residual;
-  a.out = c.out;
-  a.slots = c.slots;
-  a.counters = c.counters;
-  a.act = c.act;
-  a.early = c.early ? 1 : 0;
-  a.moe = c.moe;
-  const int grid = static_cast<int>(c.max_units < dev->sm_count ? c.max_units : dev->sm_count);
-  auto kfn = w4_stream_kernel<MT, DUAL, T>;
-  static std::atomic<uint64_t> attr_done{0};
-  if ((rc = ensure_smem_attr(kfn, Conf::SMEM, attr_done))) return rc;
-  return launch_stream(kfn, grid, Conf::THREADS, Conf::SMEM, true, m0, m1, mx, a, c.stream);
-}
-template <bool DUAL>
-static int launch_w4(const DeviceInfo* dev, const W4Call& c) {
-  const bool bf = c.dtype == GMLP_BF16;
-  switch (w4_mt(c.M)) {
-    case 8: return bf ? launch_w4_t<8, DUAL, __nv_bfloat16>(dev, c) : launch_w4_t<8, DUAL, __half>(dev, c);
-    case 16: return bf ? launch_w4_t<16, DUAL, __nv_bfloat16>(dev, c) : launch_w4_t<16, DUAL, __half>(dev, c);
-    case 32: return bf ? launch_w4_t<32, DUAL, __nv_bfloat16>(dev, c) : launch_w4_t<32, DUAL, __half>(dev, c);
-    default: return bf ? launch_w4_t<64, DUAL, __nv_bfloat16>(dev, c) : launch_w4_t<64, DUAL, __half>(dev, c);
-  }
+static int launch_w4(const DeviceInfo* dev, const W4Call& c, bool dual) {
+  return c.group == 32 ? launch_w4_g32(dev, c, dual)
+                       : (c.group == 64 ? launch_w4_g64(dev, c, dual) : launch_w4_g128(dev, c, dual));
 }
 
 template <int MPAD, bool DUAL, typename T>
@@ -207,6 +100,7 @@ static int launch_moe_t(const DeviceInfo* dev, int dtype, int64_t M, int64_t row
                         const void* w0, const void* w1, const void* x, int64_t ldx, int64_t x_rows,
                         const void* residual, void* out, float* slots, int* counters, int act, bool early,
                         const MoeTable& moe, int64_t grid_units, cudaStream_t stream) {
+  if (grid_units > 0x7fffffffLL) return fail(GMLP_ERR_SHAPE, "the call has more than 2^31 units of work");
   CUtensorMap m0, m1, mx;
   int rc;
   if ((rc = encode_map(&m0, w0, cols, experts * rows, cols, 64, 128, dtype))) return rc;
@@ -232,7 +126,7 @@ static int launch_moe_t(const DeviceInfo* dev, int dtype, int64_t M, int64_t row
   constexpr size_t smem = moe_smem_bytes<MPAD, DUAL>();
   static std::atomic<uint64_t> attr_done{0};
   if ((rc = ensure_smem_attr(kfn, smem, attr_done))) return rc;
-  return launch_stream(kfn, grid, MOE_THREADS, smem, true, m0, m1, mx, a, stream);
+  return launch_few(kfn, grid, MOE_THREADS, smem, true, stream, m0, m1, mx, a);
 }
 template <bool DUAL, typename... Args>
 static int launch_moe(int mpad, int dtype, const DeviceInfo* dev, Args... args) {
@@ -353,7 +247,7 @@ int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t
   c.early = true;
   c.max_units = ((rows + 255) / 256) * ((cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
   c.stream = st;
-  return launch_w4<false>(dev, c);
+  return launch_w4(dev, c, false);
 }
 
 // Both halves of a gated MLP on 4-bit weights, dense (moe.ids == NULL) or over experts.
@@ -365,6 +259,8 @@ static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const
   if ((rc = check_group(group, p->K))) return rc;
   if ((rc = check_group(group, p->N))) return rc;
   if ((rc = check_w4(g)) || (rc = check_w4(u)) || (rc = check_w4(d))) return rc;
+  if ((g.zero == nullptr) != (u.zero == nullptr))
+    return fail(GMLP_ERR_ARG, "gate and up weights must both have zeros or both have none");
   if ((rc = check_ptrs({x, y, work, scratch}))) return rc;
   const DeviceInfo* dev;
   if ((rc = device_info(&dev))) return rc;
@@ -404,7 +300,7 @@ static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const
   c.counters = reinterpret_cast<int*>(sc + l.counters1_off);
   c.early = !sparse;
   c.max_units = active * ((p->N + 127) / 128) * k_units;
-  if ((rc = launch_w4<true>(dev, c))) return rc;
+  if ((rc = launch_w4(dev, c, true))) return rc;
   if ((rc = launch_split(p->M, active * p->M, p->N, p->N, group, p->dtype, wk, wk + ww.t8_off, wk + ww.meta_off, true,
                          st)))
     return rc;
@@ -419,7 +315,7 @@ static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const
   c.counters = reinterpret_cast<int*>(sc + l.counters2_off);
   c.early = true;
   c.max_units = active * ((p->K + 255) / 256) * n_units;
-  return launch_w4<false>(dev, c);
+  return launch_w4(dev, c, false);
 }
 
 int gmlp_decode_fwd_w4(const gmlp_problem_t* p, int32_t group, const void* x, const void* w_gate4,

@@ -126,7 +126,7 @@ static uint32_t map_hash(const MapKey& k) {
 static unsigned dtype_bytes(int dtype) { return dtype == DTYPE_U8 ? 1u : dtype == GMLP_F32 ? 4u : 2u; }
 
 // 2-D row-major matrix [outer, inner] of 16-bit (DTYPE_U8: 8-bit, GMLP_F32: 32-bit) elements, swizzled rows of
-// `swizzle_bytes` (32 / 64 / 128), out-of-bounds elements read as zero and are not
+// `swizzle_bytes` (32 / 64 / 128; 0 = plain rows), out-of-bounds elements read as zero and are not
 // written by stores.
 int encode_map(CUtensorMap* m, const void* base, int64_t inner, int64_t outer,
                int64_t pitch_elems, uint32_t box_inner, uint32_t box_outer, int dtype,
@@ -145,7 +145,8 @@ int encode_map(CUtensorMap* m, const void* base, int64_t inner, int64_t outer,
                                  : dtype == GMLP_F32  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : dtype == GMLP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const CUtensorMapSwizzle sw = swizzle_bytes == 32   ? CU_TENSOR_MAP_SWIZZLE_32B
+  const CUtensorMapSwizzle sw = swizzle_bytes == 0    ? CU_TENSOR_MAP_SWIZZLE_NONE
+                                : swizzle_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
                                 : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                                       : CU_TENSOR_MAP_SWIZZLE_128B;
   const CUresult r = g_encode(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr,

@@ -99,11 +99,9 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
   volatile int* abortp = &abort_flag;
 
   const int row_tiles = (args.rows + 127) / 128;
-  const long long per_tile = DUAL ? args.kbt : static_cast<long long>(moe.n) * args.kbt;
-  const long long total = per_tile * (DUAL ? static_cast<long long>(moe.n) * row_tiles : row_tiles);
-  const long long ctas = total < gridDim.x ? total : gridDim.x;
-  const long long u_begin = blockIdx.x < ctas ? unit_start(blockIdx.x, total, ctas) : 0;
-  const long long u_end = blockIdx.x < ctas ? unit_start(blockIdx.x + 1, total, ctas) : 0;
+  const int per_tile = DUAL ? args.kbt : moe.n * args.kbt;
+  const Cut cut = make_cut(per_tile * (DUAL ? moe.n * row_tiles : row_tiles), gridDim.x);
+  const int u_begin = cut_start(cut, blockIdx.x), u_end = cut_start(cut, blockIdx.x + 1);
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA --
@@ -113,21 +111,21 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
       struct Pos {
         int a, rt, kb;
       };
-      auto pos_at = [&](long long u) {
+      auto pos_at = [&](int u) {
         Pos p;
-        const long long tile = u / per_tile, r = u - tile * per_tile;
+        const int tile = u / per_tile, r = u - tile * per_tile;
         if (DUAL) {
-          p.a = static_cast<int>(tile / row_tiles);
-          p.rt = static_cast<int>(tile - static_cast<long long>(p.a) * row_tiles);
-          p.kb = static_cast<int>(r);
+          p.a = tile / row_tiles;
+          p.rt = tile - p.a * row_tiles;
+          p.kb = r;
         } else {
-          p.rt = static_cast<int>(tile);
-          p.a = static_cast<int>(r / args.kbt);
-          p.kb = static_cast<int>(r - static_cast<long long>(p.a) * args.kbt);
+          p.rt = tile;
+          p.a = r / args.kbt;
+          p.kb = r - p.a * args.kbt;
         }
         return p;
       };
-      auto step = [&](Pos& p) {  // unit by unit: no 64-bit division in the issuing thread's loop
+      auto step = [&](Pos& p) {  // unit by unit: no division in the issuing thread's loop
         if (++p.kb < args.kbt) return;
         p.kb = 0;
         if (DUAL) {
@@ -156,15 +154,15 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
                          DUAL ? 0 : px.a * args.M, pol_x);
         step(px);
       };
-      long long u = u_begin;
+      int u = u_begin;
       if (args.early) {
-        const long long n0 = (u_end - u_begin) < STAGES ? (u_end - u_begin) : STAGES;
+        const int n0 = (u_end - u_begin) < STAGES ? (u_end - u_begin) : STAGES;
         for (int i = 0; i < n0; ++i) load_w(i);
         pdl_wait();
         for (int i = 0; i < n0; ++i) load_x(i);
         u += n0;
       }
-      int st = static_cast<int>((u - u_begin) % STAGES);
+      int st = (u - u_begin) % STAGES;
       uint32_t ph = static_cast<uint32_t>((u - u_begin) / STAGES) & 1u;
       bool ok = true;
       for (; u < u_end; ++u) {
@@ -182,9 +180,9 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
       if (!ok) {
         abort_flag = 1;
         atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_PRODUCER);
-        const long long done = u - u_begin;  // see the copies in flight land before the block leaves
-        for (long long i = done > STAGES ? done - STAGES : 0; i < done; ++i)
-          drain_wait(full_bar(static_cast<int>(i % STAGES)), static_cast<uint32_t>(i / STAGES) & 1u);
+        const int done = u - u_begin;  // see the copies in flight land before the block leaves
+        for (int i = done > STAGES ? done - STAGES : 0; i < done; ++i)
+          drain_wait(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u);
       }
     }
   } else if (warp == 1) {
@@ -193,7 +191,7 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
       int st = 0, seg = 0;
       uint32_t ph = 0;
       bool ok = true;
-      long long u = u_begin;
+      int u = u_begin;
       while (u < u_end && ok) {
         const Segment s = segment_at(u, u_end, per_tile);
         const int acc = seg & 1;
@@ -240,20 +238,39 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
     T* const out = static_cast<T*>(args.out);
     const T* const res = static_cast<const T*>(args.residual);
     const long long ld = args.rows;
-    if (!DUAL && total == 0) {
+    if (!DUAL && cut.total == 0) {
       // no token chose any expert: the outputs are the residual, or zero
       const long long all = static_cast<long long>(args.M) * args.rows;
       for (long long i = blockIdx.x * 128LL + ep_tid; i < all; i += gridDim.x * 128LL)
         out[i] = res ? res[i] : static_cast<T>(0.f);
     }
+    const Split sp{cut, args.M, reinterpret_cast<float4*>(args.slots), args.counters, args.status, abortp};
+    auto emit_tile = [&](int tile, int begin, int first, int last) {
+      if (DUAL) {
+        const int a = tile / row_tiles, row0 = (tile - a * row_tiles) * 128;
+        moe_factors(args.moe, args.M, moe.list[a], ep_tid, moe);
+        named_bar_sync(1, 128);
+        T* const oa = out + static_cast<long long>(a) * args.M * ld;
+        finish_tile<NACC, true, MPAD, 128>(begin, first, last, sp, ep_tid,
+                                           [&](int, int r, int i, const float4& gate, const float4& up) {
+          if (row0 + r < args.rows) emit_hidden(oa + row0 + r, ld, args.M, i, gate, up, 0.f, 0.f, args.act, &moe);
+        });
+      } else {
+        finish_tile<NACC, false, MPAD, 128>(begin, first, last, sp, ep_tid,
+                                            [&](int, int r, int i, const float4& v, const float4&) {
+          const int wr = tile * 128 + r;
+          if (wr < args.rows) emit_product(out + wr, res ? res + wr : nullptr, ld, args.M, i, v, 0.f, &moe);
+        });
+      }
+      named_bar_sync(1, 128);  // the slot, f and hit are free for the next tile
+    };
+    Pending pending;
+    bool alive = true;
     int seg = 0;
-    long long u = u_begin;
+    int u = u_begin;
     while (u < u_end) {
       const Segment s = segment_at(u, u_end, per_tile);
       const int acc = seg & 1;
-      const int a = DUAL ? static_cast<int>(s.tile / row_tiles) : 0;
-      const int rt = static_cast<int>(DUAL ? s.tile - static_cast<long long>(a) * row_tiles : s.tile);
-      if (DUAL) moe_factors(args.moe, args.M, moe.list[a], ep_tid, moe);  // seen behind the next barrier
       if (!mbar_wait_warp(tfull_bar(acc), (seg >> 1) & 1u, abortp, lane) && lane == 0) {
         abort_flag = 1;
         atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_EPILOGUE);
@@ -273,22 +290,11 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(tempty_bar(acc));
-      const Split sp{total,       ctas,   args.slots, args.counters,
-                     args.status, abortp, smem_base,  static_cast<int>(STAGES * STAGE_BYTES / (128 * 16))};
-      const int what = settle_segment<NACC, MPAD, MPAD, 128>(v, s, sp, args.M, 0, row, ep_tid);
-      if (what == SETTLE_ABORT) break;
-      const int wrow = rt * 128 + row;
-      if (what == SETTLE_EMIT && wrow < args.rows) {
-        if (DUAL)
-          store_hidden<MPAD>(args.act, out + static_cast<long long>(a) * args.M * ld + wrow, ld, args.M, 0, v[0],
-                             v[NACC - 1], 0.f, 0.f, &moe);
-        else
-          store_product<MPAD>(out + wrow, res ? res + wrow : nullptr, ld, args.M, 0, v[0], 0.f, &moe);
-      }
-      if (DUAL) named_bar_sync(1, 128);  // f and hit are overwritten for the next tile
+      if (!(alive = end_segment<NACC, MPAD, MPAD, 128>(v, s, sp, 0, row, ep_tid, pending, emit_tile))) break;
       u = s.end;
       ++seg;
     }
+    if (alive) end_units<128>(pending, per_tile, sp, ep_tid, emit_tile);
   }
 
   tc_fence_before_sync();

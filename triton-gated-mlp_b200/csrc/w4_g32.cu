@@ -1,0 +1,8 @@
+// The 4-bit stream kernels for groups of 32 columns.
+#include "few_token_host.cuh"
+
+namespace gmlp {
+int launch_w4_g32(const DeviceInfo* dev, const W4Call& c, bool dual) {
+  return dual ? launch_w4_group<0, true>(dev, c) : launch_w4_group<0, false>(dev, c);
+}
+}  // namespace gmlp

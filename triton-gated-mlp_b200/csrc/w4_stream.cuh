@@ -29,14 +29,19 @@
 //
 // Kernels of a product: w4_split_kernel (terms, powers of two and group sums of the activations, a few microseconds of
 // latency that hide behind the weight stream's start), then w4_stream_kernel.
-// Warps of w4_stream_kernel: 0 streams weights (TMA), 1 issues MMA, 2 streams activation terms (TMA), 3 streams scales
-// and zeros (4-byte cp.async: their rows have no alignment), 4..11 expand (four per tile, thread = row), then 4 (8 for
-// 64 tokens) accumulate and run the epilogue. Everything between two roles is a ring with full / empty barriers.
+// Warps of w4_stream_kernel: 0 streams weights (TMA), 1 issues MMA, 2 streams activation terms, scales and zeros (TMA), 3
+// scales and zeros whose rows are not aligned (cp.async), 4..11 expand (four per tile, thread = row), 12..19 take the sums
+// and run the epilogue (four per half of the tokens, thread = a row of both tiles). Everything between two roles is a ring with full / empty barriers, and
+// every ring turns once a unit (65,536 weights, 1,400 clocks at the copy bandwidth): a role that is one thread or one warp
+// executes an instruction every 5 to 10 clocks, so its instructions per unit are counted, and the group size is a template
+// parameter to keep them straight-line. (With hand-overs per 128 columns and run-time group loops the thread that
+// issues the MMAs was itself the bound, at 3,000 clocks per 32,768 weights.)
 //
 // Work split: stream-K over units of (two row tiles, 256 columns) as in few_token.cuh.
 #pragma once
-#include "few_token.cuh"
 #include <cuda_fp8.h>
+
+#include "few_token.cuh"
 
 namespace gmlp {
 
@@ -44,7 +49,7 @@ constexpr int W4_TILE_BYTES = 16384;  // 128 rows x 128 bytes: 256 columns
 constexpr int W4_UNIT_COLS = 256;
 constexpr int W4_HALF_COLS = 128;
 
-// Terms per activation and N of the MMA for MT token columns (a multiple of 16).
+// Terms per activation.
 template <typename T>
 __host__ __device__ constexpr int w4_terms() {
   return 2;
@@ -53,15 +58,12 @@ template <>
 __host__ __device__ constexpr int w4_terms<__half>() {
   return 3;
 }
-template <int MT, int TERMS>
-__host__ __device__ constexpr int w4_n() {
-  return (MT * TERMS + 15) / 16 * 16;
-}
 
 // ---- activations -> terms ----
 // x [R][cols] (row pitch ldx) -> t8 [TERMS][R][cols] e4m3 bytes, inside every 8 columns in the order in which
-// the masks of expand_word deliver a word's nibbles, and meta [R / M][cols / G][2][MT] floats: 2^-e, 2^-9 * sum.
-// 16 lanes take the 128 columns of a half unit (8 each); a group is 4, 8 or 16 lanes.
+// the expanders' masks deliver a word's nibbles, and meta [R / M][groups][2][MT] floats: 2^-e, 2^-9 * sum, with the groups
+// of a row padded to whole units of 256 columns (zeros there). 16 lanes take the 128 columns of a half unit (8 each);
+// a group is 4, 8 or 16 lanes.
 struct W4SplitArgs {
   const void* x;
   long long ldx;
@@ -80,7 +82,7 @@ w4_split_kernel(const W4SplitArgs args) {
   pdl_launch_dependents();
   if (args.dependent) pdl_wait();
   const int lane = threadIdx.x & 31, sub = lane & 15;
-  const int blocks = (args.cols + W4_HALF_COLS - 1) / W4_HALF_COLS;  // 128-column blocks of a row
+  const int blocks = (args.cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS * 2;  // half units of a row, padded to whole units
   const long long items = args.R * blocks;
   const long long item = (blockIdx.x * (W4_SPLIT_THREADS / 32LL) + (threadIdx.x >> 5)) * 2 + (lane >> 4);
   const long long row = item / blocks;
@@ -124,9 +126,9 @@ w4_split_kernel(const W4SplitArgs args) {
   }
   if (bad) sum = __uint_as_float(0x7fc00000u);  // a non-finite activation: the token's outputs become NaN
   for (int o = 1; o < width; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (live && (sub & (width - 1)) == 0) {
+  if (item < items && (sub & (width - 1)) == 0) {
     const long long a = row / args.M, m = row - a * args.M;
-    const int groups = args.cols >> (5 + args.gshift);
+    const int groups = blocks * (4 >> args.gshift);
     const long long g = col >> (5 + args.gshift);
     float* const p = args.meta + ((a * groups + g) * 2) * args.MT + m;
     p[0] = sum != sum ? sum : down;
@@ -135,54 +137,72 @@ w4_split_kernel(const W4SplitArgs args) {
 }
 
 // ---- the stream ----
+struct W4Maps {
+  CUtensorMap w0, w1, x;
+  CUtensorMap s0, s1, z0, z1;  // scales and zeros, where W4Args::wide
+};
 struct W4Args {
   int M;
   int rows;        // weight rows per expert (N for DUAL, outputs otherwise)
   int kbt;         // units along an expert's columns: ceil(cols / 256)
   int groups;      // cols / G
-  int gshift;      // log2(G / 32): 0, 1, 2
-  int gpg;         // groups per accumulator buffer (1, 2, 4): as many of a half unit as fit 128 columns
-  int acc_bufs;    // accumulator buffers of gpg * N columns
   long long R;     // rows of a plane of activation terms
-  uint32_t idesc;
   int* status;
-  const float* meta;     // [experts in h or 1][groups][2][MT]
+  const float* meta;       // [experts in h or 1][kbt * groups per unit][2][MT]
   const uint16_t* scale0;  // [experts][groups][rows], T
   const uint16_t* scale1;  // DUAL: the up matrix's
-  const uint8_t* zero0;  // [experts][groups][rows] or null (8)
+  const uint8_t* zero0;    // [experts][groups][rows] or null (8)
   const uint8_t* zero1;
-  const void* bias0;     // [rows] or null
+  const void* bias0;       // [rows] or null
   const void* bias1;
-  const void* residual;  // [M][rows] or null (DUAL = false)
-  void* out;             // [M][rows]; DUAL on experts: [active][M][rows]
+  const void* residual;    // [M][rows] or null (DUAL = false)
+  void* out;               // [M][rows]; DUAL on experts: [active][M][rows]
   float* slots;
   int* counters;
   int act;
+  int wide;   // scales and zeros go by TMA: rows are a multiple of 16 and the arrays 16-byte aligned
   int early;  // the weights may be streamed before the preceding kernel has finished
   MoeTable moe;
 };
 
-template <int MT, int TERMS>
+// Scales and zeros of a unit in shared memory. Copied by TMA: [2 tiles][groups][128] scales, then zeros alike. Copied by
+// words (rows that are not aligned start up to 3 bytes into a word): 416 bytes per (tile, group), zeros from byte 272.
+constexpr int W4_META_ROW = 416;
+constexpr int W4_META_ZERO = 272;
+
+template <int MT, int TERMS, int GSHIFT>
 struct W4Conf {
-  static constexpr int N = w4_n<MT, TERMS>();
-  static constexpr int ACC_WARPS = MT == 64 ? 8 : 4;
-  static constexpr int THREADS = 32 * (12 + ACC_WARPS);
-  static constexpr int COLS = MT == 64 ? 32 : MT;  // tokens per accumulator thread
-  static constexpr int X_TILE = N * 128;           // terms of a half unit: N rows of 128 columns
-  static constexpr int X_STAGE = X_TILE + 4 * 2 * MT * 4;  // + meta of up to four groups, rounded to 1 KB
-  static constexpr int X_STAGE_AL = (X_STAGE + 1023) / 1024 * 1024;
-  static constexpr int X_STAGES = 4;
-  static constexpr int M_BYTES = 12800;  // scales and zeros: four half units at G = 32, sixteen at G = 128
-  static constexpr int LEFT = 232448 - 1024 - 4096 - X_STAGES * X_STAGE_AL - M_BYTES;
-  static constexpr int W_STAGES = LEFT / (2 * W4_TILE_BYTES) > 5 ? 5 : LEFT / (2 * W4_TILE_BYTES);
-  static constexpr size_t SMEM = 1024 + static_cast<size_t>(W_STAGES) * 2 * W4_TILE_BYTES + X_STAGES * X_STAGE_AL + M_BYTES;
-  // tensor memory: accumulators in front, expanded weights (64 columns per half unit) behind
-  static constexpr int A_BUFS = N > 128 ? 2 : 4;
-  static constexpr int C_COLS = 512 - A_BUFS * 64;
-  static constexpr int MAX_ACC_BUFS = 8;
-  static_assert(W_STAGES >= 3, "ring too shallow");
+  static constexpr int N = MT < 16 ? 16 : MT;      // columns of the MMA; those behind MT hold nothing of use
+  static constexpr int THREADS = 32 * 20;
+  static constexpr int GPH = 4 >> GSHIFT;          // groups per half unit (128 columns)
+  static constexpr int GPU = 2 * GPH;              // groups per unit
+  // activation terms of a unit: [two halves][TERMS] of N rows x 128 columns, then meta [GPU][2][MT]
+  static constexpr int X_TERM = N * 128;
+  static constexpr int X_HALF = TERMS * X_TERM;
+  static constexpr int X_STAGE = (2 * X_HALF + GPU * 2 * MT * 4 + 1023) / 1024 * 1024;
+  static constexpr int M_STAGE = 2 * GPU * W4_META_ROW;  // scales and zeros of a unit
+  static constexpr int COLS = MT / 2;  // tokens per accumulator thread
+  static constexpr int SMEM_MAX = 232448 - 1024 - 4096;
+  static constexpr int X_STAGES = 3 * (X_STAGE + M_STAGE) + 3 * 2 * W4_TILE_BYTES <= SMEM_MAX ? 3 : 2;
+  static constexpr int FIT = (SMEM_MAX - X_STAGES * (X_STAGE + M_STAGE)) / (2 * W4_TILE_BYTES);
+  static constexpr int W_STAGES = FIT > 5 ? 5 : FIT;
+  static constexpr size_t SMEM = 1024 + static_cast<size_t>(W_STAGES) * 2 * W4_TILE_BYTES + X_STAGES * (X_STAGE + M_STAGE);
+  // tensor memory: accumulators in front, expanded weights (128 columns per unit) behind. An accumulator buffer holds as
+  // many (tile, group) sums of a unit as leave room for two buffers.
+  static constexpr int A_BUFS = 2;
+  static constexpr int C_COLS = 512 - A_BUFS * 128;
+  static constexpr int PAIRS = 2 * GPU;  // (half, group, tile) sums of a unit
+  static constexpr int fit_pairs() {
+    int p = PAIRS;
+    while (p > 1 && 2 * p * N > C_COLS) p /= 2;
+    return p;
+  }
+  static constexpr int BUF_PAIRS = fit_pairs();
+  static_assert(BUF_PAIRS >= 2, "a buffer holds both tiles' sums of a group");
+  static constexpr int C_BUFS_FIT = C_COLS / (BUF_PAIRS * N);
+  static constexpr int C_BUFS = C_BUFS_FIT > 4 ? 4 : C_BUFS_FIT;
+  static_assert(W_STAGES >= 3 && C_BUFS >= 2, "rings too shallow");
 };
-constexpr int W4_META_ROW = 400;  // 66 words of scales, 34 words of zeros of one (tile, group)
 
 // ---- tensor memory and MMA ----
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -197,11 +217,22 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr)
-               : "memory");
+template <int COLS>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t* r) {
+  if constexpr (COLS == 4) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int c = 0; c < COLS; c += 8)
+      asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r[c]), "=r"(r[c + 1]), "=r"(r[c + 2]), "=r"(r[c + 3]), "=r"(r[c + 4]), "=r"(r[c + 5]),
+                     "=r"(r[c + 6]), "=r"(r[c + 7])
+                   : "r"(taddr + c)
+                   : "memory");
+  }
 }
 // D[tmem] (+)= A[tmem] * B[smem], e4m3: A is 128 lanes x 8 columns, four elements a column (32 of the reduction).
 __device__ __forceinline__ void umma_f8_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
@@ -238,33 +269,28 @@ __device__ __forceinline__ uint4 ld_shared_u4(uint32_t a) {
                : "memory");
   return v;
 }
-__device__ __forceinline__ uint32_t ld_shared_u16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t ld_shared_u8(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
 
-// Bounded wait of a whole warp (or of one thread, WARP = false) that polls without the suspend hint of mbar_wait: the
-// hand-over from warp to warp takes 125 clocks instead of 213 (measured), and these roles hand over every few
-// hundred clocks.
-template <bool WARP>
+// Bounded wait of a whole warp that polls without the suspend hint of mbar_wait: the hand-over from warp to warp takes
+// 125 clocks instead of 213 (measured), and these roles hand over every few hundred clocks.
 __device__ __forceinline__ bool quick_wait(uint32_t bar, uint32_t parity, volatile int* abortp) {
   long long t0 = 0;
   for (int i = 0;; ++i) {
-    const bool ok = mbar_try_wait(bar, parity);
-    if (WARP ? __all_sync(0xffffffffu, ok) : ok) return true;
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     if ((i & 63) == 63) {
       const long long t = clock64();
       if (t0 == 0) t0 = t;
-      const bool stop = *abortp != 0 || t - t0 > WAIT_LIMIT_CYCLES;
-      if (WARP ? __any_sync(0xffffffffu, stop) : stop) return false;
+      if (__any_sync(0xffffffffu, *abortp != 0 || t - t0 > WAIT_LIMIT_CYCLES)) return false;
     }
   }
+}
+
+// One thread of a converged warp. The single-thread roles run their loops with the whole warp and elect a thread for
+// the issue itself: addresses and descriptors then live in uniform registers, and an MMA is issued every 15 clocks
+// instead of every 45 from inside an `if (lane == 0)` (measured, N = 16).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(p));
+  return p != 0;
 }
 
 // Ring position: index and the parity of its phase.
@@ -279,45 +305,37 @@ struct Ring {
   }
 };
 
-// Walks the units of a CTA: position inside the list of active experts (a) and along an expert's columns (kb).
+// Position of a unit: a in the list of active experts, kb along that expert's columns, first row of its tile.
 struct W4Walk {
-  long long left;  // units of the current row tile from here on (of all CTAs)
-  long long tile;
   int a, kb, row0;
 };
 
-template <int MT, bool DUAL, typename T>
-__global__ void __launch_bounds__(W4Conf<MT, w4_terms<T>()>::THREADS, 1)
-w4_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant__ CUtensorMap tmW1,
-                 const __grid_constant__ CUtensorMap tmX, const W4Args args) {
+template <int MT, bool DUAL, typename T, int GSHIFT>
+__global__ void __launch_bounds__(W4Conf<MT, w4_terms<T>(), GSHIFT>::THREADS, 1)
+w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   constexpr int TERMS = w4_terms<T>();
-  using C = W4Conf<MT, TERMS>;
-  constexpr int N = C::N, COLS = C::COLS, ACC_WARPS = C::ACC_WARPS, ACC_THREADS = 32 * ACC_WARPS;
-  constexpr int NW = C::W_STAGES, NX = C::X_STAGES, NA = C::A_BUFS, MAXC = C::MAX_ACC_BUFS;
+  using C = W4Conf<MT, TERMS, GSHIFT>;
+  constexpr int N = C::N;
+  constexpr int NW = C::W_STAGES, NX = C::X_STAGES, NA = C::A_BUFS, NC = C::C_BUFS;
+  constexpr int GPH = C::GPH, GPU = C::GPU, PAIRS = C::PAIRS, BUF_PAIRS = C::BUF_PAIRS;
+  constexpr int KSTEPS = 1 << GSHIFT;     // 32-column MMA steps per group
   constexpr int ROWS = DUAL ? 128 : 256;  // weight rows per row tile
-  constexpr int NM_MAX = 16;
 
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * NW + 2 * NX + 2 * NM_MAX + 2 * NA + 2 * MAXC + 1];
+  __shared__ __align__(8) uint64_t bars[2 * (NW + NX + NA + NC) + 1];
   __shared__ uint32_t tmem_base_holder;
   __shared__ int abort_flag;
   __shared__ MoeShared moe;
 
   const uint32_t w_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint8_t* const smem = smem_raw + (w_base - smem_u32(smem_raw));
   const uint32_t x_base = w_base + NW * 2 * W4_TILE_BYTES;
-  const uint32_t m_base = x_base + NX * C::X_STAGE_AL;
-  uint32_t b_at = smem_u32(bars);
-  const uint32_t wfull = b_at, wempty = wfull + 8 * NW, xfull = wempty + 8 * NW, xempty = xfull + 8 * NX,
-                 mfull = xempty + 8 * NX, mempty = mfull + 8 * NM_MAX, afull = mempty + 8 * NM_MAX,
-                 aempty = afull + 8 * NA, cfull = aempty + 8 * NA, cempty = cfull + 8 * MAXC,
-                 drain_bar = cempty + 8 * MAXC;
+  const uint32_t m_base = x_base + NX * C::X_STAGE;
+  const uint32_t wfull = smem_u32(bars), wempty = wfull + 8 * NW, xfull = wempty + 8 * NW, xempty = xfull + 8 * NX,
+                 afull = xempty + 8 * NX, aempty = afull + 8 * NA, cfull = aempty + 8 * NA, cempty = cfull + 8 * NC, drain_bar = cempty + 8 * NC;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int gph = 4 >> args.gshift;        // groups per half unit
-  const int gpu_ = 2 * gph;                // groups per unit
-  const int nm = 16 / gph;                 // ring of scales and zeros, in half units
-  const uint32_t m_stage = 2 * gph * W4_META_ROW;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < NW; ++s) {
@@ -325,27 +343,22 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant
       mbar_init(wempty + 8 * s, 8);
     }
     for (int s = 0; s < NX; ++s) {
-      mbar_init(xfull + 8 * s, 1);
-      mbar_init(xempty + 8 * s, 1 + ACC_WARPS);
-    }
-    for (int s = 0; s < NM_MAX; ++s) {
-      mbar_init(mfull + 8 * s, 32);
-      mbar_init(mempty + 8 * s, ACC_WARPS);
+      mbar_init(xfull + 8 * s, args.wide ? 1 : 1 + 32);  // the TMA bytes, and the copying lanes of warp 3
+      mbar_init(xempty + 8 * s, 1 + 8);
     }
     for (int b = 0; b < NA; ++b) {
       mbar_init(afull + 8 * b, 8);
       mbar_init(aempty + 8 * b, 1);
     }
-    for (int b = 0; b < MAXC; ++b) {
+    for (int b = 0; b < NC; ++b) {
       mbar_init(cfull + 8 * b, 1);
-      mbar_init(cempty + 8 * b, ACC_WARPS);
+      mbar_init(cempty + 8 * b, 8);
     }
     mbar_init(drain_bar, 1);
     mbar_fence_init();
     fence_proxy_async_smem();
-    tma_prefetch_desc(&tmW0);
-    tma_prefetch_desc(&tmX);
   }
+  if (warp == 2 && lane < 7) tma_prefetch_desc(&maps.w0 + lane);
   if (warp == 1) {
     tmem_alloc(smem_u32(&tmem_base_holder), 512);
     tmem_relinquish();
@@ -363,150 +376,167 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant
 
   // Units: DUAL: tile = (expert, row tile), kbt units each. Else: tile = row tile, units = (expert, kb).
   const int row_tiles = (args.rows + ROWS - 1) / ROWS;
-  const long long per_tile = DUAL ? args.kbt : static_cast<long long>(moe.n) * args.kbt;
-  const long long total = per_tile * (DUAL ? static_cast<long long>(moe.n) * row_tiles : row_tiles);
-  const long long ctas = total < gridDim.x ? total : gridDim.x;
-  const long long u_begin = blockIdx.x < ctas ? unit_start(blockIdx.x, total, ctas) : 0;
-  const long long u_end = blockIdx.x < ctas ? unit_start(blockIdx.x + 1, total, ctas) : 0;
+  const int per_tile = DUAL ? args.kbt : moe.n * args.kbt;
+  const Cut cut = make_cut(per_tile * (DUAL ? moe.n * row_tiles : row_tiles), gridDim.x);
+  const int u_begin = cut_start(cut, blockIdx.x), u_end = cut_start(cut, blockIdx.x + 1);
+  const int units = u_end - u_begin;
 
-  auto enter = [&](W4Walk& w, long long tile, long long r) {  // unit r of the tile
-    w.tile = tile;
-    w.left = per_tile - r;
-    if (DUAL) {
-      w.a = static_cast<int>(tile / row_tiles);
-      w.row0 = static_cast<int>(tile - static_cast<long long>(w.a) * row_tiles) * ROWS;
-      w.kb = static_cast<int>(r);
-    } else {
-      w.row0 = static_cast<int>(tile) * ROWS;
-      w.a = static_cast<int>(r / args.kbt);
-      w.kb = static_cast<int>(r - static_cast<long long>(w.a) * args.kbt);
-    }
-  };
   auto start = [&](W4Walk& w) {
-    if (u_begin < u_end) {
-      const long long tile = u_begin / per_tile;
-      enter(w, tile, u_begin - tile * per_tile);
+    w.a = w.kb = w.row0 = 0;
+    if (units == 0) return;
+    const int tile = u_begin / per_tile, r = u_begin - tile * per_tile;
+    if (DUAL) {
+      w.a = tile / row_tiles;
+      w.row0 = (tile - w.a * row_tiles) * ROWS;
+      w.kb = r;
+    } else {
+      w.row0 = tile * ROWS;
+      w.a = r / args.kbt;
+      w.kb = r - w.a * args.kbt;
     }
   };
-  auto step = [&](W4Walk& w) {
-    if (--w.left == 0) {
-      enter(w, w.tile + 1, 0);
-    } else if (++w.kb == args.kbt) {
-      w.kb = 0;
-      ++w.a;
+  auto step = [&](W4Walk& w) {  // the next unit, without a division
+    if (++w.kb < args.kbt) return;
+    w.kb = 0;
+    if (DUAL) {
+      w.row0 += ROWS;
+      if (w.row0 >= args.rows) {
+        w.row0 = 0;
+        ++w.a;
+      }
+    } else if (++w.a == moe.n) {
+      w.a = 0;
+      w.row0 += ROWS;
     }
   };
-  auto groups_in = [&](int kb, int half) {  // groups of a half unit that exist
-    const int left = args.groups - kb * gpu_ - half * gph;
-    return left < gph ? left : gph;
+  // groups of the unit that exist: GPU but for the last unit of an expert's columns
+  auto groups_in = [&](int kb) {
+    const int left = args.groups - kb * GPU;
+    return left < GPU ? left : GPU;
   };
 
+  // 64 tokens: 640 threads leave 96 registers each, 64 sums a thread want more. Of the block's 640 x 96 = 61,440 the helpers
+  // keep 56 and the expanders 64 a thread, the accumulators get 144: 128 x (56 + 2 x 64 + 2 x 144) = 60,416.
   if (warp == 0) {
     // ------------------------------------------------------------ weights --
-    if (lane == 0) {
-      const uint64_t pol = l2_policy_evict_first();
-      W4Walk w;
-      start(w);
-      Ring r;
-      long long u = u_begin;
-      bool ok = true;
-      for (; u < u_end; ++u) {
-        if (!(ok = quick_wait<false>(wempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
-        const uint32_t dst = w_base + r.at * 2 * W4_TILE_BYTES, fb = wfull + 8 * r.at;
-        const int y = moe.list[w.a] * args.rows + w.row0;
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const uint64_t pol = l2_policy_evict_first();
+    W4Walk w;
+    start(w);
+    Ring r;
+    int u = 0;
+    bool ok = true;
+    for (; u < units; ++u) {
+      if (!(ok = quick_wait(wempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
+      const uint32_t dst = w_base + r.at * 2 * W4_TILE_BYTES, fb = wfull + 8 * r.at;
+      const int y = moe.list[w.a] * args.rows + w.row0;
+      if (elect_one()) {
         mbar_expect_tx(fb, 2 * W4_TILE_BYTES);
-        tma_load_2d_hint(dst, &tmW0, fb, w.kb * 128, y, pol);
+        tma_load_2d_hint(dst, &maps.w0, fb, w.kb * 128, y, pol);
         if (DUAL)
-          tma_load_2d_hint(dst + W4_TILE_BYTES, &tmW1, fb, w.kb * 128, y, pol);
+          tma_load_2d_hint(dst + W4_TILE_BYTES, &maps.w1, fb, w.kb * 128, y, pol);
         else
-          tma_load_2d_hint(dst + W4_TILE_BYTES, &tmW0, fb, w.kb * 128, y + 128, pol);
-        step(w);
-        r.next(NW);
+          tma_load_2d_hint(dst + W4_TILE_BYTES, &maps.w0, fb, w.kb * 128, y + 128, pol);
       }
-      if (!ok) {
-        abort_flag = 1;
-        atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_PRODUCER);
-        const long long done = u - u_begin;  // see the copies in flight land before the block leaves
-        for (long long i = done > NW ? done - NW : 0; i < done; ++i)
-          drain_wait(wfull + 8 * static_cast<int>(i % NW), static_cast<uint32_t>(i / NW) & 1u);
-      }
+      __syncwarp();
+      step(w);
+      r.next(NW);
+    }
+    if (!ok && lane == 0) {
+      abort_flag = 1;
+      atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_PRODUCER);
+      for (int i = u > NW ? u - NW : 0; i < u; ++i)  // see the copies in flight land before the block leaves
+        drain_wait(wfull + 8 * (i % NW), static_cast<uint32_t>(i / NW) & 1u);
     }
   } else if (warp == 2) {
     // -------------------------------------------------------- activations --
-    if (lane == 0) {
-      if (args.early) pdl_wait();
-      const uint64_t pol = l2_policy_evict_last();
-      W4Walk w;
-      start(w);
-      Ring r;
-      bool ok = true;
-      long long done = 0;
-      for (long long u = u_begin; u < u_end && ok; ++u) {
-        const int a = DUAL ? 0 : w.a;
-        for (int h = 0; h < 2; ++h) {
-          const int ng = groups_in(w.kb, h);
-          if (ng <= 0) break;
-          if (!(ok = quick_wait<false>(xempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
-          const uint32_t dst = x_base + r.at * C::X_STAGE_AL, fb = xfull + 8 * r.at;
-          const uint32_t meta_bytes = ng * 2 * MT * 4;
-          mbar_expect_tx(fb, TERMS * MT * 128 + meta_bytes);
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t)
-            tma_load_2d_hint(dst + t * MT * 128, &tmX, fb, w.kb * W4_UNIT_COLS + h * W4_HALF_COLS,
-                             static_cast<int>(t * args.R) + a * args.M, pol);
-          bulk_load(dst + C::X_TILE,
-                    args.meta + (static_cast<long long>(a) * args.groups + w.kb * gpu_ + h * gph) * 2 * MT, meta_bytes, fb);
-          r.next(NX);
-          ++done;
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (args.early) pdl_wait();
+    const uint64_t pol = l2_policy_evict_last(), pol_w = l2_policy_evict_first();
+    W4Walk w;
+    start(w);
+    Ring r;
+    int u = 0;
+    bool ok = true;
+    for (; u < units; ++u) {
+      if (!(ok = quick_wait(xempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
+      const int a = DUAL ? 0 : w.a;
+      const uint32_t dst = x_base + r.at * C::X_STAGE, fb = xfull + 8 * r.at;
+      constexpr uint32_t META_BYTES = GPU * 2 * MT * 4;
+      if (elect_one()) {
+        const uint32_t sz_bytes = args.wide ? 2 * GPU * 128 * (2 + (args.zero0 != nullptr ? 1 : 0)) : 0;
+        mbar_expect_tx(fb, 2 * TERMS * MT * 128 + META_BYTES + sz_bytes);
+        if (args.wide) {
+          const uint32_t md = m_base + r.at * C::M_STAGE;
+          const int gy = moe.list[w.a] * args.groups + w.kb * GPU;
+          tma_load_2d_hint(md, &maps.s0, fb, w.row0, gy, pol_w);
+          tma_load_2d_hint(md + GPU * 256, DUAL ? &maps.s1 : &maps.s0, fb, w.row0 + (DUAL ? 0 : 128), gy, pol_w);
+          if (args.zero0 != nullptr) {
+            tma_load_2d_hint(md + 2 * GPU * 256, &maps.z0, fb, w.row0, gy, pol_w);
+            tma_load_2d_hint(md + 2 * GPU * 256 + GPU * 128, DUAL ? &maps.z1 : &maps.z0, fb, w.row0 + (DUAL ? 0 : 128), gy,
+                             pol_w);
+          }
         }
-        step(w);
+#pragma unroll
+        for (int i = 0; i < 2 * TERMS; ++i)  // a half behind the last column arrives as zeros
+          tma_load_2d_hint(dst + i * C::X_TERM, &maps.x, fb, w.kb * W4_UNIT_COLS + (i / TERMS) * W4_HALF_COLS,
+                           static_cast<int>((i % TERMS) * args.R) + a * args.M, pol);
+        bulk_load(dst + 2 * C::X_HALF, args.meta + (static_cast<long long>(a) * args.kbt + w.kb) * (GPU * 2 * MT),
+                  META_BYTES, fb);
       }
-      if (!ok) {
-        abort_flag = 1;
-        atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_PRODUCER);
-        for (long long i = done > NX ? done - NX : 0; i < done; ++i)
-          drain_wait(xfull + 8 * static_cast<int>(i % NX), static_cast<uint32_t>(i / NX) & 1u);
-      }
+      __syncwarp();
+      step(w);
+      r.next(NX);
+    }
+    if (!ok && lane == 0) {
+      abort_flag = 1;
+      atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_PRODUCER);
+      for (int i = u > NX ? u - NX : 0; i < u; ++i)
+        drain_wait(xfull + 8 * (i % NX), static_cast<uint32_t>(i / NX) & 1u);
     }
   } else if (warp == 3) {
     // --------------------------------------------------- scales and zeros --
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    // Rows of scales and zeros start anywhere (any number of weight rows is allowed): copied by 4-byte words, up to 65 + 33
+    // per (tile, group), of which the last one only as far as the rows go.
     W4Walk w;
     start(w);
     Ring r;
     bool ok = true;
-    for (long long u = u_begin; u < u_end && ok; ++u) {
-      for (int h = 0; h < 2; ++h) {
-        const int ng = groups_in(w.kb, h);
-        if (ng <= 0) break;
-        if (!(ok = quick_wait<true>(mempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
+    for (int u = 0; u < units && !args.wide; ++u) {
+      if (!(ok = quick_wait(xempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
+      const int ng = groups_in(w.kb);
+      const long long unit0 = (static_cast<long long>(moe.list[w.a]) * args.groups + w.kb * GPU) * args.rows + w.row0;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint16_t* const sc = (DUAL && t == 1) ? args.scale1 : args.scale0;
-          const uint8_t* const ze = (DUAL && t == 1) ? args.zero1 : args.zero0;
-          const int row = w.row0 + (DUAL ? 0 : t * 128);
-          const int nrow = args.rows - row < 128 ? args.rows - row : 128;
-          if (nrow <= 0) continue;
+      for (int t = 0; t < 2; ++t) {
+        const uint16_t* const sc = (DUAL && t == 1) ? args.scale1 : args.scale0;
+        const uint8_t* const ze = (DUAL && t == 1) ? args.zero1 : args.zero0;
+        const int skip = DUAL ? 0 : t * 128;
+        const int left = args.rows - w.row0 - skip;
+        const int nrow = left < 128 ? left : 128;
+#pragma unroll 1
           for (int i = 0; i < ng; ++i) {
-            const long long e0 =
-                (static_cast<long long>(moe.list[w.a]) * args.groups + w.kb * gpu_ + h * gph + i) * args.rows + row;
-            const uint32_t dst = m_base + r.at * m_stage + (t * gph + i) * W4_META_ROW;
-            // words that hold rows row .. row + nrow - 1; the last one only as far as the rows go
-            const int head = static_cast<int>(e0 & 1) * 2, bytes = head + 2 * nrow;
-            const char* const s0 = reinterpret_cast<const char*>(sc + e0) - head;
-            for (int k = lane * 4; k < bytes; k += 128)
-              cp_async_word(dst + k, s0 + k, bytes - k < 4 ? bytes - k : 4);
+            if (nrow <= 0) continue;
+            const long long e0 = unit0 + skip + static_cast<long long>(i) * args.rows;
+            const uint32_t dst = m_base + r.at * C::M_STAGE + (t * GPU + i) * W4_META_ROW + lane * 4;
+            const int head = static_cast<int>(e0 & 1) * 2, bytes = head + 2 * nrow - lane * 4;
+            const char* const s0 = reinterpret_cast<const char*>(sc + e0) - head + lane * 4;
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+              if (bytes > k * 128) cp_async_word(dst + k * 128, s0 + k * 128, bytes - k * 128 < 4 ? bytes - k * 128 : 4);
             if (ze != nullptr) {
-              const int zhead = static_cast<int>(e0 & 3), zbytes = zhead + nrow;
-              const uint8_t* const z0 = ze + e0 - zhead;
-              for (int k = lane * 4; k < zbytes; k += 128)
-                cp_async_word(dst + 264 + k, z0 + k, zbytes - k < 4 ? zbytes - k : 4);
+              const int zhead = static_cast<int>(e0 & 3), zbytes = zhead + nrow - lane * 4;
+              const uint8_t* const z0 = ze + e0 - zhead + lane * 4;
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                if (zbytes > k * 128)
+                  cp_async_word(dst + W4_META_ZERO + k * 128, z0 + k * 128, zbytes - k * 128 < 4 ? zbytes - k * 128 : 4);
             }
           }
-        }
-        cp_async_arrive(mfull + 8 * r.at);
-        r.next(nm);
       }
+      cp_async_arrive(xfull + 8 * r.at);
       step(w);
+      r.next(NX);
     }
     if (!ok && lane == 0) {
       abort_flag = 1;
@@ -515,92 +545,97 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant
     cp_async_wait_all();
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA --
-    if (lane == 0) {
-      W4Walk w;
-      start(w);
-      Ring rx, ra, rc;
-      const int ksteps = 1 << args.gshift;  // 32-column steps per group
-      const uint32_t c_cols = args.gpg * N;
-      bool ok = true;
-      for (long long u = u_begin; u < u_end && ok; ++u) {
-        for (int h = 0; h < 2 && ok; ++h) {
-          const int ng = groups_in(w.kb, h);
-          if (ng <= 0) break;
-          if (!(ok = quick_wait<false>(xfull + 8 * rx.at, rx.phase, abortp))) break;
-          if (!(ok = quick_wait<false>(afull + 8 * ra.at, ra.phase, abortp))) break;
-          const uint64_t xd = make_smem_desc(x_base + rx.at * C::X_STAGE_AL, 16, 1024);
-          const uint32_t a0 = tmem_base + C::C_COLS + ra.at * 64;
-          for (int t = 0; t < 2 && ok; ++t) {
-            for (int g0 = 0; g0 < ng; g0 += args.gpg) {
-              if (!(ok = quick_wait<false>(cempty + 8 * rc.at, rc.phase ^ 1u, abortp))) break;
-              tc_fence_after_sync();
-              const int ge = g0 + args.gpg < ng ? g0 + args.gpg : ng;
-              uint32_t d = tmem_base + rc.at * c_cols;
-              for (int g = g0; g < ge; ++g, d += N) {
-                const int k0 = g * ksteps;
-                for (int k = 0; k < ksteps; ++k)
-                  umma_f8_ts(d, a0 + t * 32 + (k0 + k) * 8, xd + static_cast<uint64_t>(2 * (k0 + k)), args.idesc,
-                             k > 0 ? 1u : 0u);
-              }
-              umma_commit(cfull + 8 * rc.at);
-              rc.next(args.acc_bufs);
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    constexpr uint32_t IDESC = make_idesc_f8(128, N);
+    const uint64_t x0 = make_smem_desc(x_base, 16, 1024);
+    Ring rx, ra, rc;
+    bool ok = true;
+    for (int u = 0; u < units && ok; ++u) {
+      if (!(ok = quick_wait(xfull + 8 * rx.at, rx.phase, abortp))) break;
+      if (!(ok = quick_wait(afull + 8 * ra.at, ra.phase, abortp))) break;
+      const uint64_t xd = x0 + static_cast<uint64_t>(rx.at * (C::X_STAGE >> 4));
+      const uint32_t a0 = tmem_base + C::C_COLS + ra.at * 128;
+      // sums in the order (half, group, tile); groups behind the last column are zeros
+#pragma unroll
+      for (int p0 = 0; p0 < PAIRS; p0 += BUF_PAIRS) {
+        if (!(ok = quick_wait(cempty + 8 * rc.at, rc.phase ^ 1u, abortp))) break;
+        tc_fence_after_sync();
+        const uint32_t d = tmem_base + rc.at * (BUF_PAIRS * N);
+        if (elect_one()) {
+#pragma unroll
+          for (int p = p0; p < p0 + BUF_PAIRS; ++p) {
+            const int t = p & 1, h = p / (2 * GPH), g = (p >> 1) % GPH;
+#pragma unroll
+            for (int k = 0; k < KSTEPS; ++k) {
+              const int kk = g * KSTEPS + k;  // 32-column step inside the half
+#pragma unroll
+              for (int i = 0; i < TERMS; ++i)
+                umma_f8_ts(d + (p - p0) * N, a0 + t * 64 + h * 32 + kk * 8,
+                           xd + static_cast<uint64_t>(((h * TERMS + i) * C::X_TERM >> 4) + 2 * kk), IDESC,
+                           k + i > 0 ? 1u : 0u);
             }
           }
-          if (!ok) break;
-          umma_commit(aempty + 8 * ra.at);
-          umma_commit(xempty + 8 * rx.at);
-          ra.next(NA);
-          rx.next(NX);
+          umma_commit(cfull + 8 * rc.at);
+          if (p0 + BUF_PAIRS == PAIRS) {
+            umma_commit(aempty + 8 * ra.at);
+            umma_commit(xempty + 8 * rx.at);
+          }
         }
-        step(w);
+        __syncwarp();
+        rc.next(NC);
       }
-      if (!ok) {
-        abort_flag = 1;
-        atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_MMA);
-        umma_commit(drain_bar);
-        drain_wait(drain_bar, 0);
-      }
+      ra.next(NA);
+      rx.next(NX);
+    }
+    if (!ok && lane == 0) {
+      abort_flag = 1;
+      atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_MMA);
+      umma_commit(drain_bar);
+      drain_wait(drain_bar, 0);
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------- expand --
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int quarter = warp & 3;
     const int tsel = (warp - 4) >> 2;  // which of the unit's two tiles
     const int row = quarter * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    W4Walk w;
-    start(w);
+    const uint32_t src0 = w_base + tsel * W4_TILE_BYTES + row * 128;
+    const uint32_t dst0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + C::C_COLS + tsel * 64;
     Ring rw, ra;
     bool ok = true;
-    for (long long u = u_begin; u < u_end && ok; ++u) {
-      if (!(ok = quick_wait<true>(wfull + 8 * rw.at, rw.phase, abortp))) break;
-      const uint32_t src = w_base + rw.at * 2 * W4_TILE_BYTES + tsel * W4_TILE_BYTES + row * 128;
-      const int halves = groups_in(w.kb, 1) > 0 ? 2 : 1;
-      for (int h = 0; h < halves; ++h) {
-        uint4 q[4];
+    for (int u = 0; u < units; ++u) {
+      if (!(ok = quick_wait(wfull + 8 * rw.at, rw.phase, abortp))) break;
+      const uint32_t src = src0 + rw.at * 2 * W4_TILE_BYTES;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) q[c] = ld_shared_u4(src + (((h * 4 + c) ^ (row & 7)) << 4));
+      for (int h = 0; h < 2; ++h) {
         uint32_t r[32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const uint32_t word[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+          const uint4 q = ld_shared_u4(src + (((h * 4 + c) ^ (row & 7)) << 4));
+          const uint32_t word[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             r[c * 8 + 2 * i] = word[i] & 0x0F0F0F0Fu;
             r[c * 8 + 2 * i + 1] = (word[i] >> 4) & 0x0F0F0F0Fu;
           }
         }
-        if (!(ok = quick_wait<true>(aempty + 8 * ra.at, ra.phase ^ 1u, abortp))) break;
-        if (h == halves - 1 && lane == 0) mbar_arrive(wempty + 8 * rw.at);  // the packed weights are in registers
-        tc_fence_after_sync();
-        tmem_st_32x32(tmem_base + lane_addr + C::C_COLS + ra.at * 64 + tsel * 32, r);
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(afull + 8 * ra.at);
-        ra.next(NA);
+        if (h == 0) {
+          ok = quick_wait(aempty + 8 * ra.at, ra.phase ^ 1u, abortp);
+          if (!ok) break;
+          tc_fence_after_sync();
+        } else {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(wempty + 8 * rw.at);  // the packed weights are in registers
+        }
+        tmem_st_32x32(dst0 + ra.at * 128 + h * 32, r);
       }
+      if (!ok) break;
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(afull + 8 * ra.at);
+      ra.next(NA);
       rw.next(NW);
-      step(w);
     }
     if (!ok && lane == 0) {
       abort_flag = 1;
@@ -608,99 +643,143 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant
     }
   } else {
     // ------------------------------------------- accumulate and finish --
-    constexpr int CH = COLS < 16 ? COLS : 16;  // token columns per tensor-memory load
+    if (MT == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    constexpr int COLS = C::COLS;
+    constexpr int CH = COLS < 16 ? COLS : 16;  // token columns per round of tensor-memory loads
+    constexpr int GROUPS = BUF_PAIRS / 2;      // groups in a buffer, both tiles' sums each
+    // sums in flight at a time: as many as 32 registers hold
+    constexpr int BATCH = BUF_PAIRS * CH <= 32 ? BUF_PAIRS : 32 / CH;
     const int quarter = warp & 3;
     const int col0 = ((warp - 12) >> 2) * COLS;
+    const bool idle = col0 >= args.M;  // no tokens in these columns
     const int row = quarter * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t acc0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
     const int ep_tid = threadIdx.x - 384;
-    const uint32_t c_cols = args.gpg * N;
+    const bool zeros = args.zero0 != nullptr;
+    const int s_row = args.wide ? 256 : W4_META_ROW, z_row = args.wide ? 128 : W4_META_ROW;
+    const int z_off = args.wide ? 2 * GPU * 256 : W4_META_ZERO;
     if (args.early) pdl_wait();  // slots, counters and outputs may still be in use
-    if (!DUAL && total == 0) {
+    if (!DUAL && cut.total == 0) {
       // no token chose any expert: the outputs are the residual, or zero
       const long long all = static_cast<long long>(args.M) * args.rows;
-      for (long long i = blockIdx.x * static_cast<long long>(ACC_THREADS) + ep_tid; i < all;
-           i += static_cast<long long>(gridDim.x) * ACC_THREADS)
+      for (long long i = blockIdx.x * 256LL + ep_tid; i < all; i += gridDim.x * 256LL)
         static_cast<T*>(args.out)[i] =
             args.residual ? static_cast<const T*>(args.residual)[i] : static_cast<T>(0.f);
     }
+    const MoeShared* const mp = is_moe ? &moe : nullptr;
+    const Split sp{cut, args.M, reinterpret_cast<float4*>(args.slots), args.counters, args.status, abortp};
+    auto emit_tile = [&](int tile, int begin, int first, int last) {
+      T* const out = static_cast<T*>(args.out);
+      const T* const b0 = static_cast<const T*>(args.bias0);
+      const long long ld = args.rows;
+      if (DUAL) {
+        const T* const b1 = static_cast<const T*>(args.bias1);
+        const int a = tile / row_tiles, row0 = (tile - a * row_tiles) * ROWS;
+        if (is_moe) {
+          moe_factors(args.moe, args.M, moe.list[a], ep_tid, moe);
+          named_bar_sync(1, 256);
+        }
+        T* const oa = out + static_cast<long long>(a) * args.M * ld;
+        finish_tile<2, true, MT, 256>(begin, first, last, sp, ep_tid,
+                                      [&](int, int r, int i, const float4& gate, const float4& up) {
+          const int wr = row0 + r;
+          if (wr < args.rows)
+            emit_hidden(oa + wr, ld, args.M, i, gate, up, b0 ? static_cast<float>(b0[wr]) : 0.f,
+                        b1 ? static_cast<float>(b1[wr]) : 0.f, args.act, mp);
+        });
+      } else {
+        const T* const res = static_cast<const T*>(args.residual);
+        finish_tile<2, false, MT, 256>(begin, first, last, sp, ep_tid,
+                                       [&](int t, int r, int i, const float4& v, const float4&) {
+          const int wr = tile * ROWS + t * 128 + r;
+          if (wr < args.rows)
+            emit_product(out + wr, res ? res + wr : nullptr, ld, args.M, i, v, b0 ? static_cast<float>(b0[wr]) : 0.f, mp);
+        });
+      }
+      named_bar_sync(1, 256);  // the slot, f and hit are free for the next tile
+    };
+    Pending pending;
+    bool alive = true;
     W4Walk w;
     start(w);
-    Ring rx, rm, rc;
-    long long u = u_begin;
+    Ring rx, rc;
+    int u = u_begin;
     while (u < u_end) {
       const Segment s = segment_at(u, u_end, per_tile);
-      const int a = DUAL ? w.a : 0;
-      const int r0 = w.row0 + row, r1 = DUAL ? r0 : r0 + 128;
       f32x2 v[2][COLS / 2];
 #pragma unroll
       for (int c = 0; c < COLS / 2; ++c) v[0][c] = v[1][c] = 0ull;
       bool ok = true;
-      for (; u < s.end && ok; ++u) {
-        for (int h = 0; h < 2 && ok; ++h) {
-          const int ng = groups_in(w.kb, h);
-          if (ng <= 0) break;
-          if (!(ok = quick_wait<true>(mfull + 8 * rm.at, rm.phase, abortp))) break;
-          if (!(ok = quick_wait<true>(xfull + 8 * rx.at, rx.phase, abortp))) break;
-          const uint32_t xm = x_base + rx.at * C::X_STAGE_AL + C::X_TILE + col0 * 4;
-          const uint32_t mm = m_base + rm.at * m_stage;
+      for (; u < s.end; ++u) {
+        const int ng = groups_in(w.kb);
+        // low bits of the first scale's index: where its row starts inside a copied word
+        const uint32_t low = args.wide ? 0u
+                                       : (static_cast<uint32_t>(moe.list[w.a]) * args.groups + w.kb * GPU) *
+                                                 static_cast<uint32_t>(args.rows) + w.row0;
+        const uint32_t low_step = args.wide ? 0u : static_cast<uint32_t>(args.rows);
+        ok = quick_wait(xfull + 8 * rx.at, rx.phase, abortp);
+        // read as ordinary memory, so that the loads between two waits go out together
+        const float* const xm =
+            reinterpret_cast<const float*>(smem + NW * 2 * W4_TILE_BYTES + rx.at * C::X_STAGE + 2 * C::X_HALF) + col0;
+        const uint8_t* const mm = smem + NW * 2 * W4_TILE_BYTES + NX * C::X_STAGE + rx.at * C::M_STAGE;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const bool zeros = ((DUAL && t == 1) ? args.zero1 : args.zero0) != nullptr;
-            for (int g0 = 0; g0 < ng && ok; g0 += args.gpg) {
-              if (!(ok = quick_wait<true>(cfull + 8 * rc.at, rc.phase, abortp))) break;
-              tc_fence_after_sync();
-              const int ge = g0 + args.gpg < ng ? g0 + args.gpg : ng;
-              uint32_t src = tmem_base + lane_addr + rc.at * c_cols + col0;
-              for (int g = g0; g < ge; ++g, src += N) {
-                const long long e0 = (static_cast<long long>(moe.list[w.a]) * args.groups + w.kb * gpu_ + h * gph + g) *
-                                         args.rows + (w.row0 + (DUAL ? 0 : t * 128));
-                const uint32_t mr = mm + (t * gph + g) * W4_META_ROW;
-                const uint32_t sbits = ld_shared_u16(mr + static_cast<uint32_t>(e0 & 1) * 2 + row * 2);
-                const float sc = 512.0f * Pack2<T>::unpack(sbits).x;
-                const float z = zeros ? static_cast<float>(ld_shared_u8(mr + 264 + static_cast<uint32_t>(e0 & 3) + row) & 15u)
-                                      : 8.0f;
-                const f32x2 s2 = f2_pack(sc, sc), z2 = f2_pack(-z, -z);
+        for (int g0 = 0; g0 < GPU; g0 += GROUPS) {
+          // scales and zeros of the buffer's sums are fetched before the sums are there
+          float sc[BUF_PAIRS], nz[BUF_PAIRS];
 #pragma unroll
-                for (int c = 0; c < COLS; c += CH) {
-                  uint32_t x[TERMS][CH];
+          for (int b = 0; b < BUF_PAIRS; ++b) {
+            const int t = b & 1, g = g0 + (b >> 1);
+            const uint32_t e = low + (DUAL ? 0 : t * 128) + g * low_step;
+            const uint8_t* const sp = mm + (t * GPU + g) * s_row + (e & 1u) * 2 + row * 2;
+            sc[b] = 512.0f * static_cast<float>(*reinterpret_cast<const T*>(sp));
+            nz[b] = -8.0f;
+            if (zeros)  // an integer below 2^23 in a float's fraction: 2^23 - (2^23 + z)
+              nz[b] = 8388608.0f -
+                      __uint_as_float(0x4B000000u | (mm[z_off + (t * GPU + g) * z_row + (e & 3u) + row] & 15u));
+            if (g >= ng) sc[b] = nz[b] = 0.f;  // a group behind the last column
+          }
+          ok = ok && quick_wait(cfull + 8 * rc.at, rc.phase, abortp);
+          tc_fence_after_sync();
+          if (!idle) {
+            const uint32_t src = acc0 + rc.at * (BUF_PAIRS * N);
 #pragma unroll
-                  for (int i = 0; i < TERMS; ++i)
+            for (int b0 = 0; b0 < BUF_PAIRS; b0 += BATCH) {
 #pragma unroll
-                    for (int k = 0; k < CH; k += 8) tmem_ld_32x8(src + i * MT + c + k, &x[i][k]);
-                  tmem_ld_wait();
+              for (int c = 0; c < COLS; c += CH) {
+                uint32_t x[BATCH][CH];
 #pragma unroll
-                  for (int k = 0; k < CH; k += 4) {
-                    const float4 p = ld_shared_f4(xm + g * 2 * MT * 4 + (c + k) * 4);
-                    const float4 q = ld_shared_f4(xm + g * 2 * MT * 4 + MT * 4 + (c + k) * 4);
+                for (int b = 0; b < BATCH; ++b) tmem_ld_cols<CH>(src + (b0 + b) * N + c, x[b]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int k = 0; k < CH; k += 4) {
+#pragma unroll
+                  for (int b = 0; b < BATCH; ++b) {
+                    const int t = (b0 + b) & 1, g = g0 + ((b0 + b) >> 1);
+                    const float* const xg = xm + g * 2 * MT + c + k;
+                    const float4 q0 = *reinterpret_cast<const float4*>(xg);
+                    const float4 q1 = *reinterpret_cast<const float4*>(xg + MT);
+                    const f32x2 s2 = f2_pack(sc[b0 + b], sc[b0 + b]), z2 = f2_pack(nz[b0 + b], nz[b0 + b]);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                       const int o = k + 2 * j;
-                      f32x2 y = f2_add(f2_pack(__uint_as_float(x[0][o]), __uint_as_float(x[0][o + 1])),
-                                       f2_pack(__uint_as_float(x[1][o]), __uint_as_float(x[1][o + 1])));
-                      if (TERMS == 3)
-                        y = f2_add(y, f2_pack(__uint_as_float(x[TERMS - 1][o]), __uint_as_float(x[TERMS - 1][o + 1])));
-                      y = f2_mul(y, j == 0 ? f2_pack(p.x, p.y) : f2_pack(p.z, p.w));
-                      y = f2_fma(z2, j == 0 ? f2_pack(q.x, q.y) : f2_pack(q.z, q.w), y);
+                      f32x2 y = f2_mul(f2_pack(__uint_as_float(x[b][o]), __uint_as_float(x[b][o + 1])),
+                                       j == 0 ? f2_pack(q0.x, q0.y) : f2_pack(q0.z, q0.w));
+                      y = f2_fma(z2, j == 0 ? f2_pack(q1.x, q1.y) : f2_pack(q1.z, q1.w), y);
                       v[t][(c + o) / 2] = f2_fma(s2, y, v[t][(c + o) / 2]);
                     }
                   }
                 }
               }
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(cempty + 8 * rc.at);
-              rc.next(args.acc_bufs);
             }
           }
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_arrive(mempty + 8 * rm.at);
-            mbar_arrive(xempty + 8 * rx.at);
-          }
-          rm.next(nm);
-          rx.next(NX);
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(cempty + 8 * rc.at);
+          rc.next(NC);
         }
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(xempty + 8 * rx.at);
+        rx.next(NX);
         step(w);
       }
       if (!ok && lane == 0) {
@@ -712,33 +791,9 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int c = 0; c < COLS / 2; ++c) f2_unpack(v[t][c], f[t][2 * c], f[t][2 * c + 1]);
-      if (DUAL && is_moe) moe_factors(args.moe, args.M, moe.list[a], ep_tid, moe);  // seen behind the next barrier
-      const Split sp{total,       ctas,   args.slots, args.counters,
-                     args.status, abortp, w_base,     NW * 2 * W4_TILE_BYTES / (ACC_THREADS * 16)};
-      const int what = settle_segment<2, COLS, MT, ACC_THREADS>(f, s, sp, args.M, col0, row, ep_tid);
-      if (what == SETTLE_ABORT) break;
-      if (what == SETTLE_EMIT) {
-        const MoeShared* const mp = is_moe ? &moe : nullptr;
-        T* const out = static_cast<T*>(args.out);
-        const T* const b0 = static_cast<const T*>(args.bias0);
-        const T* const b1 = static_cast<const T*>(args.bias1);
-        const T* const res = static_cast<const T*>(args.residual);
-        const long long ld = args.rows;
-        if (DUAL) {
-          if (r0 < args.rows)
-            store_hidden<COLS>(args.act, out + static_cast<long long>(a) * args.M * ld + r0, ld, args.M, col0, f[0],
-                               f[1], b0 ? static_cast<float>(b0[r0]) : 0.f, b1 ? static_cast<float>(b1[r0]) : 0.f, mp);
-        } else {
-          if (r0 < args.rows)
-            store_product<COLS>(out + r0, res ? res + r0 : nullptr, ld, args.M, col0, f[0],
-                                b0 ? static_cast<float>(b0[r0]) : 0.f, mp);
-          if (r1 < args.rows)
-            store_product<COLS>(out + r1, res ? res + r1 : nullptr, ld, args.M, col0, f[1],
-                                b0 ? static_cast<float>(b0[r1]) : 0.f, mp);
-        }
-      }
-      if (DUAL && is_moe) named_bar_sync(1, ACC_THREADS);  // f and hit are overwritten for the next tile
+      if (!(alive = end_segment<2, COLS, MT, 256>(f, s, sp, col0, row, ep_tid, pending, emit_tile))) break;
     }
+    if (alive) end_units<256>(pending, per_tile, sp, ep_tid, emit_tile);
   }
 
   tc_fence_before_sync();

@@ -727,6 +727,8 @@ def decode_fwd_w4(x: Tensor, w_gate: Int4Weight, b_gate: Tensor | None, w_up: In
     group = _int4_group(w_gate, (), N, K, dt, dev)
     if _int4_group(w_up, (), N, K, dt, dev) != group or _int4_group(w_down, (), K, N, dt, dev) != group:
         raise ValueError("gate, up and down weights must have one group size")
+    if (w_gate[2] is None) != (w_up[2] is None):
+        raise ValueError("gate and up weights must both have zeros or both have none")
     b_gate, b_up, b_down = _vector(b_gate, N, "b_gate"), _vector(b_up, N, "b_up"), _vector(b_down, K, "b_down")
     residual = _like(residual, (M, K), "residual")
     y = torch.empty((M, K), dtype=dt, device=dev)
@@ -851,6 +853,8 @@ def moe_decode_fwd_w4(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Int4Weigh
     group = _int4_group(w_gate, (E,), N, K, dt, dev)
     if _int4_group(w_up, (E,), N, K, dt, dev) != group or _int4_group(w_down, (E,), K, N, dt, dev) != group:
         raise ValueError("gate, up and down weights must have one group size")
+    if (w_gate[2] is None) != (w_up[2] is None):
+        raise ValueError("gate and up weights must both have zeros or both have none")
     ids, weights, k = _moe_table(x, ids, weights, E)
     residual = _like(residual, (M, K), "residual")
     y = torch.empty((M, K), dtype=dt, device=dev)
