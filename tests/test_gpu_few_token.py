@@ -40,6 +40,17 @@ def test_linear_w4(pkg, cuda_dev, M, rows, cols, group):
     ft.check(y, *ft.linear(x, _unpack(w), bias, res, dt, group), f"linear_w4 M={M} {rows}x{cols} g{group}")
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 16, 17, 64])
+@pytest.mark.parametrize("dt,group", [(BF, 128), (FP, 32)])
+def test_linear_w4_many_units_per_block(pkg, cuda_dev, M, dt, group):
+    """Every ring of the stream kernel turns several times (about 14 units of 65,536 weights per block)."""
+    g = _gen(cuda_dev, M)
+    w = _w4(pkg, g, 16384, 8192, group=group, symmetric=False, dt=dt)
+    x = _rnd(g, M, 8192, dt=dt)
+    y = pkg.ops.kernels.linear_w4(x, w)
+    ft.check(y, *ft.linear(x, _unpack(w), None, None, dt, group), f"linear_w4 M={M} g{group}")
+
+
 def test_linear_w4_every_nibble_and_zero(pkg, cuda_dev):
     """All 16 values against all 16 zeros, one column at a time: exact."""
     K_ = pkg.ops.kernels

@@ -226,7 +226,8 @@ int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t
   char* const sc = static_cast<char*>(scratch);
   const bool dep = (tuning & (1u << 26)) == 0;  // GMLP_TUNE_ORDINARY_LAUNCH
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if ((rc = launch_split(M, M, cols, ldx, group, dtype, x, wk + ww.t8_off, wk + ww.meta_off, dep, st))) return rc;
+  const bool split = M > W4_FUSED_TOKENS;
+  if (split && (rc = launch_split(M, M, cols, ldx, group, dtype, x, wk + ww.t8_off, wk + ww.meta_off, dep, st))) return rc;
   W4Call c;
   memset(&c, 0, sizeof(c));
   c.dtype = dtype;
@@ -237,6 +238,8 @@ int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t
   c.R = M;
   c.group = group;
   c.w0 = c.w1 = w;
+  c.x = x;
+  c.ldx = ldx;
   c.t8 = wk + ww.t8_off;
   c.meta = wk + ww.meta_off;
   c.bias0 = bias;
@@ -244,6 +247,7 @@ int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t
   c.out = y;
   c.slots = reinterpret_cast<float*>(sc);
   c.counters = reinterpret_cast<int*>(sc + l.counters1_off);
+  c.dependent = split || dep;
   c.early = true;
   c.max_units = ((rows + 255) / 256) * ((cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
   c.stream = st;
@@ -275,7 +279,8 @@ static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const
   const bool sparse = moe.ids != nullptr;
   const bool dep = sparse || (p->tuning & (1u << 26)) == 0;  // GMLP_TUNE_ORDINARY_LAUNCH
   const int64_t k_units = (p->K + W4_UNIT_COLS - 1) / W4_UNIT_COLS, n_units = (p->N + W4_UNIT_COLS - 1) / W4_UNIT_COLS;
-  if ((rc = launch_split(p->M, p->M, p->K, p->K, group, p->dtype, x, wk + ww.t8_off, wk + ww.meta_off, dep, st)))
+  const bool split = p->M > W4_FUSED_TOKENS;
+  if (split && (rc = launch_split(p->M, p->M, p->K, p->K, group, p->dtype, x, wk + ww.t8_off, wk + ww.meta_off, dep, st)))
     return rc;
   W4Call c;
   memset(&c, 0, sizeof(c));
@@ -292,27 +297,33 @@ static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const
   c.rows = p->N;
   c.cols = p->K;
   c.R = p->M;
+  c.x = x;
+  c.ldx = p->K;
   c.w0 = g;
   c.w1 = u;
   c.bias0 = b_gate;
   c.bias1 = b_up;
   c.out = wk;
   c.counters = reinterpret_cast<int*>(sc + l.counters1_off);
+  c.dependent = split || dep;
   c.early = !sparse;
   c.max_units = active * ((p->N + 127) / 128) * k_units;
   if ((rc = launch_w4(dev, c, true))) return rc;
-  if ((rc = launch_split(p->M, active * p->M, p->N, p->N, group, p->dtype, wk, wk + ww.t8_off, wk + ww.meta_off, true,
-                         st)))
+  if (split && (rc = launch_split(p->M, active * p->M, p->N, p->N, group, p->dtype, wk, wk + ww.t8_off, wk + ww.meta_off,
+                                  true, st)))
     return rc;
   c.rows = p->K;
   c.cols = p->N;
   c.R = active * p->M;
+  c.x = wk;
+  c.ldx = p->N;
   c.w0 = c.w1 = d;
   c.bias0 = b_down;
   c.bias1 = nullptr;
   c.residual = residual;
   c.out = y;
   c.counters = reinterpret_cast<int*>(sc + l.counters2_off);
+  c.dependent = true;
   c.early = true;
   c.max_units = active * ((p->K + 255) / 256) * n_units;
   return launch_w4(dev, c, false);

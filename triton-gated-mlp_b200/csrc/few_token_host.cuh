@@ -48,28 +48,31 @@ struct W4Call {
   int64_t M, rows, cols, experts, R;
   int group;
   W4Matrix w0, w1;
+  const void* x;  // the activations, of pitch ldx (at most W4_FUSED_TOKENS tokens), or their terms
+  int64_t ldx;
   const void *t8, *meta;
   const void *bias0, *bias1, *residual;
   void* out;
   float* slots;
   int* counters;
   int act;
-  bool early;
+  bool dependent, early;
   MoeTable moe;
   int64_t max_units;
   cudaStream_t stream;
 };
 
-template <int MT, bool DUAL, typename T, int GSHIFT>
+template <int MT, bool DUAL, typename T, int GSHIFT, bool FUSED>
 int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
-  using Conf = W4Conf<MT, w4_terms<T>(), GSHIFT>;
+  using Conf = W4Conf<MT, w4_terms<T>(), GSHIFT, FUSED>;
   if (c.max_units > 0x7fffffffLL) return fail(GMLP_ERR_SHAPE, "the call has more than 2^31 units of work");
   W4Maps m;
   int rc;
   if ((rc = encode_map(&m.w0, c.w0.q, c.cols / 2, c.experts * c.rows, c.cols / 2, 128, 128, DTYPE_U8))) return rc;
   m.w1 = m.w0;
   if (DUAL && (rc = encode_map(&m.w1, c.w1.q, c.cols / 2, c.experts * c.rows, c.cols / 2, 128, 128, DTYPE_U8))) return rc;
-  if ((rc = encode_map(&m.x, c.t8, c.cols, w4_terms<T>() * c.R, c.cols, 128, MT, DTYPE_U8))) return rc;
+  m.x = m.w0;
+  if (!FUSED && (rc = encode_map(&m.x, c.t8, c.cols, w4_terms<T>() * c.R, c.cols, 128, MT, DTYPE_U8))) return rc;
   // Scales and zeros by TMA where their rows are aligned, else word by word (a warp's copies, about as many clocks a unit
   // as the weights of the unit take to arrive; 8-token gate/up kernel, 28672 x 8192: 54 against 46 us).
   const bool wide = c.rows % 16 == 0 && aligned16(c.w0.scale) && aligned16(c.w1.scale) && aligned16(c.w0.zero) &&
@@ -90,6 +93,9 @@ int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
   a.kbt = static_cast<int>((c.cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS);
   a.groups = static_cast<int>(c.cols / c.group);
   a.R = c.R;
+  a.x = c.x;
+  a.ldx = c.ldx;
+  a.cols = static_cast<int>(c.cols);
   a.status = dev->status_ptr;
   a.meta = static_cast<const float*>(c.meta);
   a.scale0 = static_cast<const uint16_t*>(c.w0.scale);
@@ -107,20 +113,30 @@ int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
   a.early = c.early ? 1 : 0;
   a.moe = c.moe;
   const int grid = static_cast<int>(c.max_units < dev->sm_count ? c.max_units : dev->sm_count);
-  auto kfn = w4_stream_kernel<MT, DUAL, T, GSHIFT>;
+  auto kfn = w4_stream_kernel<MT, DUAL, T, GSHIFT, FUSED>;
   static std::atomic<uint64_t> attr_done{0};
   if ((rc = ensure_smem_attr(kfn, Conf::SMEM, attr_done))) return rc;
-  return launch_few(kfn, grid, Conf::THREADS, Conf::SMEM, true, c.stream, m, a);
+  return launch_few(kfn, grid, Conf::THREADS, Conf::SMEM, c.dependent, c.stream, m, a);
 }
-template <int GSHIFT, bool DUAL>
-int launch_w4_group(const DeviceInfo* dev, const W4Call& c) {
-  const bool bf = c.dtype == GMLP_BF16;
+// Up to this many tokens the stream kernel makes the terms itself, in four warps that have nothing else to do then (a launch
+// less per product); more tokens a unit take those warps longer than the unit's weights take to arrive.
+constexpr int W4_FUSED_TOKENS = 4;
+
+template <int GSHIFT, bool DUAL, typename T>
+int launch_w4_type(const DeviceInfo* dev, const W4Call& c) {
+  if (c.M <= W4_FUSED_TOKENS) return launch_w4_t<8, DUAL, T, GSHIFT, true>(dev, c);
   switch (w4_mt(c.M)) {
-    case 8: return bf ? launch_w4_t<8, DUAL, __nv_bfloat16, GSHIFT>(dev, c) : launch_w4_t<8, DUAL, __half, GSHIFT>(dev, c);
-    case 16: return bf ? launch_w4_t<16, DUAL, __nv_bfloat16, GSHIFT>(dev, c) : launch_w4_t<16, DUAL, __half, GSHIFT>(dev, c);
-    case 32: return bf ? launch_w4_t<32, DUAL, __nv_bfloat16, GSHIFT>(dev, c) : launch_w4_t<32, DUAL, __half, GSHIFT>(dev, c);
-    default: return bf ? launch_w4_t<64, DUAL, __nv_bfloat16, GSHIFT>(dev, c) : launch_w4_t<64, DUAL, __half, GSHIFT>(dev, c);
+    case 8: return launch_w4_t<8, DUAL, T, GSHIFT, false>(dev, c);
+    case 16: return launch_w4_t<16, DUAL, T, GSHIFT, false>(dev, c);
+    case 32: return launch_w4_t<32, DUAL, T, GSHIFT, false>(dev, c);
+    default: return launch_w4_t<64, DUAL, T, GSHIFT, false>(dev, c);
   }
+}
+template <int GSHIFT>
+int launch_w4_group(const DeviceInfo* dev, const W4Call& c, bool dual) {
+  if (c.dtype == GMLP_BF16)
+    return dual ? launch_w4_type<GSHIFT, true, __nv_bfloat16>(dev, c) : launch_w4_type<GSHIFT, false, __nv_bfloat16>(dev, c);
+  return dual ? launch_w4_type<GSHIFT, true, __half>(dev, c) : launch_w4_type<GSHIFT, false, __half>(dev, c);
 }
 // One translation unit each (w4_g32.cu, w4_g64.cu, w4_g128.cu): they compile side by side.
 int launch_w4_g32(const DeviceInfo* dev, const W4Call& c, bool dual);

@@ -2,7 +2,5 @@
 #include "few_token_host.cuh"
 
 namespace gmlp {
-int launch_w4_g32(const DeviceInfo* dev, const W4Call& c, bool dual) {
-  return dual ? launch_w4_group<0, true>(dev, c) : launch_w4_group<0, false>(dev, c);
-}
+int launch_w4_g32(const DeviceInfo* dev, const W4Call& c, bool dual) { return launch_w4_group<0>(dev, c, dual); }
 }  // namespace gmlp

@@ -60,6 +60,49 @@ __host__ __device__ constexpr int w4_terms<__half>() {
 }
 
 // ---- activations -> terms ----
+// Eight columns of a lane, groups of `width` neighbouring lanes: the terms' codes (bytes in the order in which the
+// expanders' masks deliver a word's nibbles: columns 0 4 1 5 | 2 6 3 7), 2^-e and 2^-9 times the group's sum.
+template <int TERMS>
+__device__ __forceinline__ void split_terms(const float (&v)[8], int width, uint2 (&codes)[TERMS], float& down, float& sum) {
+  float amax = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    amax = fmaxf(amax, fabsf(v[i]));
+    bad |= !(fabsf(v[i]) < INFINITY);
+  }
+  for (int o = 1; o < width; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  // 2^e: the largest value goes to [128, 256). e is limited so that 2^e and 2^-e are normal numbers.
+  int ex = 7 - (static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127);
+  ex = ex > 120 ? 120 : ex;
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+  down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+  float rest[8];
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rest[i] = v[i] * up;
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    constexpr int PERM[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+    uint32_t pair[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int a = PERM[2 * i], b = PERM[2 * i + 1];
+      const __nv_fp8x2_storage_t c = __nv_cvt_float2_to_fp8x2(make_float2(rest[a], rest[b]), __NV_SATFINITE, __NV_E4M3);
+      const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(c, __NV_E4M3)));
+      rest[a] -= back.x;
+      rest[b] -= back.y;
+      sum += back.x + back.y;
+      pair[i] = c;
+    }
+    codes[t] = make_uint2(pair[0] | (pair[1] << 16), pair[2] | (pair[3] << 16));
+  }
+  if (bad) sum = __uint_as_float(0x7fc00000u);
+  for (int o = 1; o < width; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (sum != sum) down = sum;  // a non-finite activation: the token's outputs become NaN
+  sum *= down * 0.001953125f;
+}
+
 // x [R][cols] (row pitch ldx) -> t8 [TERMS][R][cols] e4m3 bytes, inside every 8 columns in the order in which
 // the expanders' masks deliver a word's nibbles, and meta [R / M][groups][2][MT] floats: 2^-e, 2^-9 * sum, with the groups
 // of a row padded to whole units of 256 columns (zeros there). 16 lanes take the 128 columns of a half unit (8 each);
@@ -90,49 +133,22 @@ w4_split_kernel(const W4SplitArgs args) {
   const bool live = item < items && col < args.cols;
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (live) load8(static_cast<const T*>(args.x) + row * args.ldx + col, v);
-  float amax = 0.f;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    amax = fmaxf(amax, fabsf(v[i]));
-    bad |= !(fabsf(v[i]) < INFINITY);
-  }
   const int width = 4 << args.gshift;  // lanes per group
-  for (int o = 1; o < width; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  // 2^e: the largest value goes to [128, 256). e is limited so that 2^e and 2^-e are normal numbers.
-  int ex = 7 - (static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127);
-  ex = ex > 120 ? 120 : ex;
-  const float up = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
-  const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-  float rest[8];
-  float sum = 0.f;
+  uint2 code[TERMS];
+  float down, sum;
+  split_terms<TERMS>(v, width, code, down, sum);
+  if (live) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) rest[i] = v[i] * up;
-#pragma unroll
-  for (int t = 0; t < TERMS; ++t) {
-    uint32_t code[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __nv_fp8_storage_t c = __nv_cvt_float_to_fp8(rest[i], __NV_SATFINITE, __NV_E4M3);
-      const float back = __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
-      rest[i] -= back;
-      sum += back;
-      code[i] = c;
-    }
-    // bytes in the order of the nibbles: columns 0 4 1 5 | 2 6 3 7
-    const uint32_t lo = code[0] | (code[4] << 8) | (code[1] << 16) | (code[5] << 24);
-    const uint32_t hi = code[2] | (code[6] << 8) | (code[3] << 16) | (code[7] << 24);
-    if (live) *reinterpret_cast<uint2*>(args.t8 + (t * args.R + row) * args.cols + col) = make_uint2(lo, hi);
+    for (int t = 0; t < TERMS; ++t)
+      *reinterpret_cast<uint2*>(args.t8 + (t * args.R + row) * args.cols + col) = code[t];
   }
-  if (bad) sum = __uint_as_float(0x7fc00000u);  // a non-finite activation: the token's outputs become NaN
-  for (int o = 1; o < width; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (item < items && (sub & (width - 1)) == 0) {
     const long long a = row / args.M, m = row - a * args.M;
     const int groups = blocks * (4 >> args.gshift);
     const long long g = col >> (5 + args.gshift);
     float* const p = args.meta + ((a * groups + g) * 2) * args.MT + m;
-    p[0] = sum != sum ? sum : down;
-    p[args.MT] = sum * down * 0.001953125f;
+    p[0] = down;
+    p[args.MT] = sum;
   }
 }
 
@@ -147,6 +163,9 @@ struct W4Args {
   int kbt;         // units along an expert's columns: ceil(cols / 256)
   int groups;      // cols / G
   long long R;     // rows of a plane of activation terms
+  const void* x;   // FUSED: the activations themselves, [M] or [active * M] rows of pitch ldx
+  long long ldx;
+  int cols;
   int* status;
   const float* meta;       // [experts in h or 1][kbt * groups per unit][2][MT]
   const uint16_t* scale0;  // [experts][groups][rows], T
@@ -170,10 +189,15 @@ struct W4Args {
 constexpr int W4_META_ROW = 416;
 constexpr int W4_META_ZERO = 272;
 
-template <int MT, int TERMS, int GSHIFT>
+template <int MT, int TERMS, int GSHIFT, bool FUSED>
 struct W4Conf {
+  static_assert(!FUSED || MT == 8, "the fused form takes up to four tokens");
   static constexpr int N = MT < 16 ? 16 : MT;      // columns of the MMA; those behind MT hold nothing of use
-  static constexpr int THREADS = 32 * 20;
+  // accumulating threads: four warps per share of the tokens; 64 tokens take sixteen warps, since with eight each thread's
+  // 64 sums left two warps a scheduler, whose loads and products wait for each other (103 against 8x us)
+  static constexpr int SHARES = FUSED ? 1 : (MT == 64 ? 4 : 2);
+  static constexpr int EPI = 128 * SHARES;
+  static constexpr int THREADS = 32 * (12 + 4 * SHARES + (FUSED ? 4 : 0));
   static constexpr int GPH = 4 >> GSHIFT;          // groups per half unit (128 columns)
   static constexpr int GPU = 2 * GPH;              // groups per unit
   // activation terms of a unit: [two halves][TERMS] of N rows x 128 columns, then meta [GPU][2][MT]
@@ -181,9 +205,9 @@ struct W4Conf {
   static constexpr int X_HALF = TERMS * X_TERM;
   static constexpr int X_STAGE = (2 * X_HALF + GPU * 2 * MT * 4 + 1023) / 1024 * 1024;
   static constexpr int M_STAGE = 2 * GPU * W4_META_ROW;  // scales and zeros of a unit
-  static constexpr int COLS = MT / 2;  // tokens per accumulator thread
+  static constexpr int COLS = FUSED ? 4 : MT / SHARES;  // tokens per accumulator thread
   static constexpr int SMEM_MAX = 232448 - 1024 - 4096;
-  static constexpr int X_STAGES = 3 * (X_STAGE + M_STAGE) + 3 * 2 * W4_TILE_BYTES <= SMEM_MAX ? 3 : 2;
+  static constexpr int X_STAGES = FUSED ? 4 : 3 * (X_STAGE + M_STAGE) + 3 * 2 * W4_TILE_BYTES <= SMEM_MAX ? 3 : 2;
   static constexpr int FIT = (SMEM_MAX - X_STAGES * (X_STAGE + M_STAGE)) / (2 * W4_TILE_BYTES);
   static constexpr int W_STAGES = FIT > 5 ? 5 : FIT;
   static constexpr size_t SMEM = 1024 + static_cast<size_t>(W_STAGES) * 2 * W4_TILE_BYTES + X_STAGES * (X_STAGE + M_STAGE);
@@ -310,11 +334,11 @@ struct W4Walk {
   int a, kb, row0;
 };
 
-template <int MT, bool DUAL, typename T, int GSHIFT>
-__global__ void __launch_bounds__(W4Conf<MT, w4_terms<T>(), GSHIFT>::THREADS, 1)
+template <int MT, bool DUAL, typename T, int GSHIFT, bool FUSED>
+__global__ void __launch_bounds__(W4Conf<MT, w4_terms<T>(), GSHIFT, FUSED>::THREADS, 1)
 w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   constexpr int TERMS = w4_terms<T>();
-  using C = W4Conf<MT, TERMS, GSHIFT>;
+  using C = W4Conf<MT, TERMS, GSHIFT, FUSED>;
   constexpr int N = C::N;
   constexpr int NW = C::W_STAGES, NX = C::X_STAGES, NA = C::A_BUFS, NC = C::C_BUFS;
   constexpr int GPH = C::GPH, GPU = C::GPU, PAIRS = C::PAIRS, BUF_PAIRS = C::BUF_PAIRS;
@@ -328,7 +352,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   __shared__ MoeShared moe;
 
   const uint32_t w_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint8_t* const smem = smem_raw + (w_base - smem_u32(smem_raw));
+  uint8_t* const smem = smem_raw + (w_base - smem_u32(smem_raw));
   const uint32_t x_base = w_base + NW * 2 * W4_TILE_BYTES;
   const uint32_t m_base = x_base + NX * C::X_STAGE;
   const uint32_t wfull = smem_u32(bars), wempty = wfull + 8 * NW, xfull = wempty + 8 * NW, xempty = xfull + 8 * NX,
@@ -343,8 +367,9 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       mbar_init(wempty + 8 * s, 8);
     }
     for (int s = 0; s < NX; ++s) {
-      mbar_init(xfull + 8 * s, args.wide ? 1 : 1 + 32);  // the TMA bytes, and the copying lanes of warp 3
-      mbar_init(xempty + 8 * s, 1 + 8);
+      // the TMA bytes, the copying lanes of warp 3, a converting warp per token
+      mbar_init(xfull + 8 * s, 1 + (args.wide ? 0 : 32) + (FUSED ? args.M : 0));
+      mbar_init(xempty + 8 * s, 1 + C::EPI / 32);
     }
     for (int b = 0; b < NA; ++b) {
       mbar_init(afull + 8 * b, 8);
@@ -352,7 +377,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     }
     for (int b = 0; b < NC; ++b) {
       mbar_init(cfull + 8 * b, 1);
-      mbar_init(cempty + 8 * b, 8);
+      mbar_init(cempty + 8 * b, C::EPI / 32);
     }
     mbar_init(drain_bar, 1);
     mbar_fence_init();
@@ -415,11 +440,11 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     return left < GPU ? left : GPU;
   };
 
-  // 64 tokens: 640 threads leave 96 registers each, 64 sums a thread want more. Of the block's 640 x 96 = 61,440 the helpers
-  // keep 56 and the expanders 64 a thread, the accumulators get 144: 128 x (56 + 2 x 64 + 2 x 144) = 60,416.
+  // 64 tokens: 896 threads leave 72 registers each. Of the block's 896 x 72 = 64,512 the helpers keep 40 and the expanders
+  // 56 a thread, the accumulators get 88: 128 x (40 + 2 x 56 + 4 x 88) = 64,512.
   if (warp == 0) {
     // ------------------------------------------------------------ weights --
-    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     const uint64_t pol = l2_policy_evict_first();
     W4Walk w;
     start(w);
@@ -450,8 +475,8 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     }
   } else if (warp == 2) {
     // -------------------------------------------------------- activations --
-    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (args.early) pdl_wait();
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (args.early && !FUSED) pdl_wait();
     const uint64_t pol = l2_policy_evict_last(), pol_w = l2_policy_evict_first();
     W4Walk w;
     start(w);
@@ -465,7 +490,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       constexpr uint32_t META_BYTES = GPU * 2 * MT * 4;
       if (elect_one()) {
         const uint32_t sz_bytes = args.wide ? 2 * GPU * 128 * (2 + (args.zero0 != nullptr ? 1 : 0)) : 0;
-        mbar_expect_tx(fb, 2 * TERMS * MT * 128 + META_BYTES + sz_bytes);
+        mbar_expect_tx(fb, (FUSED ? 0 : 2 * TERMS * MT * 128 + META_BYTES) + sz_bytes);
         if (args.wide) {
           const uint32_t md = m_base + r.at * C::M_STAGE;
           const int gy = moe.list[w.a] * args.groups + w.kb * GPU;
@@ -477,12 +502,14 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
                              pol_w);
           }
         }
+        if (!FUSED) {
 #pragma unroll
-        for (int i = 0; i < 2 * TERMS; ++i)  // a half behind the last column arrives as zeros
-          tma_load_2d_hint(dst + i * C::X_TERM, &maps.x, fb, w.kb * W4_UNIT_COLS + (i / TERMS) * W4_HALF_COLS,
-                           static_cast<int>((i % TERMS) * args.R) + a * args.M, pol);
-        bulk_load(dst + 2 * C::X_HALF, args.meta + (static_cast<long long>(a) * args.kbt + w.kb) * (GPU * 2 * MT),
-                  META_BYTES, fb);
+          for (int i = 0; i < 2 * TERMS; ++i)  // a half behind the last column arrives as zeros
+            tma_load_2d_hint(dst + i * C::X_TERM, &maps.x, fb, w.kb * W4_UNIT_COLS + (i / TERMS) * W4_HALF_COLS,
+                             static_cast<int>((i % TERMS) * args.R) + a * args.M, pol);
+          bulk_load(dst + 2 * C::X_HALF, args.meta + (static_cast<long long>(a) * args.kbt + w.kb) * (GPU * 2 * MT),
+                    META_BYTES, fb);
+        }
       }
       __syncwarp();
       step(w);
@@ -496,7 +523,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     }
   } else if (warp == 3) {
     // --------------------------------------------------- scales and zeros --
-    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     // Rows of scales and zeros start anywhere (any number of weight rows is allowed): copied by 4-byte words, up to 65 + 33
     // per (tile, group), of which the last one only as far as the rows go.
     W4Walk w;
@@ -545,7 +572,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     cp_async_wait_all();
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA --
-    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     constexpr uint32_t IDESC = make_idesc_f8(128, N);
     const uint64_t x0 = make_smem_desc(x_base, 16, 1024);
     Ring rx, ra, rc;
@@ -595,7 +622,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------- expand --
-    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     const int quarter = warp & 3;
     const int tsel = (warp - 4) >> 2;  // which of the unit's two tiles
     const int row = quarter * 32 + lane;
@@ -641,10 +668,77 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       abort_flag = 1;
       atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_MMA);
     }
+  } else if (FUSED && warp >= 16) {
+    // ------------------------------------------- activations -> terms --
+    // (unit, token) pairs in turn, one a warp: the row's 256 columns, eight a lane, the two halves of the warp the two halves
+    // of the unit. Written where TMA would have put them (128-byte rows, 16-byte chunks swizzled by the row).
+    if (args.early) pdl_wait();
+    const int sub = lane & 15, half = lane >> 4;
+    W4Walk wn;  // position of the pair being fetched
+    start(wn);
+    // A warp takes every fourth unit at most, and a parity tells a stage's phase only to a waiter that is not a whole turn
+    // of the ring away from it: when a warp has seen unit u - NX released, unit u + 4 - 2 NX has been.
+    static_assert(!FUSED || NX >= 4, "a converting warp would take one phase of a stage for another");
+    Ring r;  // stage of unit `at_unit`
+    int at_unit = 0;
+    bool ok = true;
+    auto fetch = [&](int p, const W4Walk& q) {
+      const int m = p % args.M, col = q.kb * W4_UNIT_COLS + lane * 8;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (col < args.cols)
+        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(args.x) +
+                                            ((DUAL ? 0 : static_cast<long long>(q.a) * args.M) + m) * args.ldx + col);
+      return v;
+    };
+    const int pairs = units * args.M;
+    int p = warp - 16;
+    int next_unit = 0;
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (p < pairs) {
+      for (; next_unit < p / args.M; ++next_unit) step(wn);
+      raw = fetch(p, wn);
+    }
+    for (; p < pairs; p += 4) {
+      const uint4 cur = raw;
+      if (p + 4 < pairs) {
+        for (; next_unit < (p + 4) / args.M; ++next_unit) step(wn);
+        raw = fetch(p + 4, wn);
+      }
+      float v[8];
+      const float2 v0 = Pack2<T>::unpack(cur.x), v1 = Pack2<T>::unpack(cur.y), v2 = Pack2<T>::unpack(cur.z),
+                   v3 = Pack2<T>::unpack(cur.w);
+      v[0] = v0.x; v[1] = v0.y; v[2] = v1.x; v[3] = v1.y;
+      v[4] = v2.x; v[5] = v2.y; v[6] = v3.x; v[7] = v3.y;
+      uint2 code[TERMS];
+      float down, sum;
+      constexpr int WIDTH = 4 << GSHIFT;
+      split_terms<TERMS>(v, WIDTH, code, down, sum);
+      const int m = p % args.M;
+      for (; at_unit < p / args.M; ++at_unit) r.next(NX);
+      ok = quick_wait(xempty + 8 * r.at, r.phase ^ 1u, abortp);
+      if (!ok) break;
+      uint8_t* const xs = smem + NW * 2 * W4_TILE_BYTES + r.at * C::X_STAGE;
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+        *reinterpret_cast<uint2*>(xs + (half * TERMS + t) * C::X_TERM + m * 128 + (((sub >> 1) ^ (m & 7)) << 4) +
+                                  (sub & 1) * 8) = code[t];
+      if ((sub & (WIDTH - 1)) == 0) {
+        float* const mt = reinterpret_cast<float*>(xs + 2 * C::X_HALF) + (half * GPH + sub / WIDTH) * 2 * MT + m;
+        mt[0] = down;
+        mt[MT] = sum;
+      }
+      fence_proxy_async_smem();  // the MMA reads the terms
+      __syncwarp();
+      if (lane == 0) mbar_arrive(xfull + 8 * r.at);
+    }
+    if (!ok && lane == 0) {
+      abort_flag = 1;
+      atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_PRODUCER);
+    }
   } else {
     // ------------------------------------------- accumulate and finish --
-    if (MT == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
-    constexpr int COLS = C::COLS;
+    if (MT == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    constexpr int COLS = C::COLS, EPI = C::EPI;
     constexpr int CH = COLS < 16 ? COLS : 16;  // token columns per round of tensor-memory loads
     constexpr int GROUPS = BUF_PAIRS / 2;      // groups in a buffer, both tiles' sums each
     // sums in flight at a time: as many as 32 registers hold
@@ -662,7 +756,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     if (!DUAL && cut.total == 0) {
       // no token chose any expert: the outputs are the residual, or zero
       const long long all = static_cast<long long>(args.M) * args.rows;
-      for (long long i = blockIdx.x * 256LL + ep_tid; i < all; i += gridDim.x * 256LL)
+      for (long long i = blockIdx.x * static_cast<long long>(EPI) + ep_tid; i < all; i += gridDim.x * static_cast<long long>(EPI))
         static_cast<T*>(args.out)[i] =
             args.residual ? static_cast<const T*>(args.residual)[i] : static_cast<T>(0.f);
     }
@@ -677,10 +771,10 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
         const int a = tile / row_tiles, row0 = (tile - a * row_tiles) * ROWS;
         if (is_moe) {
           moe_factors(args.moe, args.M, moe.list[a], ep_tid, moe);
-          named_bar_sync(1, 256);
+          named_bar_sync(1, EPI);
         }
         T* const oa = out + static_cast<long long>(a) * args.M * ld;
-        finish_tile<2, true, MT, 256>(begin, first, last, sp, ep_tid,
+        finish_tile<2, true, MT, EPI>(begin, first, last, sp, ep_tid,
                                       [&](int, int r, int i, const float4& gate, const float4& up) {
           const int wr = row0 + r;
           if (wr < args.rows)
@@ -689,14 +783,14 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
         });
       } else {
         const T* const res = static_cast<const T*>(args.residual);
-        finish_tile<2, false, MT, 256>(begin, first, last, sp, ep_tid,
+        finish_tile<2, false, MT, EPI>(begin, first, last, sp, ep_tid,
                                        [&](int t, int r, int i, const float4& v, const float4&) {
           const int wr = tile * ROWS + t * 128 + r;
           if (wr < args.rows)
             emit_product(out + wr, res ? res + wr : nullptr, ld, args.M, i, v, b0 ? static_cast<float>(b0[wr]) : 0.f, mp);
         });
       }
-      named_bar_sync(1, 256);  // the slot, f and hit are free for the next tile
+      named_bar_sync(1, EPI);  // the slot, f and hit are free for the next tile
     };
     Pending pending;
     bool alive = true;
@@ -791,9 +885,9 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int c = 0; c < COLS / 2; ++c) f2_unpack(v[t][c], f[t][2 * c], f[t][2 * c + 1]);
-      if (!(alive = end_segment<2, COLS, MT, 256>(f, s, sp, col0, row, ep_tid, pending, emit_tile))) break;
+      if (!(alive = end_segment<2, COLS, MT, EPI>(f, s, sp, col0, row, ep_tid, pending, emit_tile))) break;
     }
-    if (alive) end_units<256>(pending, per_tile, sp, ep_tid, emit_tile);
+    if (alive) end_units<EPI>(pending, per_tile, sp, ep_tid, emit_tile);
   }
 
   tc_fence_before_sync();
