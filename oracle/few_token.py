@@ -9,7 +9,8 @@ The bounds count, term by term,
     core may truncate, hence 2^-23 and not 2^-24); a sum of n columns in groups of G takes at most n / 16 steps of the
     matrix instruction (16 columns each, counted as 2 additions) and n / G of the group sums, and at most 32 joins;
   * 4-bit products only: an activation enters as a sum of e4m3 numbers that is off by at most 2^-17 of the largest
-    activation of its token and group;
+    activation of its token and group (up to 4 tokens), or of its token (a token's rows of all experts in the down
+    projection of a mixture);
   * the gate activation in 32 bits: 2^-19 relative (exp and division of the fast kind, each below 2^-21), and
     its slope, at most 1.13 for every activation here.
 """
@@ -37,12 +38,19 @@ def _half_step(v: Tensor, dt: torch.dtype) -> Tensor:
     return v.abs() * (f.eps / 2) + f.smallest_normal * f.eps / 2
 
 
+def _block_largest(x: Tensor, group: int) -> Tensor:
+    """The value that the error of an element's terms is relative to."""
+    if x.shape[0] <= 4:
+        return _largest(x, group)
+    return x.abs().amax(-1, keepdim=True).expand_as(x)
+
+
 def _largest(x: Tensor, group: int) -> Tensor:
     """|x| of every element replaced by the largest of its group of columns."""
     return x.abs().unflatten(-1, (-1, group)).amax(-1, keepdim=True).expand(*x.shape[:-1], -1, group).flatten(-2)
 
 
-def product(x: Tensor, w: Tensor, group: int = 0):
+def product(x: Tensor, w: Tensor, group: int = 0, largest: Tensor | None = None):
     """x w^T in 64 bits and the bound of its 32-bit sums (group > 0: on 4-bit weights with that group size). A 4-bit
     product adds up q and takes the zero point off at the end: its magnitudes are up to (15 + 15) scale, where the
     group's largest |w| is at least 7.5 scale (weights made by a quantiser that uses the range): 4 times that."""
@@ -53,7 +61,7 @@ def product(x: Tensor, w: Tensor, group: int = 0):
         return v, (x.abs() @ w.abs().transpose(-1, -2)) * (steps * 2.0 ** -23)
     size = 4 * _largest(w, group)
     return v, (x.abs() @ size.transpose(-1, -2)) * (steps * 2.0 ** -23) + \
-        (_largest(x, group) @ w.abs().transpose(-1, -2)) * 2.0 ** -17
+        ((_block_largest(x, group) if largest is None else largest) @ w.abs().transpose(-1, -2)) * 2.0 ** -17
 
 
 _ACTS = {
@@ -63,10 +71,10 @@ _ACTS = {
 }
 
 
-def hidden(x: Tensor, wg: Tensor, bg, wu: Tensor, bu, act: str, group: int = 0):
+def hidden(x: Tensor, wg: Tensor, bg, wu: Tensor, bu, act: str, group: int = 0, largest: Tensor | None = None):
     """act(x wg^T + bg) * (x wu^T + bu) before its rounding, and the bound."""
-    g, dg = product(x, wg, group)
-    u, du = product(x, wu, group)
+    g, dg = product(x, wg, group, largest)
+    u, du = product(x, wu, group, largest)
     g = g if bg is None else g + bg
     u = u if bu is None else u + bu
     a = _ACTS[act](g)
@@ -119,17 +127,27 @@ def moe(x, ids, weights, wg, wu, wd, residual, dt, act="silu", group: int = 0):
     top = torch.where(valid, weights.double().abs(), torch.zeros_like(weights).double()).amax(1, keepdim=True)
     y, dy = torch.zeros_like(x), torch.zeros_like(x)
     active = int(hit.any(0).sum())
+    x_largest = _block_largest(x, group) if group else None
+    parts = []
     for e in range(E):
         t = torch.nonzero(hit[:, e])[:, 0]
         if len(t) == 0:
             continue
-        h, dh = hidden(x[t], wg[e], None, wu[e], None, act, group)
+        h, dh = hidden(x[t], wg[e], None, wu[e], None, act, group, None if x_largest is None else x_largest[t])
         f = torch.where(top[t] > 0, share[t, e][:, None] / top[t], torch.zeros_like(top[t]))
         h, dh = h * f, dh * f.abs() + (h * f).abs() * 2.0 ** -22
-        dh = dh + _half_step(h, dt)
+        parts.append((e, t, h, dh + _half_step(h, dt)))
+    # what a token's hidden values are relative to when they become terms: their group, or all its hidden values
+    token_largest = torch.zeros((T, 1), dtype=torch.float64, device=x.device)
+    for e, t, h, dh in parts:
+        token_largest[t] = torch.maximum(token_largest[t], h.abs().amax(1, keepdim=True))
+    for e, t, h, dh in parts:
+        largest = None
+        if group:
+            largest = _largest(h, group) if T <= 4 else token_largest[t].expand_as(h)
         y[t] += top[t] * (h @ wd[e].t())
         # one sum over all active experts: its steps count for every part
-        own = product(h, wd[e], group)[1]
+        own = product(h, wd[e], group, largest)[1]
         dy[t] += top[t] * (dh @ wd[e].abs().t() + own * active)
     return finish(y, dy + y.abs() * 2.0 ** -22, None, None if residual is None else residual.double(), dt)
 

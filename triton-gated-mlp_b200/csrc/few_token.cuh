@@ -260,10 +260,28 @@ __device__ __forceinline__ void hidden4(float (&h)[4], const float4& g, const fl
   h[2] = act_fine<ACT>(g.z + bg) * (u.z + bu);
   h[3] = act_fine<ACT>(g.w + bg) * (u.w + bu);
 }
-// Four tokens of a hidden row: act(gate + bg) * (up + bu), on experts times the token's factor, or 0.
+// Four tokens' factors, 1 without any.
+__device__ __forceinline__ float4 token_factors(const float* rs, int M, int i) {
+  float4 r = make_float4(1.f, 1.f, 1.f, 1.f);
+  if (rs != nullptr) {
+    r.x = rs[4 * i];
+    if (4 * i + 1 < M) r.y = rs[4 * i + 1];
+    if (4 * i + 2 < M) r.z = rs[4 * i + 2];
+    if (4 * i + 3 < M) r.w = rs[4 * i + 3];
+  }
+  return r;
+}
+__device__ __forceinline__ float4 times(const float4& a, const float4& b) {
+  return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w);
+}
+// Four tokens of a hidden row: act(gate + bg) * (up + bu), on experts times the token's factor, or 0. rs: [M] factors on
+// the sums, or null.
 template <typename T>
-__device__ __forceinline__ void emit_hidden(T* po, long long ld, int M, int i, const float4& gate, const float4& up,
+__device__ __forceinline__ void emit_hidden(T* po, long long ld, int M, int i, float4 gate, float4 up, const float* rs,
                                             float bg, float bu, int act, const MoeShared* moe) {
+  const float4 r = token_factors(rs, M, i);
+  gate = times(gate, r);
+  up = times(up, r);
   float h[4];
   switch (act) {
     case ACT_SILU: hidden4<ACT_SILU>(h, gate, up, bg, bu); break;
@@ -284,10 +302,11 @@ __device__ __forceinline__ void emit_hidden(T* po, long long ld, int M, int i, c
     }
   }
 }
-// Four tokens of an output row: v (* wmax) + bias + residual.
+// Four tokens of an output row: v (* rs) (* wmax) + bias + residual.
 template <typename T>
-__device__ __forceinline__ void emit_product(T* po, const T* pr, long long ld, int M, int i, const float4& v, float bias,
-                                             const MoeShared* moe) {
+__device__ __forceinline__ void emit_product(T* po, const T* pr, long long ld, int M, int i, float4 v, const float* rs,
+                                             float bias, const MoeShared* moe) {
+  v = times(v, token_factors(rs, M, i));
   const float a[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {

@@ -47,10 +47,10 @@ static int check_group(int32_t group, int64_t cols) {
   return GMLP_OK;
 }
 
-// Work buffer of a 4-bit call: [hidden state][activation terms][their meta data]. The terms of x and, later, of the
-// hidden state take turns in one place.
+// Work buffer of a 4-bit call: [hidden state][activation terms][group sums][token factors]. The terms of x and, later, of the
+// hidden state take turns in one place; up to W4_FUSED_TOKENS tokens there is only the hidden state.
 struct W4Work {
-  size_t t8_off, meta_off, total;
+  size_t t8_off, meta_off, row_off, total;
 };
 static size_t w4_t8_bytes(int64_t rows, int64_t cols, int dtype) {
   return static_cast<size_t>(dtype == GMLP_BF16 ? w4_terms<__nv_bfloat16>() : w4_terms<__half>()) * rows * cols;
@@ -59,16 +59,19 @@ static size_t w4_t8_bytes(int64_t rows, int64_t cols, int dtype) {
 static W4Work w4_work(int64_t M, int64_t K, int64_t N, int64_t active, int group, int dtype) {
   W4Work w;
   w.t8_off = align_up(static_cast<size_t>(active * M * N) * 2, 256);
+  w.meta_off = w.row_off = w.total = std::max<size_t>(w.t8_off, 16);
+  if (M <= W4_FUSED_TOKENS) return w;
   w.meta_off = w.t8_off + align_up(std::max(w4_t8_bytes(M, K, dtype), w4_t8_bytes(active * M, N, dtype)), 256);
   const int64_t k_units = (K + W4_UNIT_COLS - 1) / W4_UNIT_COLS, n_units = (N + W4_UNIT_COLS - 1) / W4_UNIT_COLS;
-  w.total = w.meta_off + static_cast<size_t>(std::max(k_units, active * n_units)) * (W4_UNIT_COLS / group) * 2 * w4_mt(M) *
-                             sizeof(float);
+  w.row_off = w.meta_off + static_cast<size_t>(std::max(k_units, active * n_units)) * (W4_UNIT_COLS / group) * w4_mt(M) *
+                               sizeof(float);
+  w.total = w.row_off + FEW_MAX_TOKENS * sizeof(float);
   return w;
 }
 
 // Activations as e4m3 terms (see w4_stream.cuh).
-static int launch_split(int64_t M, int64_t R, int64_t cols, int64_t ldx, int group, int dtype, const void* x, void* t8,
-                        void* meta, bool dependent, cudaStream_t stream) {
+static int launch_split(int64_t M, int64_t R, int64_t cols, int64_t ldx, int group, int dtype, const void* x, char* work,
+                        const W4Work& w, const MoeTable& moe, bool dependent, cudaStream_t stream) {
   W4SplitArgs a;
   a.x = x;
   a.ldx = ldx;
@@ -77,17 +80,15 @@ static int launch_split(int64_t M, int64_t R, int64_t cols, int64_t ldx, int gro
   a.MT = w4_mt(M);
   a.cols = static_cast<int>(cols);
   a.gshift = group == 32 ? 0 : (group == 64 ? 1 : 2);
-  a.t8 = static_cast<uint8_t*>(t8);
-  a.meta = static_cast<float*>(meta);
+  a.t8 = reinterpret_cast<uint8_t*>(work + w.t8_off);
+  a.meta = reinterpret_cast<float*>(work + w.meta_off);
+  a.rowscale = reinterpret_cast<float*>(work + w.row_off);
   a.dependent = dependent ? 1 : 0;
-  const int64_t items = R * ((cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS) * 2;
-  const int64_t per_block = W4_SPLIT_THREADS / 16;
-  const int64_t blocks = (items + per_block - 1) / per_block;
-  if (blocks > 0x7fffffffLL) return fail(GMLP_ERR_SHAPE, "too many activations");
-  return dtype == GMLP_BF16 ? launch_few(w4_split_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks),
-                                         W4_SPLIT_THREADS, 0, dependent, stream, a)
-                            : launch_few(w4_split_kernel<__half>, static_cast<unsigned>(blocks), W4_SPLIT_THREADS, 0,
-                                         dependent, stream, a);
+  a.moe = moe;
+  const unsigned grid = static_cast<unsigned>(M) * W4_SPLIT_CLUSTER;
+  return dtype == GMLP_BF16
+             ? launch_few(w4_split_kernel<__nv_bfloat16>, grid, W4_SPLIT_THREADS, 0, dependent, stream, a, W4_SPLIT_CLUSTER)
+             : launch_few(w4_split_kernel<__half>, grid, W4_SPLIT_THREADS, 0, dependent, stream, a, W4_SPLIT_CLUSTER);
 }
 
 static int launch_w4(const DeviceInfo* dev, const W4Call& c, bool dual) {
@@ -126,7 +127,7 @@ static int launch_moe_t(const DeviceInfo* dev, int dtype, int64_t M, int64_t row
   constexpr size_t smem = moe_smem_bytes<MPAD, DUAL>();
   static std::atomic<uint64_t> attr_done{0};
   if ((rc = ensure_smem_attr(kfn, smem, attr_done))) return rc;
-  return launch_few(kfn, grid, MOE_THREADS, smem, true, stream, m0, m1, mx, a);
+  return launch_few(kfn, grid, MOE_THREADS, smem, true, stream, MoeMaps{m0, m1, mx}, a);
 }
 template <bool DUAL, typename... Args>
 static int launch_moe(int mpad, int dtype, const DeviceInfo* dev, Args... args) {
@@ -227,7 +228,8 @@ int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t
   const bool dep = (tuning & (1u << 26)) == 0;  // GMLP_TUNE_ORDINARY_LAUNCH
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool split = M > W4_FUSED_TOKENS;
-  if (split && (rc = launch_split(M, M, cols, ldx, group, dtype, x, wk + ww.t8_off, wk + ww.meta_off, dep, st))) return rc;
+  if (split && (rc = launch_split(M, M, cols, ldx, group, dtype, x, wk, ww, MoeTable{nullptr, nullptr, 0, 0}, dep, st)))
+    return rc;
   W4Call c;
   memset(&c, 0, sizeof(c));
   c.dtype = dtype;
@@ -242,6 +244,7 @@ int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t
   c.ldx = ldx;
   c.t8 = wk + ww.t8_off;
   c.meta = wk + ww.meta_off;
+  c.rowscale = wk + ww.row_off;
   c.bias0 = bias;
   c.residual = residual;
   c.out = y;
@@ -280,7 +283,7 @@ static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const
   const bool dep = sparse || (p->tuning & (1u << 26)) == 0;  // GMLP_TUNE_ORDINARY_LAUNCH
   const int64_t k_units = (p->K + W4_UNIT_COLS - 1) / W4_UNIT_COLS, n_units = (p->N + W4_UNIT_COLS - 1) / W4_UNIT_COLS;
   const bool split = p->M > W4_FUSED_TOKENS;
-  if (split && (rc = launch_split(p->M, p->M, p->K, p->K, group, p->dtype, x, wk + ww.t8_off, wk + ww.meta_off, dep, st)))
+  if (split && (rc = launch_split(p->M, p->M, p->K, p->K, group, p->dtype, x, wk, ww, MoeTable{nullptr, nullptr, 0, 0}, dep, st)))
     return rc;
   W4Call c;
   memset(&c, 0, sizeof(c));
@@ -290,6 +293,7 @@ static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const
   c.group = group;
   c.t8 = wk + ww.t8_off;
   c.meta = wk + ww.meta_off;
+  c.rowscale = wk + ww.row_off;
   c.slots = reinterpret_cast<float*>(sc);
   c.act = p->act;
   c.moe = moe;
@@ -309,8 +313,7 @@ static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const
   c.early = !sparse;
   c.max_units = active * ((p->N + 127) / 128) * k_units;
   if ((rc = launch_w4(dev, c, true))) return rc;
-  if (split && (rc = launch_split(p->M, active * p->M, p->N, p->N, group, p->dtype, wk, wk + ww.t8_off, wk + ww.meta_off,
-                                  true, st)))
+  if (split && (rc = launch_split(p->M, active * p->M, p->N, p->N, group, p->dtype, wk, wk, ww, moe, true, st)))
     return rc;
   c.rows = p->K;
   c.cols = p->N;
@@ -416,25 +419,10 @@ int gmlp_moe_route(int64_t M, int64_t K, int32_t experts, int32_t top_k, int32_t
   // one warp per expert at a time; up to eight blocks a token
   int cluster = 1;
   while (cluster < 8 && cluster * (ROUTE_THREADS / 32) < experts) cluster *= 2;
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(M * cluster));
-  cfg.blockDim = dim3(ROUTE_THREADS);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  cudaError_t e = dtype == GMLP_BF16 ? cudaLaunchKernelEx(&cfg, moe_route_kernel<__nv_bfloat16>, a)
-                                     : cudaLaunchKernelEx(&cfg, moe_route_kernel<__half>, a);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(GMLP_ERR_LAUNCH, "kernel launch: %s", cudaGetErrorString(e));
-  return GMLP_OK;
+  const unsigned grid = static_cast<unsigned>(M * cluster);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == GMLP_BF16 ? launch_few(moe_route_kernel<__nv_bfloat16>, grid, ROUTE_THREADS, 0, true, st, a, cluster)
+                            : launch_few(moe_route_kernel<__half>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
 }
 
 }  // extern "C"

@@ -9,27 +9,45 @@
 namespace gmlp {
 
 // ---------------------------------------------------------------- launching --
-// Launches kfn(args...) with programmatic stream serialization where `dependent`.
-template <typename... KArgs, typename... Args>
-int launch_few(void (*kfn)(KArgs...), unsigned grid, unsigned threads, size_t smem, bool dependent, cudaStream_t stream,
-               const Args&... args) {
+// Launches a kernel with programmatic stream serialization where `dependent`, in clusters where `cluster` > 1.
+inline int launch_few_args(const void* kfn, unsigned grid, unsigned threads, size_t smem, bool dependent,
+                           cudaStream_t stream, void** args, int cluster) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
   if (dependent) {
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kfn, args...);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(GMLP_ERR_LAUNCH, "kernel launch: %s", cudaGetErrorString(e));
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, kfn, args);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(GMLP_ERR_LAUNCH, "kernel launch: %s", cudaGetErrorString(e));
+  }
   return GMLP_OK;
+}
+template <typename A>
+int launch_few(void (*kfn)(const A), unsigned grid, unsigned threads, size_t smem, bool dependent, cudaStream_t stream,
+               A a, int cluster = 1) {
+  void* args[] = {&a};
+  return launch_few_args(reinterpret_cast<const void*>(kfn), grid, threads, smem, dependent, stream, args, cluster);
+}
+template <typename Maps, typename A>
+int launch_few(void (*kfn)(const Maps, const A), unsigned grid, unsigned threads, size_t smem, bool dependent,
+               cudaStream_t stream, Maps m, A a) {
+  void* args[] = {&m, &a};
+  return launch_few_args(reinterpret_cast<const void*>(kfn), grid, threads, smem, dependent, stream, args, 1);
 }
 
 // One 4-bit weight matrix (of one or of all experts).
@@ -48,9 +66,9 @@ struct W4Call {
   int64_t M, rows, cols, experts, R;
   int group;
   W4Matrix w0, w1;
-  const void* x;  // the activations, of pitch ldx (at most W4_FUSED_TOKENS tokens), or their terms
+  const void* x;  // up to W4_FUSED_TOKENS tokens: the activations, of pitch ldx; else their terms:
   int64_t ldx;
-  const void *t8, *meta;
+  const void *t8, *meta, *rowscale;
   const void *bias0, *bias1, *residual;
   void* out;
   float* slots;
@@ -98,6 +116,7 @@ int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
   a.cols = static_cast<int>(c.cols);
   a.status = dev->status_ptr;
   a.meta = static_cast<const float*>(c.meta);
+  a.rowscale = static_cast<const float*>(c.rowscale);
   a.scale0 = static_cast<const uint16_t*>(c.w0.scale);
   a.scale1 = static_cast<const uint16_t*>(c.w1.scale);
   a.zero0 = static_cast<const uint8_t*>(c.w0.zero);
@@ -118,10 +137,6 @@ int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
   if ((rc = ensure_smem_attr(kfn, Conf::SMEM, attr_done))) return rc;
   return launch_few(kfn, grid, Conf::THREADS, Conf::SMEM, c.dependent, c.stream, m, a);
 }
-// Up to this many tokens the stream kernel makes the terms itself, in four warps that have nothing else to do then (a launch
-// less per product); more tokens a unit take those warps longer than the unit's weights take to arrive.
-constexpr int W4_FUSED_TOKENS = 4;
-
 template <int GSHIFT, bool DUAL, typename T>
 int launch_w4_type(const DeviceInfo* dev, const W4Call& c) {
   if (c.M <= W4_FUSED_TOKENS) return launch_w4_t<8, DUAL, T, GSHIFT, true>(dev, c);

@@ -25,6 +25,10 @@ struct MoeArgs {
   MoeTable moe;
 };
 
+struct MoeMaps {
+  CUtensorMap w0, w1, x;
+};
+
 constexpr int MOE_THREADS = 192;
 template <int MPAD, bool DUAL>
 __host__ __device__ constexpr int moe_stage_bytes() {
@@ -42,8 +46,7 @@ constexpr size_t moe_smem_bytes() {
 
 template <int MPAD, bool DUAL, typename T>
 __global__ void __launch_bounds__(MOE_THREADS, 1)
-moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant__ CUtensorMap tmW1,
-                  const __grid_constant__ CUtensorMap tmX, const MoeArgs args) {
+moe_stream_kernel(const __grid_constant__ MoeMaps maps, const MoeArgs args) {
   constexpr int NACC = DUAL ? 2 : 1;
   constexpr int STAGES = moe_stages<MPAD, DUAL>();
   constexpr uint32_t W_BYTES = 16384;
@@ -81,8 +84,8 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
     mbar_init(drain_bar, 1);
     mbar_fence_init();
     fence_proxy_async_smem();
-    tma_prefetch_desc(&tmW0);
-    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&maps.w0);
+    tma_prefetch_desc(&maps.x);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(&tmem_base_holder), TMEM_COLS);
@@ -145,12 +148,12 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
         const int y = moe.list[pw.a] * args.rows + pw.rt * 128;
         const uint32_t sw = smem_base + st * STAGE_BYTES;
         mbar_expect_tx(full_bar(st), STAGE_BYTES);
-        tma_load_2d_hint(sw, &tmW0, full_bar(st), pw.kb * 64, y, pol_w);
-        if (DUAL) tma_load_2d_hint(sw + W_BYTES, &tmW1, full_bar(st), pw.kb * 64, y, pol_w);
+        tma_load_2d_hint(sw, &maps.w0, full_bar(st), pw.kb * 64, y, pol_w);
+        if (DUAL) tma_load_2d_hint(sw + W_BYTES, &maps.w1, full_bar(st), pw.kb * 64, y, pol_w);
         step(pw);
       };
       auto load_x = [&](int st) {
-        tma_load_2d_hint(smem_base + st * STAGE_BYTES + X_OFF, &tmX, full_bar(st), px.kb * 64,
+        tma_load_2d_hint(smem_base + st * STAGE_BYTES + X_OFF, &maps.x, full_bar(st), px.kb * 64,
                          DUAL ? 0 : px.a * args.M, pol_x);
         step(px);
       };
@@ -253,13 +256,13 @@ moe_stream_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constan
         T* const oa = out + static_cast<long long>(a) * args.M * ld;
         finish_tile<NACC, true, MPAD, 128>(begin, first, last, sp, ep_tid,
                                            [&](int, int r, int i, const float4& gate, const float4& up) {
-          if (row0 + r < args.rows) emit_hidden(oa + row0 + r, ld, args.M, i, gate, up, 0.f, 0.f, args.act, &moe);
+          if (row0 + r < args.rows) emit_hidden(oa + row0 + r, ld, args.M, i, gate, up, nullptr, 0.f, 0.f, args.act, &moe);
         });
       } else {
         finish_tile<NACC, false, MPAD, 128>(begin, first, last, sp, ep_tid,
                                             [&](int, int r, int i, const float4& v, const float4&) {
           const int wr = tile * 128 + r;
-          if (wr < args.rows) emit_product(out + wr, res ? res + wr : nullptr, ld, args.M, i, v, 0.f, &moe);
+          if (wr < args.rows) emit_product(out + wr, res ? res + wr : nullptr, ld, args.M, i, v, nullptr, 0.f, &moe);
         });
       }
       named_bar_sync(1, 128);  // the slot, f and hit are free for the next tile
@@ -337,6 +340,7 @@ moe_route_kernel(const RouteArgs args) {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
   const long long token = blockIdx.x / size;
   pdl_launch_dependents();
+  cluster_sync_all();  // the first block's shared memory is written below: it has to be there
   pdl_wait();
   const T* const x = static_cast<const T*>(args.x) + token * args.ldx;
   const int e0 = static_cast<int>(static_cast<long long>(args.E) * rank / size);

@@ -9,29 +9,34 @@
 //    8..15 the first binade, with the same spacing). So a packed word needs two masks and a shift to become eight
 //    operands of tcgen05.mma.kind::f8f6f4, exactly:  q 2^-9.
 // 2. An activation is a short sum of 8-bit floats. e4m3 has 4 significant bits, bf16 8, fp16 11: with a power of
-//    two per token and group that brings the group's largest value to [128, 256),
+//    two that brings the largest value of a block of activations to [128, 256),
 //      x 2^e = t_1 + t_2 (bf16)   or   t_1 + t_2 + t_3 (fp16),   t_i the e4m3 rounding of what is left.
-//    That is exact for values within 2^-9 (bf16) or 2^-6 (fp16) of the group's largest; below, the error is at most
-//    2^-10 (half the spacing of e4m3's subnormals) where the largest is at least 2^7: 2^-17 of the group's largest
+//    That is exact for values within 2^-9 (bf16) or 2^-6 (fp16) of the block's largest; below, the error is at most
+//    2^-10 (half the spacing of e4m3's subnormals) where the largest is at least 2^7: 2^-17 of the block's largest
 //    value, 256 (bf16) or 32 (fp16) times less than that value's own half step.
-//    The terms are separate columns of the MMA (the tensor pipe is idle at so few columns), so nothing else changes.
+//    The terms are MMAs into one accumulator (the tensor pipe has the time: an MMA of N <= 64 columns takes N / 2 clocks, at
+//    least 16, and the weights of one arrive every 89).
+//    The block: up to 4 tokens, a token and group (terms made inside the kernel, unit by unit); above, a whole token.
 // Per row r, token m:
-//   y[r][m] = sum_g 512 s[r][g] * ( 2^-e(m,g) * sum_i acc_i[r][m]  -  z[r][g] * 2^-9 sx[m][g] ),
-//   acc_i = sum_{c in g} (q[r][c] 2^-9) t_i[c][m],   sx = sum_{c in g} x[m][c]
+//   y[r][m] = 512 sum_g s[r][g] * ( acc[r][m]  -  z[r][g] * sx[m][g] ) * 2^-e,
+//   acc = sum_i sum_{c in g} (q[r][c] 2^-9) t_i[c][m],   sx = 2^-9 sum_{c in g} x[m][c] 2^e
 // with the scale, the zero point and the power of two applied in 32 bits when a group's sums leave tensor memory:
 // neither weights nor activations are rounded (but for the bound above), and that work is per token and group, not per
-// weight. (Expanding to 16-bit operands instead was built first: exact integers q - zero in bf16 / fp16. It ran at
+// weight: three operations per token and group while 2^-e belongs to the group, two when it belongs to the token. That
+// is why it does from 5 tokens on: those operations, and fetching sx and 2^-e, are what 64 tokens wait for.
+// (Expanding to 16-bit operands instead was built first: exact integers q - zero in bf16 / fp16. It ran at
 // 1.5 TB/s: three times the instructions per weight, twice the tensor-memory traffic, twice the MMAs.)
 //
 // Path of a weight: HBM -> shared memory by TMA (packed, 128 rows x 128 bytes = 256 columns per tile, two tiles a
 // unit) -> registers of the thread that owns its row -> tensor memory (tcgen05.st), from which the MMA takes its A
 // operand (128 weight rows; the tokens' terms are the N dimension). Shared memory carries only packed weights.
 //
-// Kernels of a product: w4_split_kernel (terms, powers of two and group sums of the activations, a few microseconds of
-// latency that hide behind the weight stream's start), then w4_stream_kernel.
+// Kernels of a product: w4_stream_kernel; from 5 tokens on w4_split_kernel before it (terms, powers of two and group sums of
+// the activations, a few microseconds of latency that hide behind the weight stream's start).
 // Warps of w4_stream_kernel: 0 streams weights (TMA), 1 issues MMA, 2 streams activation terms, scales and zeros (TMA), 3
-// scales and zeros whose rows are not aligned (cp.async), 4..11 expand (four per tile, thread = row), 12..19 take the sums
-// and run the epilogue (four per half of the tokens, thread = a row of both tiles). Everything between two roles is a ring with full / empty barriers, and
+// packs scales and zeros, and copies those whose rows are not aligned (cp.async), 4..11 expand (four per tile, thread = row), 12..19 take the sums
+// and run the epilogue (thread = a row of both tiles; up to 4 tokens 12..15, and 16..19 make activation terms; up to 32 tokens
+// four warps per half of the tokens, 64 tokens four per quarter). Everything between two roles is a ring with full / empty barriers, and
 // every ring turns once a unit (65,536 weights, 1,400 clocks at the copy bandwidth): a role that is one thread or one warp
 // executes an instruction every 5 to 10 clocks, so its instructions per unit are counted, and the group size is a template
 // parameter to keep them straight-line. (With hand-overs per 128 columns and run-time group loops the thread that
@@ -60,30 +65,23 @@ __host__ __device__ constexpr int w4_terms<__half>() {
 }
 
 // ---- activations -> terms ----
-// Eight columns of a lane, groups of `width` neighbouring lanes: the terms' codes (bytes in the order in which the
-// expanders' masks deliver a word's nibbles: columns 0 4 1 5 | 2 6 3 7), 2^-e and 2^-9 times the group's sum.
+// The power of two, as an exponent, that brings `amax` to [128, 256); limited so that it and its inverse are normal numbers.
+__device__ __forceinline__ int split_exponent(float amax) {
+  const int ex = 7 - (static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127);
+  return ex > 120 ? 120 : ex;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+// Eight columns of a lane times 2^ex: the terms' codes (bytes in the order in which the expanders' masks deliver a word's
+// nibbles: columns 0 4 1 5 | 2 6 3 7); returns the sum of the terms.
 template <int TERMS>
-__device__ __forceinline__ void split_terms(const float (&v)[8], int width, uint2 (&codes)[TERMS], float& down, float& sum) {
-  float amax = 0.f;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    amax = fmaxf(amax, fabsf(v[i]));
-    bad |= !(fabsf(v[i]) < INFINITY);
-  }
-  for (int o = 1; o < width; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  // 2^e: the largest value goes to [128, 256). e is limited so that 2^e and 2^-e are normal numbers.
-  int ex = 7 - (static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127);
-  ex = ex > 120 ? 120 : ex;
-  const float up = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
-  down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-  float rest[8];
-  sum = 0.f;
+__device__ __forceinline__ float split_terms(const float (&v)[8], int ex, uint2 (&codes)[TERMS]) {
+  constexpr int PERM[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+  const float up = power_of_two(ex);
+  float rest[8], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) rest[i] = v[i] * up;
 #pragma unroll
   for (int t = 0; t < TERMS; ++t) {
-    constexpr int PERM[8] = {0, 4, 1, 5, 2, 6, 3, 7};
     uint32_t pair[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -97,58 +95,109 @@ __device__ __forceinline__ void split_terms(const float (&v)[8], int width, uint
     }
     codes[t] = make_uint2(pair[0] | (pair[1] << 16), pair[2] | (pair[3] << 16));
   }
-  if (bad) sum = __uint_as_float(0x7fc00000u);
-  for (int o = 1; o < width; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (sum != sum) down = sum;  // a non-finite activation: the token's outputs become NaN
-  sum *= down * 0.001953125f;
+  return sum;
 }
+// Largest magnitude of eight columns; a NaN or an infinity gives NaN, which then belongs in the token's outputs.
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+  float amax = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    amax = fmaxf(amax, fabsf(v[i]));
+    bad |= !(fabsf(v[i]) < INFINITY);
+  }
+  return bad ? __uint_as_float(0x7fc00000u) : amax;
+}
+__device__ __forceinline__ float nan_max(float a, float b) { return (b > a || b != b) ? b : a; }
 
-// x [R][cols] (row pitch ldx) -> t8 [TERMS][R][cols] e4m3 bytes, inside every 8 columns in the order in which
-// the expanders' masks deliver a word's nibbles, and meta [R / M][groups][2][MT] floats: 2^-e, 2^-9 * sum, with the groups
-// of a row padded to whole units of 256 columns (zeros there). 16 lanes take the 128 columns of a half unit (8 each);
-// a group is 4, 8 or 16 lanes.
+// x [active][M][cols] (row pitch ldx) -> t8 [TERMS][R][cols] e4m3 bytes, meta [active][groups][MT] floats 2^-9 sum_g x 2^e with
+// the groups of a row padded to whole units of 256 columns (zeros there), and per token 512 2^-e (NaN where the token holds
+// a NaN or an infinity). A cluster of blocks per token: each takes a share of the token's half units (128 columns, 16
+// lanes of 8; a group is 4, 8 or 16 lanes), finds their largest value, and goes over them again with the token's.
 struct W4SplitArgs {
   const void* x;
   long long ldx;
-  long long R;  // rows: M, or active experts * M
+  long long R;  // rows of a plane of t8
   int M, MT, cols, gshift;
   uint8_t* t8;
   float* meta;
+  float* rowscale;
   int dependent;
+  MoeTable moe;
 };
 constexpr int W4_SPLIT_THREADS = 256;
+constexpr int W4_SPLIT_CLUSTER = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(W4_SPLIT_THREADS)
 w4_split_kernel(const W4SplitArgs args) {
   constexpr int TERMS = w4_terms<T>();
+  __shared__ MoeShared moe;
+  __shared__ float warp_max[W4_SPLIT_THREADS / 32];
+  __shared__ float block_max[W4_SPLIT_CLUSTER];
   pdl_launch_dependents();
+  cluster_sync_all();  // the other blocks' shared memory is written below: they have to be there
   if (args.dependent) pdl_wait();
-  const int lane = threadIdx.x & 31, sub = lane & 15;
+  moe_collect(args.moe, args.M, moe);
+  const uint32_t rank = cluster_ctarank();
+  const int m = blockIdx.x / W4_SPLIT_CLUSTER;
+  const int tid = threadIdx.x, lane = tid & 31, sub = lane & 15;
   const int blocks = (args.cols + W4_UNIT_COLS - 1) / W4_UNIT_COLS * 2;  // half units of a row, padded to whole units
-  const long long items = args.R * blocks;
-  const long long item = (blockIdx.x * (W4_SPLIT_THREADS / 32LL) + (threadIdx.x >> 5)) * 2 + (lane >> 4);
-  const long long row = item / blocks;
-  const int col = static_cast<int>(item - row * blocks) * W4_HALF_COLS + sub * 8;
-  const bool live = item < items && col < args.cols;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (live) load8(static_cast<const T*>(args.x) + row * args.ldx + col, v);
-  const int width = 4 << args.gshift;  // lanes per group
-  uint2 code[TERMS];
-  float down, sum;
-  split_terms<TERMS>(v, width, code, down, sum);
-  if (live) {
+  const int items = moe.n * blocks;
+  const int lo = static_cast<int>(static_cast<long long>(items) * rank / W4_SPLIT_CLUSTER);
+  const int hi = static_cast<int>(static_cast<long long>(items) * (rank + 1) / W4_SPLIT_CLUSTER);
+  auto load = [&](int item, float (&v)[8]) {  // true: the lane's columns exist
+    const int a = item / blocks, col = (item - a * blocks) * W4_HALF_COLS + sub * 8;
+    const bool live = item < hi && col < args.cols;
 #pragma unroll
-    for (int t = 0; t < TERMS; ++t)
-      *reinterpret_cast<uint2*>(args.t8 + (t * args.R + row) * args.cols + col) = code[t];
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    if (live) load8(static_cast<const T*>(args.x) + (static_cast<long long>(a) * args.M + m) * args.ldx + col, v);
+    return live;
+  };
+  float amax = 0.f;
+  for (int item = lo + (tid >> 4); item < hi; item += W4_SPLIT_THREADS / 16) {
+    float v[8];
+    load(item, v);
+    amax = nan_max(amax, amax8(v));
   }
-  if (item < items && (sub & (width - 1)) == 0) {
-    const long long a = row / args.M, m = row - a * args.M;
-    const int groups = blocks * (4 >> args.gshift);
-    const long long g = col >> (5 + args.gshift);
-    float* const p = args.meta + ((a * groups + g) * 2) * args.MT + m;
-    p[0] = down;
-    p[args.MT] = sum;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = nan_max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (lane == 0) warp_max[tid >> 5] = amax;
+  __syncthreads();
+  if (tid < W4_SPLIT_CLUSTER) {
+    amax = warp_max[0];
+#pragma unroll
+    for (int i = 1; i < W4_SPLIT_THREADS / 32; ++i) amax = nan_max(amax, warp_max[i]);
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&block_max[rank]), tid)), "f"(amax)
+                 : "memory");
+  }
+  __syncwarp();
+  cluster_sync_all();
+  amax = block_max[0];
+#pragma unroll
+  for (int i = 1; i < W4_SPLIT_CLUSTER; ++i) amax = nan_max(amax, block_max[i]);
+  const bool bad = amax != amax;
+  const int ex = bad ? 0 : split_exponent(amax);
+  if (rank == 0 && tid == 0) args.rowscale[m] = bad ? amax : 512.0f * power_of_two(-ex);
+  const int width = 4 << args.gshift;  // lanes per group
+  for (int first = lo; first < hi; first += W4_SPLIT_THREADS / 16) {
+    const int item = first + (tid >> 4);
+    float v[8];
+    const bool live = load(item, v);
+    uint2 code[TERMS];
+    float sum = split_terms<TERMS>(v, ex, code);
+    for (int o = 1; o < width; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (item >= hi) continue;
+    const int a = item / blocks, col = (item - a * blocks) * W4_HALF_COLS + sub * 8;
+    if (live) {
+      uint8_t* const p = args.t8 + (static_cast<long long>(a) * args.M + m) * args.cols + col;
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) *reinterpret_cast<uint2*>(p + t * args.R * args.cols) = code[t];
+    }
+    if ((sub & (width - 1)) == 0) {
+      const long long g = static_cast<long long>(a) * (blocks * (4 >> args.gshift)) + (col >> (5 + args.gshift));
+      args.meta[g * args.MT + m] = sum * 0.001953125f;
+    }
   }
 }
 
@@ -163,11 +212,12 @@ struct W4Args {
   int kbt;         // units along an expert's columns: ceil(cols / 256)
   int groups;      // cols / G
   long long R;     // rows of a plane of activation terms
-  const void* x;   // FUSED: the activations themselves, [M] or [active * M] rows of pitch ldx
+  const void* x;   // FUSED: the activations, [M] or [active * M] rows of pitch ldx
   long long ldx;
   int cols;
   int* status;
-  const float* meta;       // [experts in h or 1][kbt * groups per unit][2][MT]
+  const float* meta;       // not FUSED: [experts in h or 1][kbt * groups per unit][MT] sx
+  const float* rowscale;   // not FUSED: [M] 512 2^-e
   const uint16_t* scale0;  // [experts][groups][rows], T
   const uint16_t* scale1;  // DUAL: the up matrix's
   const uint8_t* zero0;    // [experts][groups][rows] or null (8)
@@ -189,28 +239,35 @@ struct W4Args {
 constexpr int W4_META_ROW = 416;
 constexpr int W4_META_ZERO = 272;
 
+// FUSED: the terms are made in the kernel, with a power of two per token and group. Four warps make them, each takes a (unit,
+// token) pair in turn; a pair takes about 800 clocks, a unit's weights 1,400 to arrive, which carries four tokens (8
+// tokens, 28672 x 8192: 85 us, 73 with six such warps, against 50 with the terms made beforehand).
+constexpr int W4_FUSED_TOKENS = 4;
 template <int MT, int TERMS, int GSHIFT, bool FUSED>
 struct W4Conf {
-  static_assert(!FUSED || MT == 8, "the fused form takes up to four tokens");
+  static_assert(!FUSED || MT == 8, "one instantiation of each fused form");
   static constexpr int N = MT < 16 ? 16 : MT;      // columns of the MMA; those behind MT hold nothing of use
-  // accumulating threads: four warps per share of the tokens; 64 tokens take sixteen warps, since with eight each thread's
-  // 64 sums left two warps a scheduler, whose loads and products wait for each other (103 against 8x us)
+  // accumulating threads: four warps per share of the tokens; 64 tokens take sixteen warps (with eight, 64 sums a thread)
   static constexpr int SHARES = FUSED ? 1 : (MT == 64 ? 4 : 2);
   static constexpr int EPI = 128 * SHARES;
-  static constexpr int THREADS = 32 * (12 + 4 * SHARES + (FUSED ? 4 : 0));
+  static constexpr int CONVERTERS = FUSED ? 4 : 0;
+  static constexpr int THREADS = 32 * (12 + 4 * SHARES + CONVERTERS);
   static constexpr int GPH = 4 >> GSHIFT;          // groups per half unit (128 columns)
   static constexpr int GPU = 2 * GPH;              // groups per unit
-  // activation terms of a unit: [two halves][TERMS] of N rows x 128 columns, then meta [GPU][2][MT]
+  static constexpr int FACTORS = FUSED ? 2 : 1;    // per token and group: 2^-e (FUSED) and sx
+  // activation terms of a unit: [two halves][TERMS] of N rows x 128 columns, then [GPU][FACTORS][MT] factors
   static constexpr int X_TERM = N * 128;
   static constexpr int X_HALF = TERMS * X_TERM;
-  static constexpr int X_STAGE = (2 * X_HALF + GPU * 2 * MT * 4 + 1023) / 1024 * 1024;
-  static constexpr int M_STAGE = 2 * GPU * W4_META_ROW;  // scales and zeros of a unit
-  static constexpr int COLS = FUSED ? 4 : MT / SHARES;  // tokens per accumulator thread
+  static constexpr int X_STAGE = (2 * X_HALF + GPU * FACTORS * MT * 4 + 1023) / 1024 * 1024;
+  static constexpr int M_STAGE = 2 * GPU * W4_META_ROW;  // scales and zeros of a unit as they lie in memory
+  static constexpr int S_STAGE = 2 * GPU * 128 * 4;      // and as a word per row: scale << 16 | zero
+  static constexpr int SIDE = X_STAGE + M_STAGE + S_STAGE;
+  static constexpr int COLS = FUSED ? W4_FUSED_TOKENS : MT / SHARES;  // tokens per accumulator thread
   static constexpr int SMEM_MAX = 232448 - 1024 - 4096;
-  static constexpr int X_STAGES = FUSED ? 4 : 3 * (X_STAGE + M_STAGE) + 3 * 2 * W4_TILE_BYTES <= SMEM_MAX ? 3 : 2;
-  static constexpr int FIT = (SMEM_MAX - X_STAGES * (X_STAGE + M_STAGE)) / (2 * W4_TILE_BYTES);
+  static constexpr int X_STAGES = FUSED ? CONVERTERS : 3 * SIDE + 3 * 2 * W4_TILE_BYTES <= SMEM_MAX ? 3 : 2;
+  static constexpr int FIT = (SMEM_MAX - X_STAGES * SIDE) / (2 * W4_TILE_BYTES);
   static constexpr int W_STAGES = FIT > 5 ? 5 : FIT;
-  static constexpr size_t SMEM = 1024 + static_cast<size_t>(W_STAGES) * 2 * W4_TILE_BYTES + X_STAGES * (X_STAGE + M_STAGE);
+  static constexpr size_t SMEM = 1024 + static_cast<size_t>(W_STAGES) * 2 * W4_TILE_BYTES + X_STAGES * SIDE;
   // tensor memory: accumulators in front, expanded weights (128 columns per unit) behind. An accumulator buffer holds as
   // many (tile, group) sums of a unit as leave room for two buffers.
   static constexpr int A_BUFS = 2;
@@ -225,7 +282,7 @@ struct W4Conf {
   static_assert(BUF_PAIRS >= 2, "a buffer holds both tiles' sums of a group");
   static constexpr int C_BUFS_FIT = C_COLS / (BUF_PAIRS * N);
   static constexpr int C_BUFS = C_BUFS_FIT > 4 ? 4 : C_BUFS_FIT;
-  static_assert(W_STAGES >= 3 && C_BUFS >= 2, "rings too shallow");
+  static_assert(W_STAGES >= 2 && C_BUFS >= 2, "rings too shallow");
 };
 
 // ---- tensor memory and MMA ----
@@ -294,6 +351,17 @@ __device__ __forceinline__ uint4 ld_shared_u4(uint32_t a) {
   return v;
 }
 
+// Bounded wait for the producers, which wait most of the time and several units ahead: the hardware parks the warp between
+// polls (each poll takes issue slots from the warps that work).
+__device__ __forceinline__ bool idle_wait(uint32_t bar, uint32_t parity, volatile int* abortp) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    if (__all_sync(0xffffffffu, mbar_try_wait_suspend(bar, parity, 2000u))) return true;
+    if (__any_sync(0xffffffffu, *abortp != 0 || clock64() - t0 > WAIT_LIMIT_CYCLES)) return false;
+    __nanosleep(100);
+  }
+}
 // Bounded wait of a whole warp that polls without the suspend hint of mbar_wait: the hand-over from warp to warp takes
 // 125 clocks instead of 213 (measured), and these roles hand over every few hundred clocks.
 __device__ __forceinline__ bool quick_wait(uint32_t bar, uint32_t parity, volatile int* abortp) {
@@ -346,7 +414,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   constexpr int ROWS = DUAL ? 128 : 256;  // weight rows per row tile
 
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * (NW + NX + NA + NC) + 1];
+  __shared__ __align__(8) uint64_t bars[2 * (NW + NX + NA + NC) + NX + 1];
   __shared__ uint32_t tmem_base_holder;
   __shared__ int abort_flag;
   __shared__ MoeShared moe;
@@ -356,7 +424,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   const uint32_t x_base = w_base + NW * 2 * W4_TILE_BYTES;
   const uint32_t m_base = x_base + NX * C::X_STAGE;
   const uint32_t wfull = smem_u32(bars), wempty = wfull + 8 * NW, xfull = wempty + 8 * NW, xempty = xfull + 8 * NX,
-                 afull = xempty + 8 * NX, aempty = afull + 8 * NA, cfull = aempty + 8 * NA, cempty = cfull + 8 * NC, drain_bar = cempty + 8 * NC;
+                 afull = xempty + 8 * NX, aempty = afull + 8 * NA, cfull = aempty + 8 * NA, cempty = cfull + 8 * NC, sfull = cempty + 8 * NC, drain_bar = sfull + 8 * NX;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -370,6 +438,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       // the TMA bytes, the copying lanes of warp 3, a converting warp per token
       mbar_init(xfull + 8 * s, 1 + (args.wide ? 0 : 32) + (FUSED ? args.M : 0));
       mbar_init(xempty + 8 * s, 1 + C::EPI / 32);
+      mbar_init(sfull + 8 * s, 1);
     }
     for (int b = 0; b < NA; ++b) {
       mbar_init(afull + 8 * b, 8);
@@ -452,7 +521,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     int u = 0;
     bool ok = true;
     for (; u < units; ++u) {
-      if (!(ok = quick_wait(wempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
+      if (!(ok = idle_wait(wempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
       const uint32_t dst = w_base + r.at * 2 * W4_TILE_BYTES, fb = wfull + 8 * r.at;
       const int y = moe.list[w.a] * args.rows + w.row0;
       if (elect_one()) {
@@ -484,10 +553,10 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     int u = 0;
     bool ok = true;
     for (; u < units; ++u) {
-      if (!(ok = quick_wait(xempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
+      if (!(ok = idle_wait(xempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
       const int a = DUAL ? 0 : w.a;
       const uint32_t dst = x_base + r.at * C::X_STAGE, fb = xfull + 8 * r.at;
-      constexpr uint32_t META_BYTES = GPU * 2 * MT * 4;
+      constexpr uint32_t META_BYTES = GPU * MT * 4;
       if (elect_one()) {
         const uint32_t sz_bytes = args.wide ? 2 * GPU * 128 * (2 + (args.zero0 != nullptr ? 1 : 0)) : 0;
         mbar_expect_tx(fb, (FUSED ? 0 : 2 * TERMS * MT * 128 + META_BYTES) + sz_bytes);
@@ -507,7 +576,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
           for (int i = 0; i < 2 * TERMS; ++i)  // a half behind the last column arrives as zeros
             tma_load_2d_hint(dst + i * C::X_TERM, &maps.x, fb, w.kb * W4_UNIT_COLS + (i / TERMS) * W4_HALF_COLS,
                              static_cast<int>((i % TERMS) * args.R) + a * args.M, pol);
-          bulk_load(dst + 2 * C::X_HALF, args.meta + (static_cast<long long>(a) * args.kbt + w.kb) * (GPU * 2 * MT),
+          bulk_load(dst + 2 * C::X_HALF, args.meta + (static_cast<long long>(a) * args.kbt + w.kb) * (GPU * MT),
                     META_BYTES, fb);
         }
       }
@@ -524,28 +593,35 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   } else if (warp == 3) {
     // --------------------------------------------------- scales and zeros --
     if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    // Rows of scales and zeros start anywhere (any number of weight rows is allowed): copied by 4-byte words, up to 65 + 33
-    // per (tile, group), of which the last one only as far as the rows go.
-    W4Walk w;
+    // One word per row, tile and group for all the accumulating threads: scale << 16 | zero. Where the rows of scales and zeros
+    // are not aligned (any number of weight rows is allowed) this warp copies them too, up to 65 + 33 words of 4 bytes per
+    // (tile, group), of which the last one only as far as the rows go, and runs as many units ahead with that as there
+    // are stages.
+    const bool zeros = args.zero0 != nullptr;
+    uint8_t* const m_stages = smem + NW * 2 * W4_TILE_BYTES + NX * C::X_STAGE;
+    uint8_t* const s_stages = m_stages + NX * C::M_STAGE;
+    const int ahead = args.wide ? 0 : NX - 1;
+    W4Walk wc, w;  // positions of the unit being copied and of the unit being packed
+    start(wc);
     start(w);
-    Ring r;
+    Ring rc, r;
     bool ok = true;
-    for (int u = 0; u < units && !args.wide; ++u) {
-      if (!(ok = quick_wait(xempty + 8 * r.at, r.phase ^ 1u, abortp))) break;
-      const int ng = groups_in(w.kb);
-      const long long unit0 = (static_cast<long long>(moe.list[w.a]) * args.groups + w.kb * GPU) * args.rows + w.row0;
+    for (int u = 0; u < units + ahead && ok; ++u) {
+      if (!args.wide && u < units) {
+        if (!(ok = quick_wait(xempty + 8 * rc.at, rc.phase ^ 1u, abortp))) break;
+        const int ng = groups_in(wc.kb);
+        const long long unit0 = (static_cast<long long>(moe.list[wc.a]) * args.groups + wc.kb * GPU) * args.rows + wc.row0;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint16_t* const sc = (DUAL && t == 1) ? args.scale1 : args.scale0;
-        const uint8_t* const ze = (DUAL && t == 1) ? args.zero1 : args.zero0;
-        const int skip = DUAL ? 0 : t * 128;
-        const int left = args.rows - w.row0 - skip;
-        const int nrow = left < 128 ? left : 128;
+        for (int t = 0; t < 2; ++t) {
+          const uint16_t* const sc = (DUAL && t == 1) ? args.scale1 : args.scale0;
+          const uint8_t* const ze = (DUAL && t == 1) ? args.zero1 : args.zero0;
+          const int skip = DUAL ? 0 : t * 128;
+          const int left = args.rows - wc.row0 - skip;
+          const int nrow = left < 128 ? left : 128;
 #pragma unroll 1
-          for (int i = 0; i < ng; ++i) {
-            if (nrow <= 0) continue;
+          for (int i = 0; i < ng && nrow > 0; ++i) {
             const long long e0 = unit0 + skip + static_cast<long long>(i) * args.rows;
-            const uint32_t dst = m_base + r.at * C::M_STAGE + (t * GPU + i) * W4_META_ROW + lane * 4;
+            const uint32_t dst = m_base + rc.at * C::M_STAGE + (t * GPU + i) * W4_META_ROW + lane * 4;
             const int head = static_cast<int>(e0 & 1) * 2, bytes = head + 2 * nrow - lane * 4;
             const char* const s0 = reinterpret_cast<const char*>(sc + e0) - head + lane * 4;
 #pragma unroll
@@ -560,8 +636,44 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
                   cp_async_word(dst + W4_META_ZERO + k * 128, z0 + k * 128, zbytes - k * 128 < 4 ? zbytes - k * 128 : 4);
             }
           }
+        }
+        cp_async_arrive(xfull + 8 * rc.at);
+        step(wc);
+        rc.next(NX);
       }
-      cp_async_arrive(xfull + 8 * r.at);
+      if (u < ahead) continue;
+      if (!(ok = quick_wait(xfull + 8 * r.at, r.phase, abortp))) break;
+      const int ng = groups_in(w.kb);
+      const uint8_t* const mm = m_stages + r.at * C::M_STAGE;
+      uint4* const ss = reinterpret_cast<uint4*>(s_stages + r.at * C::S_STAGE) + lane;  // four rows a lane
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int g = 0; g < GPU; ++g) {
+          uint32_t z = 0x08080808u, s01, s23;
+          if (args.wide) {
+            const uint2 q = *reinterpret_cast<const uint2*>(mm + (t * GPU + g) * 256 + lane * 8);
+            s01 = q.x;
+            s23 = q.y;
+            if (zeros) z = *reinterpret_cast<const uint32_t*>(mm + 2 * GPU * 256 + (t * GPU + g) * 128 + lane * 4);
+          } else {
+            // where the rows start inside the copied words: low bits of the first one's index
+            const uint32_t e = (static_cast<uint32_t>(moe.list[w.a]) * args.groups + w.kb * GPU + g) *
+                                   static_cast<uint32_t>(args.rows) + w.row0 + (DUAL ? 0 : t * 128);
+            const uint8_t* const mr = mm + (t * GPU + g) * W4_META_ROW;
+            const uint16_t* const sp = reinterpret_cast<const uint16_t*>(mr + (e & 1u) * 2) + lane * 4;
+            s01 = sp[0] | (static_cast<uint32_t>(sp[1]) << 16);
+            s23 = sp[2] | (static_cast<uint32_t>(sp[3]) << 16);
+            const uint8_t* const zp = mr + W4_META_ZERO + (e & 3u) + lane * 4;
+            if (zeros) z = zp[0] | (zp[1] << 8) | (zp[2] << 16) | (static_cast<uint32_t>(zp[3]) << 24);
+          }
+          uint4 o = make_uint4((s01 << 16) | (z & 15u), (s01 & 0xFFFF0000u) | ((z >> 8) & 15u),
+                               (s23 << 16) | ((z >> 16) & 15u), (s23 & 0xFFFF0000u) | ((z >> 24) & 15u));
+          if (g >= ng) o = make_uint4(0u, 0u, 0u, 0u);  // a group behind the last column has a scale of zero
+          ss[(t * GPU + g) * 32] = o;
+        }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sfull + 8 * r.at);
       step(w);
       r.next(NX);
     }
@@ -676,45 +788,53 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     const int sub = lane & 15, half = lane >> 4;
     W4Walk wn;  // position of the pair being fetched
     start(wn);
-    // A warp takes every fourth unit at most, and a parity tells a stage's phase only to a waiter that is not a whole turn
-    // of the ring away from it: when a warp has seen unit u - NX released, unit u + 4 - 2 NX has been.
-    static_assert(!FUSED || NX >= 4, "a converting warp would take one phase of a stage for another");
-    Ring r;  // stage of unit `at_unit`
-    int at_unit = 0;
+    // A parity tells a stage's phase only to a waiter that is not a whole turn of the ring away from it: a warp that goes
+    // from unit u to u + d has seen unit u - NX released, and needs u + d - 2 NX to be: d <= NX.
+    static_assert(!FUSED || NX >= C::CONVERTERS, "a converting warp would take one phase of a stage for another");
+    Ring r;  // stage of `unit`
     bool ok = true;
-    auto fetch = [&](int p, const W4Walk& q) {
-      const int m = p % args.M, col = q.kb * W4_UNIT_COLS + lane * 8;
+    auto fetch = [&](int m) {
+      const int col = wn.kb * W4_UNIT_COLS + lane * 8;
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (col < args.cols)
         v = *reinterpret_cast<const uint4*>(static_cast<const T*>(args.x) +
-                                            ((DUAL ? 0 : static_cast<long long>(q.a) * args.M) + m) * args.ldx + col);
+                                            ((DUAL ? 0 : static_cast<long long>(wn.a) * args.M) + m) * args.ldx + col);
       return v;
     };
-    const int pairs = units * args.M;
-    int p = warp - 16;
-    int next_unit = 0;
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (p < pairs) {
-      for (; next_unit < p / args.M; ++next_unit) step(wn);
-      raw = fetch(p, wn);
-    }
-    for (; p < pairs; p += 4) {
-      const uint4 cur = raw;
-      if (p + 4 < pairs) {
-        for (; next_unit < (p + 4) / args.M; ++next_unit) step(wn);
-        raw = fetch(p + 4, wn);
+    // (unit, token) of this pair and, one ahead, of the pair being fetched
+    int unit = 0, m = 0, next_unit = 0, next_m = warp - 16;
+    auto settle_next = [&]() {
+      while (next_m >= args.M) {
+        next_m -= args.M;
+        ++next_unit;
+        if (next_unit < units) step(wn);
       }
+    };
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    settle_next();
+    if (next_unit < units) raw = fetch(next_m);
+    while (next_unit < units) {
+      for (; unit < next_unit; ++unit) r.next(NX);
+      m = next_m;
+      const uint4 cur = raw;
+      next_m += C::CONVERTERS;
+      settle_next();
+      if (next_unit < units) raw = fetch(next_m);
       float v[8];
       const float2 v0 = Pack2<T>::unpack(cur.x), v1 = Pack2<T>::unpack(cur.y), v2 = Pack2<T>::unpack(cur.z),
                    v3 = Pack2<T>::unpack(cur.w);
       v[0] = v0.x; v[1] = v0.y; v[2] = v1.x; v[3] = v1.y;
       v[4] = v2.x; v[5] = v2.y; v[6] = v3.x; v[7] = v3.y;
+      constexpr int WIDTH = 4 << GSHIFT;  // lanes of a group
+      float amax = amax8(v);
+#pragma unroll
+      for (int o = 1; o < WIDTH; o <<= 1) amax = nan_max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      const int ex = amax != amax ? 0 : split_exponent(amax);
       uint2 code[TERMS];
-      float down, sum;
-      constexpr int WIDTH = 4 << GSHIFT;
-      split_terms<TERMS>(v, WIDTH, code, down, sum);
-      const int m = p % args.M;
-      for (; at_unit < p / args.M; ++at_unit) r.next(NX);
+      float sum = split_terms<TERMS>(v, ex, code);
+#pragma unroll
+      for (int o = 1; o < WIDTH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float down = amax != amax ? amax : power_of_two(-ex);
       ok = quick_wait(xempty + 8 * r.at, r.phase ^ 1u, abortp);
       if (!ok) break;
       uint8_t* const xs = smem + NW * 2 * W4_TILE_BYTES + r.at * C::X_STAGE;
@@ -725,7 +845,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       if ((sub & (WIDTH - 1)) == 0) {
         float* const mt = reinterpret_cast<float*>(xs + 2 * C::X_HALF) + (half * GPH + sub / WIDTH) * 2 * MT + m;
         mt[0] = down;
-        mt[MT] = sum;
+        mt[MT] = sum * 0.001953125f;
       }
       fence_proxy_async_smem();  // the MMA reads the terms
       __syncwarp();
@@ -749,9 +869,6 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     const int row = quarter * 32 + lane;
     const uint32_t acc0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
     const int ep_tid = threadIdx.x - 384;
-    const bool zeros = args.zero0 != nullptr;
-    const int s_row = args.wide ? 256 : W4_META_ROW, z_row = args.wide ? 128 : W4_META_ROW;
-    const int z_off = args.wide ? 2 * GPU * 256 : W4_META_ZERO;
     if (args.early) pdl_wait();  // slots, counters and outputs may still be in use
     if (!DUAL && cut.total == 0) {
       // no token chose any expert: the outputs are the residual, or zero
@@ -765,6 +882,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     auto emit_tile = [&](int tile, int begin, int first, int last) {
       T* const out = static_cast<T*>(args.out);
       const T* const b0 = static_cast<const T*>(args.bias0);
+      const float* const rs = FUSED ? nullptr : args.rowscale;
       const long long ld = args.rows;
       if (DUAL) {
         const T* const b1 = static_cast<const T*>(args.bias1);
@@ -778,7 +896,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
                                       [&](int, int r, int i, const float4& gate, const float4& up) {
           const int wr = row0 + r;
           if (wr < args.rows)
-            emit_hidden(oa + wr, ld, args.M, i, gate, up, b0 ? static_cast<float>(b0[wr]) : 0.f,
+            emit_hidden(oa + wr, ld, args.M, i, gate, up, rs, b0 ? static_cast<float>(b0[wr]) : 0.f,
                         b1 ? static_cast<float>(b1[wr]) : 0.f, args.act, mp);
         });
       } else {
@@ -787,7 +905,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
                                        [&](int t, int r, int i, const float4& v, const float4&) {
           const int wr = tile * ROWS + t * 128 + r;
           if (wr < args.rows)
-            emit_product(out + wr, res ? res + wr : nullptr, ld, args.M, i, v, b0 ? static_cast<float>(b0[wr]) : 0.f, mp);
+            emit_product(out + wr, res ? res + wr : nullptr, ld, args.M, i, v, rs, b0 ? static_cast<float>(b0[wr]) : 0.f, mp);
         });
       }
       named_bar_sync(1, EPI);  // the slot, f and hit are free for the next tile
@@ -805,70 +923,75 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       for (int c = 0; c < COLS / 2; ++c) v[0][c] = v[1][c] = 0ull;
       bool ok = true;
       for (; u < s.end; ++u) {
-        const int ng = groups_in(w.kb);
-        // low bits of the first scale's index: where its row starts inside a copied word
-        const uint32_t low = args.wide ? 0u
-                                       : (static_cast<uint32_t>(moe.list[w.a]) * args.groups + w.kb * GPU) *
-                                                 static_cast<uint32_t>(args.rows) + w.row0;
-        const uint32_t low_step = args.wide ? 0u : static_cast<uint32_t>(args.rows);
-        ok = quick_wait(xfull + 8 * rx.at, rx.phase, abortp);
+        // (warp 3 saw the unit's factors land before it arrived here)
+        ok = quick_wait(sfull + 8 * rx.at, rx.phase, abortp);
         // read as ordinary memory, so that the loads between two waits go out together
-        const float* const xm =
-            reinterpret_cast<const float*>(smem + NW * 2 * W4_TILE_BYTES + rx.at * C::X_STAGE + 2 * C::X_HALF) + col0;
-        const uint8_t* const mm = smem + NW * 2 * W4_TILE_BYTES + NX * C::X_STAGE + rx.at * C::M_STAGE;
+        const uint8_t* const side = smem + NW * 2 * W4_TILE_BYTES;
+        const float* const xm = reinterpret_cast<const float*>(side + rx.at * C::X_STAGE + 2 * C::X_HALF) + col0;
+        const uint32_t* const ss =
+            reinterpret_cast<const uint32_t*>(side + NX * (C::X_STAGE + C::M_STAGE) + rx.at * C::S_STAGE) + row;
 #pragma unroll
         for (int g0 = 0; g0 < GPU; g0 += GROUPS) {
           // scales and zeros of the buffer's sums are fetched before the sums are there
           float sc[BUF_PAIRS], nz[BUF_PAIRS];
 #pragma unroll
           for (int b = 0; b < BUF_PAIRS; ++b) {
-            const int t = b & 1, g = g0 + (b >> 1);
-            const uint32_t e = low + (DUAL ? 0 : t * 128) + g * low_step;
-            const uint8_t* const sp = mm + (t * GPU + g) * s_row + (e & 1u) * 2 + row * 2;
-            sc[b] = 512.0f * static_cast<float>(*reinterpret_cast<const T*>(sp));
-            nz[b] = -8.0f;
-            if (zeros)  // an integer below 2^23 in a float's fraction: 2^23 - (2^23 + z)
-              nz[b] = 8388608.0f -
-                      __uint_as_float(0x4B000000u | (mm[z_off + (t * GPU + g) * z_row + (e & 3u) + row] & 15u));
-            if (g >= ng) sc[b] = nz[b] = 0.f;  // a group behind the last column
+            const uint32_t sz = ss[((b & 1) * GPU + g0 + (b >> 1)) * 128];
+            sc[b] = (FUSED ? 512.0f : 1.0f) * Pack2<T>::unpack(sz >> 16).x;
+            // an integer below 2^23 in a float's fraction: 2^23 - (2^23 + z)
+            nz[b] = 8388608.0f - __uint_as_float(0x4B000000u | (sz & 15u));
           }
           ok = ok && quick_wait(cfull + 8 * rc.at, rc.phase, abortp);
           tc_fence_after_sync();
-          if (!idle) {
-            const uint32_t src = acc0 + rc.at * (BUF_PAIRS * N);
+          const uint32_t src = acc0 + rc.at * (BUF_PAIRS * N);
 #pragma unroll
-            for (int b0 = 0; b0 < BUF_PAIRS; b0 += BATCH) {
+          for (int b0 = 0; b0 < BUF_PAIRS; b0 += BATCH) {
 #pragma unroll
-              for (int c = 0; c < COLS; c += CH) {
-                uint32_t x[BATCH][CH];
+            for (int c = 0; c < COLS; c += CH) {
+              uint32_t x[BATCH][CH];
+              if (!idle) {
 #pragma unroll
                 for (int b = 0; b < BATCH; ++b) tmem_ld_cols<CH>(src + (b0 + b) * N + c, x[b]);
                 tmem_ld_wait();
+              }
+              if (b0 + BATCH == BUF_PAIRS && c + CH == COLS) {  // the last sums are in registers
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(cempty + 8 * rc.at);
+              }
+              if (!idle) {
 #pragma unroll
                 for (int k = 0; k < CH; k += 4) {
 #pragma unroll
                   for (int b = 0; b < BATCH; ++b) {
                     const int t = (b0 + b) & 1, g = g0 + ((b0 + b) >> 1);
-                    const float* const xg = xm + g * 2 * MT + c + k;
-                    const float4 q0 = *reinterpret_cast<const float4*>(xg);
-                    const float4 q1 = *reinterpret_cast<const float4*>(xg + MT);
-                    const f32x2 s2 = f2_pack(sc[b0 + b], sc[b0 + b]), z2 = f2_pack(nz[b0 + b], nz[b0 + b]);
+                    const float4 q0 = *reinterpret_cast<const float4*>(xm + g * C::FACTORS * MT + c + k);
+                    const float tok[4] = {q0.x, q0.y, q0.z, q0.w};
+                    if constexpr (FUSED) {
+                      const float4 q1 = *reinterpret_cast<const float4*>(xm + g * 2 * MT + MT + c + k);
+                      const float sx[4] = {q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                      const int o = k + 2 * j;
-                      f32x2 y = f2_mul(f2_pack(__uint_as_float(x[b][o]), __uint_as_float(x[b][o + 1])),
-                                       j == 0 ? f2_pack(q0.x, q0.y) : f2_pack(q0.z, q0.w));
-                      y = f2_fma(z2, j == 0 ? f2_pack(q1.x, q1.y) : f2_pack(q1.z, q1.w), y);
-                      v[t][(c + o) / 2] = f2_fma(s2, y, v[t][(c + o) / 2]);
+                      for (int j = 0; j < 4; j += 2) {
+                        const float y0 = tok[j] * fmaf(nz[b0 + b], sx[j], __uint_as_float(x[b][k + j]));
+                        const float y1 = tok[j + 1] * fmaf(nz[b0 + b], sx[j + 1], __uint_as_float(x[b][k + j + 1]));
+                        v[t][(c + k + j) / 2] =
+                            f2_fma(f2_pack(sc[b0 + b], sc[b0 + b]), f2_pack(y0, y1), v[t][(c + k + j) / 2]);
+                      }
+                    } else {
+                      // two tokens an instruction: what bounds many tokens is issue slots
+                      const f32x2 s2 = f2_pack(sc[b0 + b], sc[b0 + b]), z2 = f2_pack(nz[b0 + b], nz[b0 + b]);
+#pragma unroll
+                      for (int j = 0; j < 4; j += 2) {
+                        f32x2 y = f2_pack(__uint_as_float(x[b][k + j]), __uint_as_float(x[b][k + j + 1]));
+                        y = f2_fma(z2, f2_pack(tok[j], tok[j + 1]), y);
+                        v[t][(c + k + j) / 2] = f2_fma(s2, y, v[t][(c + k + j) / 2]);
+                      }
                     }
                   }
                 }
               }
             }
           }
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(cempty + 8 * rc.at);
           rc.next(NC);
         }
         if (!ok) break;
