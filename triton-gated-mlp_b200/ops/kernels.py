@@ -584,25 +584,29 @@ def dequantize_weight_int4(w: Int4Weight) -> Tensor:
 def _int4_group(w: Int4Weight, lead: tuple, rows: int, cols: int, dt: torch.dtype, dev: torch.device) -> int:
     """Checks a 4-bit weight against the shape it must have; returns its group size."""
     q, s, z = w
-    groups = s.shape[-2] if s.dim() >= 2 else 0
-    if (q.dtype is not torch.uint8 or q.shape != (*lead, rows, cols // 2) or q.device != dev or not q.is_contiguous()
-            or cols % 8):
+    sh = s.shape
+    groups = sh[-2] if len(sh) >= 2 else 0
+    group = cols // groups if groups else 0
+    want = (*lead, groups, rows)
+    if (group in INT4_GROUPS and groups * group == cols and q.dtype is torch.uint8 and q.shape == (*lead, rows, cols // 2)
+            and s.dtype is dt and sh == want and q.is_contiguous() and s.is_contiguous() and q.device == dev
+            and s.device == dev
+            and (z is None or (z.dtype is torch.uint8 and z.shape == want and z.is_contiguous() and z.device == dev))):
+        return group
+    if q.dtype is not torch.uint8 or q.shape != (*lead, rows, cols // 2) or q.device != dev or not q.is_contiguous():
         raise ValueError(f"4-bit weights must be contiguous uint8 of shape {(*lead, rows, cols // 2)} on {dev}; got "
                          f"{q.dtype} {tuple(q.shape)} on {q.device}")
-    group = cols // groups if groups else 0
     if group not in INT4_GROUPS or groups * group != cols:
         raise ValueError(f"4-bit weights of {cols} columns need cols / group scales per row with group in "
                          f"{INT4_GROUPS}; got scales of shape {tuple(s.shape)}")
-    if s.dtype is not dt or s.shape != (*lead, groups, rows) or s.device != dev or not s.is_contiguous():
-        raise ValueError(f"scales must be contiguous {dt} of shape {(*lead, groups, rows)} on {dev}; got {s.dtype} "
+    if s.dtype is not dt or s.shape != want or s.device != dev or not s.is_contiguous():
+        raise ValueError(f"scales must be contiguous {dt} of shape {want} on {dev}; got {s.dtype} "
                          f"{tuple(s.shape)} on {s.device}")
-    if z is not None and (z.dtype is not torch.uint8 or z.shape != s.shape or z.device != dev
-                          or not z.is_contiguous()):
-        raise ValueError(f"zeros must be contiguous uint8 of shape {tuple(s.shape)} on {dev}")
-    return group
+    raise ValueError(f"zeros must be contiguous uint8 of shape {want} on {dev}")
 
 
 _few_scratch: dict = {}
+_FEW_WORK_KEPT = 64 << 20   # larger work buffers are allocated by the call
 
 
 def few_scratch(K: int, N: int, experts: int, device: torch.device) -> Tensor:
@@ -612,10 +616,12 @@ def few_scratch(K: int, N: int, experts: int, device: torch.device) -> Tensor:
     return torch.zeros((nbytes,), dtype=torch.uint8, device=device)
 
 
-def _scratch_for(K: int, N: int, experts: int, dev: torch.device, stream: int) -> Tensor:
-    """The scratch of calls without one of their own: one buffer per (device, stream), since calls on a stream are
-    ordered, and one per graph capture, cleared inside the graph: no two graphs, and no graph and an eager call, ever
-    share counters. A new buffer is made when a kernel has given up a wait since (its counters may be dirty)."""
+def _scratch_for(counters: int, work: int, dev: torch.device, stream: int):
+    """(scratch address, bytes, work address) of calls without buffers of their own: one pair of buffers per (device,
+    stream), since calls on a stream are ordered, and one per graph capture, cleared inside the graph: no two graphs, and
+    no graph and an eager call, ever share counters. New ones are made when a kernel has given up a wait since
+    (its counters may be dirty). A work buffer above 64 MB is the call's own (it must live until the call has enqueued
+    its kernels: the third entry keeps it)."""
     cap = 0
     if torch.cuda.is_current_stream_capturing():
         v = C.c_uint64(0)
@@ -623,24 +629,38 @@ def _scratch_for(K: int, N: int, experts: int, dev: torch.device, stream: int) -
         cap = v.value
     key = (dev.index, stream, cap != 0)
     tag = (cap, _lib.scratch_epoch())
-    need = (-(-N // 128)) * experts * 4 + (-(-K // 128)) * 4 + 512
     have = _few_scratch.get(key)
-    if have is None or have[0] != tag or have[1] < need:
+    if have is None or have[0] != tag or have[1] < counters:
         if len(_few_scratch) > 32:
             _few_scratch.clear()
-        lib = load()
-        room = need if cap else max(need, 1 << 16)   # eager buffers serve calls of many shapes
-        slots = lib.gmlp_few_scratch_counters()
+        room = counters if cap else max(counters, 1 << 16)   # eager buffers serve calls of many shapes
+        slots = load().gmlp_few_scratch_counters()
         buf = torch.empty((slots + room,), dtype=torch.uint8, device=dev)
         buf[slots:].zero_()
-        have = _few_scratch[key] = (tag, room, buf)
-    return have[2]
+        have = _few_scratch[key] = [tag, room, buf, buf.data_ptr(), slots + room, None, 0]
+    keep = have
+    if work > have[6]:
+        own = torch.empty((work,), dtype=torch.uint8, device=dev)
+        if work > _FEW_WORK_KEPT:
+            return have[3], have[4], own.data_ptr(), own
+        have[5], have[6] = own, work
+    return have[3], have[4], (have[5].data_ptr() if have[5] is not None else None), keep
 
 
-def _w4_work(M: int, K: int, N: int, experts: int, group: int, dt: torch.dtype, dev: torch.device) -> Tensor:
-    """Work buffer of one 4-bit call (gmlp_w4_work_bytes)."""
-    return torch.empty((load().gmlp_w4_work_bytes(M, K, N, experts, group, dtype_code(dt)),), dtype=torch.uint8,
-                       device=dev)
+def _few_buffers(scratch: Tensor | None, K: int, N: int, experts: int, work: int, dev: torch.device, stream: int):
+    """Addresses of scratch and work buffer, and what has to stay alive until the call has been made."""
+    if scratch is None:
+        return _scratch_for((-(-N // 128)) * experts * 4 + (-(-K // 128)) * 4 + 512, work, dev, stream)
+    own = torch.empty((work,), dtype=torch.uint8, device=dev)
+    return scratch.data_ptr(), scratch.numel() * scratch.element_size(), own.data_ptr(), own
+
+
+def _w4_work_bytes(M: int, K: int, N: int, experts: int, group: int, dt: torch.dtype) -> int:
+    return load().gmlp_w4_work_bytes(M, K, N, experts, group, 0 if dt is torch.bfloat16 else 1)
+
+
+def _raw_stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _rows_of(x: Tensor) -> Tensor:
@@ -689,7 +709,7 @@ def linear_w4(x: Tensor, w: Int4Weight, bias: Tensor | None = None, residual: Te
     N = w[0].shape[0]
     group = _int4_group(w, (), N, K, dt, dev)
     bias, residual = _vector(bias, N, "bias"), _like(residual, (M, N), "residual")
-    y = torch.empty((M, N), dtype=dt, device=dev)
+    y = x.new_empty((M, N))
     if M == 0 or N == 0:
         return y
     ldx = K
@@ -698,14 +718,12 @@ def linear_w4(x: Tensor, w: Int4Weight, bias: Tensor | None = None, residual: Te
     else:
         x = _rows_of(x)
     with _on(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if scratch is None:
-            scratch = _scratch_for(N, N, 1, dev, stream)
-        work = _w4_work(M, K, 0, 1, group, dt, dev)
+        stream = _raw_stream(dev)
+        sc, sc_bytes, work, keep = _few_buffers(scratch, N, N, 1, nbytes := _w4_work_bytes(M, K, 0, 1, group, dt), dev,
+                                                stream)
         check(load().gmlp_w4_linear(M, N, K, group, dtype_code(dt), x.data_ptr(), ldx, w[0].data_ptr(),
-                                    w[1].data_ptr(), ptr(w[2]), ptr(bias), ptr(residual), y.data_ptr(),
-                                    work.data_ptr(), work.numel(), scratch.data_ptr(), scratch.numel() * scratch.element_size(),
-                                    (1 << 26) if ordinary_launch else 0, stream))
+                                    w[1].data_ptr(), ptr(w[2]), ptr(bias), ptr(residual), y.data_ptr(), work, nbytes,
+                                    sc, sc_bytes, (1 << 26) if ordinary_launch else 0, stream))
     return y
 
 
@@ -731,21 +749,19 @@ def decode_fwd_w4(x: Tensor, w_gate: Int4Weight, b_gate: Tensor | None, w_up: In
         raise ValueError("gate and up weights must both have zeros or both have none")
     b_gate, b_up, b_down = _vector(b_gate, N, "b_gate"), _vector(b_up, N, "b_up"), _vector(b_down, K, "b_down")
     residual = _like(residual, (M, K), "residual")
-    y = torch.empty((M, K), dtype=dt, device=dev)
+    y = x.new_empty((M, K))
     if M == 0:
         return y
     x = _rows_of(x)
-    work = _w4_work(M, K, N, 1, group, dt, dev)
     prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act, (1 << 26) if ordinary_launch else 0)
     with _on(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if scratch is None:
-            scratch = _scratch_for(K, N, 1, dev, stream)
+        stream = _raw_stream(dev)
+        sc, sc_bytes, work, keep = _few_buffers(scratch, K, N, 1, nbytes := _w4_work_bytes(M, K, N, 1, group, dt), dev,
+                                                stream)
         check(load().gmlp_decode_fwd_w4(
             C.byref(prob), group, x.data_ptr(), w_gate[0].data_ptr(), w_gate[1].data_ptr(), ptr(w_gate[2]), ptr(b_gate),
             w_up[0].data_ptr(), w_up[1].data_ptr(), ptr(w_up[2]), ptr(b_up), w_down[0].data_ptr(), w_down[1].data_ptr(),
-            ptr(w_down[2]), ptr(b_down), ptr(residual), y.data_ptr(), work.data_ptr(), work.numel(), scratch.data_ptr(),
-            scratch.numel() * scratch.element_size(), stream))
+            ptr(w_down[2]), ptr(b_down), ptr(residual), y.data_ptr(), work, nbytes, sc, sc_bytes, stream))
     return y
 
 
@@ -770,15 +786,14 @@ def moe_route(x: Tensor, w_router: Tensor, top_k: int, renormalize: bool = True)
         raise ValueError(f"{E} experts: 1 to {MOE_MAX_EXPERTS} are supported")
     if not 1 <= top_k <= min(E, MOE_MAX_TOP_K):
         raise ValueError(f"top_k={top_k}: 1 to {min(E, MOE_MAX_TOP_K)} are supported for {E} experts")
-    ids = torch.empty((M, top_k), dtype=torch.int32, device=dev)
-    weights = torch.empty((M, top_k), dtype=torch.float32, device=dev)
+    ids = x.new_empty((M, top_k), dtype=torch.int32)
+    weights = x.new_empty((M, top_k), dtype=torch.float32)
     if M == 0:
         return ids, weights
     x, w_router = _rows_of(x), _rows_of(w_router)
     with _on(dev):
         check(load().gmlp_moe_route(M, K, E, top_k, 1 if renormalize else 0, dtype_code(dt), x.data_ptr(), K,
-                                    w_router.data_ptr(), ids.data_ptr(), weights.data_ptr(),
-                                    torch.cuda.current_stream(dev).cuda_stream))
+                                    w_router.data_ptr(), ids.data_ptr(), weights.data_ptr(), _raw_stream(dev)))
     return ids, weights
 
 
@@ -819,23 +834,20 @@ def moe_decode_fwd(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Tensor, w_up
                          f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
     ids, weights, k = _moe_table(x, ids, weights, E)
     residual = _like(residual, (M, K), "residual")
-    y = torch.empty((M, K), dtype=dt, device=dev)
+    y = x.new_empty((M, K))
     if M == 0:
         return y
     if not moe_decode_supported(M, K, N, E):
         raise ValueError(f"the mixture-of-experts decode path needs K and N multiples of 64; got K={K} N={N}")
     x, w_gate, w_up, w_down = _rows_of(x), _c(w_gate), _c(w_up), _c(w_down)
     active = min(E, M * k)
-    h = torch.empty((active, M, N), dtype=dt, device=dev)
     prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act)
     with _on(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if scratch is None:
-            scratch = _scratch_for(K, N, active, dev, stream)
+        stream = _raw_stream(dev)
+        sc, sc_bytes, h, keep = _few_buffers(scratch, K, N, active, 2 * active * M * N, dev, stream)
         check(load().gmlp_moe_decode_fwd(
             C.byref(prob), E, k, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-            w_down.data_ptr(), ptr(residual), h.data_ptr(), y.data_ptr(), scratch.data_ptr(),
-            scratch.numel() * scratch.element_size(), stream))
+            w_down.data_ptr(), ptr(residual), h, y.data_ptr(), sc, sc_bytes, stream))
     return y
 
 
@@ -857,22 +869,21 @@ def moe_decode_fwd_w4(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Int4Weigh
         raise ValueError("gate and up weights must both have zeros or both have none")
     ids, weights, k = _moe_table(x, ids, weights, E)
     residual = _like(residual, (M, K), "residual")
-    y = torch.empty((M, K), dtype=dt, device=dev)
+    y = x.new_empty((M, K))
     if M == 0:
         return y
     x = _rows_of(x)
     active = min(E, M * k)
-    work = _w4_work(M, K, N, active, group, dt, dev)
     prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act)
     with _on(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if scratch is None:
-            scratch = _scratch_for(K, N, active, dev, stream)
+        stream = _raw_stream(dev)
+        sc, sc_bytes, work, keep = _few_buffers(scratch, K, N, active,
+                                                nbytes := _w4_work_bytes(M, K, N, active, group, dt), dev, stream)
         check(load().gmlp_moe_decode_fwd_w4(
             C.byref(prob), group, E, k, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate[0].data_ptr(),
             w_gate[1].data_ptr(), ptr(w_gate[2]), w_up[0].data_ptr(), w_up[1].data_ptr(), ptr(w_up[2]),
-            w_down[0].data_ptr(), w_down[1].data_ptr(), ptr(w_down[2]), ptr(residual), y.data_ptr(), work.data_ptr(),
-            work.numel(), scratch.data_ptr(), scratch.numel() * scratch.element_size(), stream))
+            w_down[0].data_ptr(), w_down[1].data_ptr(), ptr(w_down[2]), ptr(residual), y.data_ptr(), work, nbytes, sc,
+            sc_bytes, stream))
     return y
 
 
