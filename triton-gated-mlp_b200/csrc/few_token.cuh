@@ -105,7 +105,7 @@ struct Cut {
   int ctas;       // CTAs that have units (at most one per unit)
   int each, odd;  // units per CTA; the first `odd` CTAs have one more
 };
-__device__ __forceinline__ Cut make_cut(int total, int grid) {
+__host__ __device__ __forceinline__ Cut make_cut(int total, int grid) {
   Cut c;
   c.total = total;
   c.ctas = total < grid ? total : grid;
@@ -191,51 +191,48 @@ __device__ __forceinline__ void publish_segment(const float (&v)[NT][COLS], cons
   }
 }
 
+__device__ __forceinline__ float4 plus(const float4& a, const float4& b) {
+  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
 // This CTA's share of a tile whose parts are in the slots: emit(t, row, i, sums) for four tokens 4i .. 4i + 3 of a row, with
-// JOINT over both tiles at once (emit(0, row, i, gate, up)). The first part of the next item is on its way while an item
-// is finished.
+// JOINT over both tiles at once (emit(0, row, i, gate, up)).
 template <int NT, bool JOINT, int COLS_ALL, int THREADS, typename Emit>
 __device__ __forceinline__ void finish_tile(int tile_begin, int first, int last, const Split& sp, int ep_tid, Emit emit) {
   constexpr int SLOT4 = NT * COLS_ALL / 4 * 128;
   const int nq = (sp.M + 3) / 4, parts = last - first + 1, mine = blockIdx.x - first;
   const int items = (JOINT ? 1 : NT) * nq * 128;
-  const int lo = items * mine / parts, hi = items * (mine + 1) / parts;  // at most 2 * 16 * 128 * 1024
+  const int share = (items + parts - 1) / parts;
+  const int lo = share * mine, hi = lo + share < items ? lo + share : items;
   const float4* const s0 = sp.slots + static_cast<long long>(slot_of(sp.cut, first, tile_begin)) * SLOT4;
   const float4* const s1 = sp.slots + (2LL * first + 2) * SLOT4;  // the others start in the middle of the tile
-  float4 next_a = make_float4(0.f, 0.f, 0.f, 0.f), next_b = next_a;
-  int t = 0, row = 0, i = 0;
-  auto place = [&](int it) {
-    t = JOINT ? 0 : it / (nq * 128);
-    const int rest = it - t * nq * 128;
-    i = rest >> 7;
-    row = rest & 127;
-    return (t * (COLS_ALL / 4) + i) * 128 + row;
-  };
-  auto fetch = [&](int it) {
-    const int at = place(it);
-    next_a = __ldcg(s0 + at);
-    if (JOINT) next_b = __ldcg(s0 + at + COLS_ALL / 4 * 128);
-  };
-  if (lo + ep_tid < hi) fetch(lo + ep_tid);
+  const int per_t = nq * 128;
 #pragma unroll 1
   for (int it = lo + ep_tid; it < hi; it += THREADS) {
-    float4 a = next_a, b = next_b;
-    if (it + THREADS < hi) fetch(it + THREADS);
-    const float4* s = s1 + place(it);
-#pragma unroll 4
-    for (int c = 1; c < parts; ++c, s += 2 * SLOT4) {
-      const float4 q = __ldcg(s);
-      a.x += q.x;
-      a.y += q.y;
-      a.z += q.z;
-      a.w += q.w;
-      if (JOINT) {
-        const float4 r = __ldcg(s + COLS_ALL / 4 * 128);
-        b.x += r.x;
-        b.y += r.y;
-        b.z += r.z;
-        b.w += r.w;
-      }
+    const int t = (!JOINT && it >= per_t) ? 1 : 0;
+    const int rest = it - t * per_t;
+    const int i = rest >> 7, row = rest & 127;
+    const int at = (t * (COLS_ALL / 4) + i) * 128 + row;
+    constexpr int UP = COLS_ALL / 4 * 128;  // from a gate value to its up value
+    float4 a = __ldcg(s0 + at), b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (JOINT) b = __ldcg(s0 + at + UP);
+    const float4* s = s1 + at;
+    // up to eight parts (four with two tiles) on their way at a time, added in CTA order
+    constexpr int BATCH = JOINT ? 4 : 8;
+#pragma unroll 1
+    for (int c = 1; c < parts; c += BATCH, s += 2 * SLOT4 * BATCH) {
+      float4 q[BATCH], r[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (c + k < parts) {
+          q[k] = __ldcg(s + 2 * SLOT4 * k);
+          if (JOINT) r[k] = __ldcg(s + 2 * SLOT4 * k + UP);
+        }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (c + k < parts) {
+          a = plus(a, q[k]);
+          if (JOINT) b = plus(b, r[k]);
+        }
     }
     emit(t, row, i, a, b);
   }
@@ -341,14 +338,22 @@ template <int THREADS, typename EmitTile>
 __device__ __forceinline__ void end_units(const Pending& pending, int per_tile, const Split& sp, int ep_tid,
                                           EmitTile emit_tile) {
   if (pending.n == 0) return;
+  int first[2], last[2];  // CTAs that have parts of the tile
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const int begin = pending.tile[p < pending.n ? p : 0] * per_tile;
+    // this CTA is the last one of a tile that it met first, and the first of one that it ends in the middle of
+    const bool tail = begin < cut_start(sp.cut, blockIdx.x);
+    const bool ends = cut_start(sp.cut, blockIdx.x + 1) >= begin + per_tile;
+    first[p] = tail ? cut_owner(sp.cut, begin) : static_cast<int>(blockIdx.x);
+    last[p] = ends ? static_cast<int>(blockIdx.x) : cut_owner(sp.cut, begin + per_tile - 1);
+  }
   // thread 0 waits for the parts of the first tile, thread 32 for those of the second
   const int k = ep_tid >> 5;
   const bool waiter = (ep_tid & 31) == 0 && k < pending.n;
-  int my_tile = 0, my_parts = 0;
+  const int my_tile = k == 0 ? pending.tile[0] : pending.tile[1];
+  const int my_parts = k == 0 ? last[0] - first[0] + 1 : last[1] - first[1] + 1;
   if (waiter) {
-    my_tile = k == 0 ? pending.tile[0] : pending.tile[1];
-    const int begin = my_tile * per_tile;
-    my_parts = cut_owner(sp.cut, begin + per_tile - 1) - cut_owner(sp.cut, begin) + 1;
     const long long t0 = clock64();
     while ((ld_acquire(sp.counters + my_tile) & 0xffff) != my_parts) {
       if (*sp.abortp != 0 || clock64() - t0 > WAIT_LIMIT_CYCLES) {
@@ -362,8 +367,7 @@ __device__ __forceinline__ void end_units(const Pending& pending, int per_tile, 
 #pragma unroll 1
   for (int p = 0; p < pending.n; ++p) {
     const int tile = p == 0 ? pending.tile[0] : pending.tile[1];
-    const int begin = tile * per_tile;
-    emit_tile(tile, begin, cut_owner(sp.cut, begin), cut_owner(sp.cut, begin + per_tile - 1));
+    emit_tile(tile, tile * per_tile, p == 0 ? first[0] : first[1], p == 0 ? last[0] : last[1]);
   }
   // the last CTA to have seen all parts leaves the counter ready for the next call
   if (waiter && (atomicAdd(sp.counters + my_tile, 0x10000) >> 16) == my_parts - 1) sp.counters[my_tile] = 0;

@@ -231,6 +231,7 @@ struct W4Args {
   int act;
   int wide;   // scales and zeros go by TMA: rows are a multiple of 16 and the arrays 16-byte aligned
   int early;  // the weights may be streamed before the preceding kernel has finished
+  Cut cut;    // a dense call's; on experts the kernel makes it from the routing table
   MoeTable moe;
 };
 
@@ -428,30 +429,21 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    abort_flag = 0;
-    for (int s = 0; s < NW; ++s) {
-      mbar_init(wfull + 8 * s, 1);
-      mbar_init(wempty + 8 * s, 8);
-    }
-    for (int s = 0; s < NX; ++s) {
-      // the TMA bytes, the copying lanes of warp 3, a converting warp per token
-      mbar_init(xfull + 8 * s, 1 + (args.wide ? 0 : 32) + (FUSED ? args.M : 0));
-      mbar_init(xempty + 8 * s, 1 + C::EPI / 32);
-      mbar_init(sfull + 8 * s, 1);
-    }
-    for (int b = 0; b < NA; ++b) {
-      mbar_init(afull + 8 * b, 8);
-      mbar_init(aempty + 8 * b, 1);
-    }
-    for (int b = 0; b < NC; ++b) {
-      mbar_init(cfull + 8 * b, 1);
-      mbar_init(cempty + 8 * b, C::EPI / 32);
-    }
-    mbar_init(drain_bar, 1);
+  // one barrier a thread
+  constexpr int BARS = 2 * (NW + NX + NA + NC) + NX + 1;
+  if (threadIdx.x < BARS) {
+    const uint32_t bar = wfull + 8 * threadIdx.x;
+    int count = 1;  // wfull (TMA), aempty and cfull (MMA), sfull (warp 3), drain
+    if (bar >= wempty && bar < xfull) count = 8;                               // expanding warps
+    if (bar >= xfull && bar < xempty) count = 1 + (args.wide ? 0 : 32) + (FUSED ? args.M : 0);  // TMA, copying lanes, tokens
+    if (bar >= xempty && bar < afull) count = 1 + C::EPI / 32;                 // MMA, accumulating warps
+    if (bar >= afull && bar < aempty) count = 8;
+    if (bar >= cempty && bar < sfull) count = C::EPI / 32;
+    mbar_init(bar, count);
     mbar_fence_init();
     fence_proxy_async_smem();
   }
+  if (threadIdx.x == 64) abort_flag = 0;
   if (warp == 2 && lane < 7) tma_prefetch_desc(&maps.w0 + lane);
   if (warp == 1) {
     tmem_alloc(smem_u32(&tmem_base_holder), 512);
@@ -471,7 +463,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   // Units: DUAL: tile = (expert, row tile), kbt units each. Else: tile = row tile, units = (expert, kb).
   const int row_tiles = (args.rows + ROWS - 1) / ROWS;
   const int per_tile = DUAL ? args.kbt : moe.n * args.kbt;
-  const Cut cut = make_cut(per_tile * (DUAL ? moe.n * row_tiles : row_tiles), gridDim.x);
+  const Cut cut = is_moe ? make_cut(per_tile * (DUAL ? moe.n * row_tiles : row_tiles), gridDim.x) : args.cut;
   const int u_begin = cut_start(cut, blockIdx.x), u_end = cut_start(cut, blockIdx.x + 1);
   const int units = u_end - u_begin;
 
@@ -480,12 +472,12 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     if (units == 0) return;
     const int tile = u_begin / per_tile, r = u_begin - tile * per_tile;
     if (DUAL) {
-      w.a = tile / row_tiles;
+      w.a = is_moe ? tile / row_tiles : 0;
       w.row0 = (tile - w.a * row_tiles) * ROWS;
       w.kb = r;
     } else {
       w.row0 = tile * ROWS;
-      w.a = r / args.kbt;
+      w.a = is_moe ? r / args.kbt : 0;
       w.kb = r - w.a * args.kbt;
     }
   };
