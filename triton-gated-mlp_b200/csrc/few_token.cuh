@@ -49,20 +49,17 @@ __device__ __forceinline__ void moe_collect(const MoeTable& t, int M, MoeShared&
     __syncthreads();
     return;
   }
+  uint32_t* const top = reinterpret_cast<uint32_t*>(s.wmax);  // magnitudes as integers: the same order, NaN on top
   for (int i = tid; i < MOE_MAX_EXPERTS / 32; i += blockDim.x) s.seen[i] = 0u;
+  for (int i = tid; i < FEW_MAX_TOKENS; i += blockDim.x) top[i] = 0u;
   __syncthreads();
-  for (int i = tid; i < M * t.top_k; i += blockDim.x) {
+  for (int i = tid; i < M * t.top_k; i += blockDim.x) {  // all entries at once: a token's own would be a chain of loads
     const int e = t.ids[i];
-    if (static_cast<unsigned>(e) < static_cast<unsigned>(t.experts)) atomicOr(&s.seen[e >> 5], 1u << (e & 31));
-  }
-  for (int m = tid; m < M; m += blockDim.x) {
-    float w = 0.f;
-    for (int j = 0; j < t.top_k; ++j) {
-      if (static_cast<unsigned>(t.ids[m * t.top_k + j]) >= static_cast<unsigned>(t.experts)) continue;
-      const float a = fabsf(t.weights[m * t.top_k + j]);
-      w = (a > w || a != a) ? a : w;  // a NaN stays: it belongs in the token's output
+    const uint32_t w = __float_as_uint(t.weights[i]) & 0x7fffffffu;
+    if (static_cast<unsigned>(e) < static_cast<unsigned>(t.experts)) {
+      atomicOr(&s.seen[e >> 5], 1u << (e & 31));
+      atomicMax(&top[i / t.top_k], w);  // a NaN belongs in the token's output
     }
-    s.wmax[m] = w;
   }
   __syncthreads();
   if (tid < 32) {
@@ -87,11 +84,14 @@ __device__ __forceinline__ void moe_factors(const MoeTable& t, int M, int e, int
   if (ep_tid >= M) return;
   float w = 0.f;
   int hit = 0;
-  for (int j = 0; j < t.top_k; ++j)
+#pragma unroll 8
+  for (int j = 0; j < t.top_k; ++j) {
+    const float x = t.weights[ep_tid * t.top_k + j];
     if (t.ids[ep_tid * t.top_k + j] == e) {
-      w += t.weights[ep_tid * t.top_k + j];  // the same expert twice in a token adds
+      w += x;  // the same expert twice in a token adds
       hit = 1;
     }
+  }
   const float top = s.wmax[ep_tid];
   s.f[ep_tid] = top == 0.f ? 0.f : w / top;
   s.hit[ep_tid] = hit;
@@ -102,23 +102,32 @@ __device__ __forceinline__ void moe_factors(const MoeTable& t, int M, int e, int
 // instructions, and a single warp at the start of a kernel takes a microsecond for four of them. ----
 struct Cut {
   int total;      // units of the launch
-  int ctas;       // CTAs that have units (at most one per unit)
-  int each, odd;  // units per CTA; the first `odd` CTAs have one more
+  int grain;      // units that are not cut apart: 1, or a whole row tile where that is short
+  int ctas;       // CTAs that have units (at most one per grain)
+  int each, odd;  // grains per CTA; the first `odd` CTAs have one more
 };
-__host__ __device__ __forceinline__ Cut make_cut(int total, int grid) {
+__host__ __device__ __forceinline__ Cut make_cut(int total, int grain, int grid) {
   Cut c;
+  const int grains = grain == 1 ? total : total / grain;  // (a tile is the grain: total is a multiple)
   c.total = total;
-  c.ctas = total < grid ? total : grid;
-  c.each = c.ctas > 0 ? total / c.ctas : 0;
-  c.odd = total - c.each * c.ctas;
+  c.grain = grain;
+  c.ctas = grains < grid ? grains : grid;
+  c.each = c.ctas > 0 ? grains / c.ctas : 0;
+  c.odd = grains - c.each * c.ctas;
   return c;
 }
 __device__ __forceinline__ int cut_start(const Cut& c, int cta) {
-  return cta >= c.ctas ? c.total : cta * c.each + (cta < c.odd ? cta : c.odd);
+  return cta >= c.ctas ? c.total : (cta * c.each + (cta < c.odd ? cta : c.odd)) * c.grain;
 }
-__device__ __forceinline__ int cut_owner(const Cut& c, int unit) {  // the CTA that has the unit
+__device__ __forceinline__ int cut_owner(const Cut& c, int unit) {  // the CTA that has the unit; only where tiles are cut
   const int big = c.odd * (c.each + 1);
   return unit < big ? unit / (c.each + 1) : c.odd + (unit - big) / c.each;
+}
+// Joining the parts of a tile takes some 6,000 clocks after its last unit (publish, see the others' parts, fetch them). Where
+// one CTA streams the whole tile in less, tiles stay whole.
+constexpr int JOIN_CLOCKS = 6000;
+__host__ __device__ __forceinline__ int cut_grain(int per_tile, int unit_clocks) {
+  return per_tile > 0 && per_tile * unit_clocks <= JOIN_CLOCKS ? per_tile : 1;
 }
 
 struct Segment {
@@ -195,8 +204,8 @@ __device__ __forceinline__ float4 plus(const float4& a, const float4& b) {
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
 // This CTA's share of a tile whose parts are in the slots: emit(t, row, i, sums) for four tokens 4i .. 4i + 3 of a row, with
-// JOINT over both tiles at once (emit(0, row, i, gate, up)).
-template <int NT, bool JOINT, int COLS_ALL, int THREADS, typename Emit>
+// JOINT over both tiles at once (emit(0, row, i, gate, up)). ITEMS of a thread are worked on together.
+template <int NT, bool JOINT, int COLS_ALL, int THREADS, int ITEMS, typename Emit>
 __device__ __forceinline__ void finish_tile(int tile_begin, int first, int last, const Split& sp, int ep_tid, Emit emit) {
   constexpr int SLOT4 = NT * COLS_ALL / 4 * 128;
   const int nq = (sp.M + 3) / 4, parts = last - first + 1, mine = blockIdx.x - first;
@@ -206,35 +215,50 @@ __device__ __forceinline__ void finish_tile(int tile_begin, int first, int last,
   const float4* const s0 = sp.slots + static_cast<long long>(slot_of(sp.cut, first, tile_begin)) * SLOT4;
   const float4* const s1 = sp.slots + (2LL * first + 2) * SLOT4;  // the others start in the middle of the tile
   const int per_t = nq * 128;
+  constexpr int UP = COLS_ALL / 4 * 128;  // from a gate value to its up value
 #pragma unroll 1
-  for (int it = lo + ep_tid; it < hi; it += THREADS) {
-    const int t = (!JOINT && it >= per_t) ? 1 : 0;
-    const int rest = it - t * per_t;
-    const int i = rest >> 7, row = rest & 127;
-    const int at = (t * (COLS_ALL / 4) + i) * 128 + row;
-    constexpr int UP = COLS_ALL / 4 * 128;  // from a gate value to its up value
-    float4 a = __ldcg(s0 + at), b = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (JOINT) b = __ldcg(s0 + at + UP);
-    const float4* s = s1 + at;
-    // up to eight parts (four with two tiles) on their way at a time, added in CTA order
-    constexpr int BATCH = JOINT ? 4 : 8;
+  for (int it0 = lo + ep_tid; it0 < hi; it0 += THREADS * ITEMS) {
+    float4 a[ITEMS], b[ITEMS];
+    int at[ITEMS];
+#pragma unroll
+    for (int n = 0; n < ITEMS; ++n) {  // the items' loads go out together
+      const int it = it0 + n * THREADS;
+      const int t = (!JOINT && it >= per_t) ? 1 : 0;
+      at[n] = t * (COLS_ALL / 4 * 128) + (it - t * per_t);
+      if (it < hi) {
+        a[n] = __ldcg(s0 + at[n]);
+        if (JOINT) b[n] = __ldcg(s0 + at[n] + UP);
+      }
+    }
+    const float4* s = s1;
+    // up to BATCH parts of an item on their way at a time, added in CTA order
+    constexpr int BATCH = ITEMS > 1 ? 1 : (JOINT ? 4 : 8);
 #pragma unroll 1
     for (int c = 1; c < parts; c += BATCH, s += 2 * SLOT4 * BATCH) {
-      float4 q[BATCH], r[BATCH];
+      float4 q[ITEMS][BATCH], r[ITEMS][BATCH];
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k)
-        if (c + k < parts) {
-          q[k] = __ldcg(s + 2 * SLOT4 * k);
-          if (JOINT) r[k] = __ldcg(s + 2 * SLOT4 * k + UP);
-        }
+      for (int n = 0; n < ITEMS; ++n)
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k)
-        if (c + k < parts) {
-          a = plus(a, q[k]);
-          if (JOINT) b = plus(b, r[k]);
-        }
+        for (int k = 0; k < BATCH; ++k)
+          if (it0 + n * THREADS < hi && c + k < parts) {
+            q[n][k] = __ldcg(s + 2 * SLOT4 * k + at[n]);
+            if (JOINT) r[n][k] = __ldcg(s + 2 * SLOT4 * k + at[n] + UP);
+          }
+#pragma unroll
+      for (int n = 0; n < ITEMS; ++n)
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+          if (it0 + n * THREADS < hi && c + k < parts) {
+            a[n] = plus(a[n], q[n][k]);
+            if (JOINT) b[n] = plus(b[n], r[n][k]);
+          }
     }
-    emit(t, row, i, a, b);
+#pragma unroll
+    for (int n = 0; n < ITEMS; ++n) {
+      const int it = it0 + n * THREADS;
+      const int t = (!JOINT && it >= per_t) ? 1 : 0;
+      if (it < hi) emit(t, (it - t * per_t) & 127, (it - t * per_t) >> 7, a[n], b[n]);
+    }
   }
 }
 

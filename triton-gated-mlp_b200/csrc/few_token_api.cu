@@ -142,6 +142,13 @@ static int launch_moe(int mpad, int dtype, const DeviceInfo* dev, Args... args) 
             : launch_moe_t<64, DUAL, __half>(dev, dtype, args...);
 }
 
+template <typename T>
+static int launch_route(const RouteArgs& a, unsigned grid, int cluster, cudaStream_t st) {
+  if (a.E <= 32) return launch_few(moe_route_kernel<T, 1>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
+  if (a.E <= 128) return launch_few(moe_route_kernel<T, 4>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
+  return launch_few(moe_route_kernel<T, 16>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
+}
+
 static int check_few(const gmlp_problem_t* p, const char* what) {
   int rc;
   if ((rc = check_problem(p))) return rc;
@@ -416,13 +423,12 @@ int gmlp_moe_route(int64_t M, int64_t K, int32_t experts, int32_t top_k, int32_t
   a.renormalize = renormalize ? 1 : 0;
   a.ids = ids;
   a.weights = weights;
-  // one warp per expert at a time; up to eight blocks a token
+  // a warp takes two experts at a time; up to eight blocks a token
   int cluster = 1;
-  while (cluster < 8 && cluster * (ROUTE_THREADS / 32) < experts) cluster *= 2;
+  while (cluster < 8 && cluster * 2 * (ROUTE_THREADS / 32) < experts) cluster *= 2;
   const unsigned grid = static_cast<unsigned>(M * cluster);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == GMLP_BF16 ? launch_few(moe_route_kernel<__nv_bfloat16>, grid, ROUTE_THREADS, 0, true, st, a, cluster)
-                            : launch_few(moe_route_kernel<__half>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
+  return dtype == GMLP_BF16 ? launch_route<__nv_bfloat16>(a, grid, cluster, st) : launch_route<__half>(a, grid, cluster, st);
 }
 
 }  // extern "C"

@@ -132,7 +132,7 @@ int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
   a.early = c.early ? 1 : 0;
   a.moe = c.moe;
   const int grid = static_cast<int>(c.max_units < dev->sm_count ? c.max_units : dev->sm_count);
-  if (c.moe.ids == nullptr) a.cut = make_cut(static_cast<int>(c.max_units), grid);
+  if (c.moe.ids == nullptr) a.cut = make_cut(static_cast<int>(c.max_units), cut_grain(a.kbt, W4_UNIT_CLOCKS), grid);
   auto kfn = w4_stream_kernel<MT, DUAL, T, GSHIFT, FUSED>;
   static std::atomic<uint64_t> attr_done{0};
   if ((rc = ensure_smem_attr(kfn, Conf::SMEM, attr_done))) return rc;

@@ -71,22 +71,15 @@ moe_stream_kernel(const __grid_constant__ MoeMaps maps, const MoeArgs args) {
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    abort_flag = 0;
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
-    }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), 4);
-    }
-    mbar_init(drain_bar, 1);
+  constexpr int BARS = 2 * STAGES + 5;  // one a thread
+  if (threadIdx.x < BARS) {
+    const uint32_t bar = bar_base + 8 * threadIdx.x;
+    mbar_init(bar, bar >= tempty_bar(0) && bar < drain_bar ? 4 : 1);
     mbar_fence_init();
     fence_proxy_async_smem();
-    tma_prefetch_desc(&maps.w0);
-    tma_prefetch_desc(&maps.x);
   }
+  if (threadIdx.x == 64) abort_flag = 0;
+  if (warp == 3 && lane < 3) tma_prefetch_desc(&maps.w0 + lane);
   if (warp == 1) {
     tmem_alloc(smem_u32(&tmem_base_holder), TMEM_COLS);
     tmem_relinquish();
@@ -103,7 +96,8 @@ moe_stream_kernel(const __grid_constant__ MoeMaps maps, const MoeArgs args) {
 
   const int row_tiles = (args.rows + 127) / 128;
   const int per_tile = DUAL ? args.kbt : moe.n * args.kbt;
-  const Cut cut = make_cut(per_tile * (DUAL ? moe.n * row_tiles : row_tiles), gridDim.x);
+  const Cut cut = make_cut(per_tile * (DUAL ? moe.n * row_tiles : row_tiles), cut_grain(per_tile, (DUAL ? 2 : 1) * 300),
+                           gridDim.x);  // 300 clocks: 16 KB into one SM while the others are idle
   const int u_begin = cut_start(cut, blockIdx.x), u_end = cut_start(cut, blockIdx.x + 1);
 
   if (warp == 0) {
@@ -254,12 +248,12 @@ moe_stream_kernel(const __grid_constant__ MoeMaps maps, const MoeArgs args) {
         moe_factors(args.moe, args.M, moe.list[a], ep_tid, moe);
         named_bar_sync(1, 128);
         T* const oa = out + static_cast<long long>(a) * args.M * ld;
-        finish_tile<NACC, true, MPAD, 128>(begin, first, last, sp, ep_tid,
+        finish_tile<NACC, true, MPAD, 128, (MPAD > 16 ? 4 : 1)>(begin, first, last, sp, ep_tid,
                                            [&](int, int r, int i, const float4& gate, const float4& up) {
           if (row0 + r < args.rows) emit_hidden(oa + row0 + r, ld, args.M, i, gate, up, nullptr, 0.f, 0.f, args.act, &moe);
         });
       } else {
-        finish_tile<NACC, false, MPAD, 128>(begin, first, last, sp, ep_tid,
+        finish_tile<NACC, false, MPAD, 128, (MPAD > 16 ? 4 : 1)>(begin, first, last, sp, ep_tid,
                                             [&](int, int r, int i, const float4& v, const float4&) {
           const int wr = tile * 128 + r;
           if (wr < args.rows) emit_product(out + wr, res ? res + wr : nullptr, ld, args.M, i, v, nullptr, 0.f, &moe);
@@ -311,11 +305,11 @@ moe_stream_kernel(const __grid_constant__ MoeMaps maps, const MoeArgs args) {
 
 // ---- router ----
 // logits l[t][e] = x_t . Wr_e; p = softmax(l); the top_k largest (equal ones: lowest index first; NaN ranks lowest) with
-// weights p, or p divided by their sum. A cluster of C blocks per token: each takes E / C experts, a warp per expert
-// and pass, products exact in fp32, eight of them summed in fp32 and added to an fp64 sum, so that the order of the
+// weights p, or p divided by their sum. A cluster of C blocks per token: each warp takes two experts
+// a pass, products exact in fp32, eight of them summed in fp32 and added to an fp64 sum, so that the order of the
 // logits (a choice next to a border) is that of the exact sums but for a relative 1e-7. The logits go to the first
 // block's shared memory (distributed shared memory), whose first warp selects. Latency-bound: C spreads the 2 E K bytes
-// of a token over SMs, since one SM draws about 100 GB/s per resident warp group.
+// of a token over SMs.
 constexpr int ROUTE_THREADS = 256;
 struct RouteArgs {
   const void* x;
@@ -325,49 +319,64 @@ struct RouteArgs {
   int* ids;
   float* weights;
 };
-__device__ __forceinline__ unsigned long long sort_key(double v) {
-  if (v != v) return 1ull;  // NaN: above a removed entry (0), below -inf
-  const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
-  return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+// Order of logits as an integer whose low 9 bits are the index, larger for lower indices: one maximum finds the largest
+// logit and, among equal ones (equal in 43 of the 52 fraction bits), the lowest index. NaN ranks below -inf.
+__device__ __forceinline__ unsigned long long sort_key(double v, int e) {
+  unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
+  b = (b >> 63) ? ~b : b | 0x8000000000000000ull;
+  if (v != v) b = 0x0008000000000000ull;  // below the key of -inf, above that of a removed entry (0)
+  return (b & ~511ull) | static_cast<unsigned long long>(511 - e);
 }
-template <typename T>
+// PER: experts per lane of the selecting warp.
+template <typename T, int PER>
 __global__ void __launch_bounds__(ROUTE_THREADS)
 moe_route_kernel(const RouteArgs args) {
-  __shared__ double logits[MOE_MAX_EXPERTS];
+  __shared__ double logits[32 * PER];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t rank, size;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
-  const long long token = blockIdx.x / size;
+  const unsigned token = blockIdx.x / size;
   pdl_launch_dependents();
   cluster_sync_all();  // the first block's shared memory is written below: it has to be there
   pdl_wait();
   const T* const x = static_cast<const T*>(args.x) + token * args.ldx;
-  const int e0 = static_cast<int>(static_cast<long long>(args.E) * rank / size);
-  const int e1 = static_cast<int>(static_cast<long long>(args.E) * (rank + 1) / size);
   const uint32_t dst0 = mapa_shared(smem_u32(logits), 0);
-  for (int e = e0 + warp; e < e1; e += ROUTE_THREADS / 32) {
-    const T* const w = static_cast<const T*>(args.w) + static_cast<long long>(e) * args.K;
-    double sum = 0.0;
-#pragma unroll 8
+  // experts warp-major over the cluster, two at a time: they share the loads of x
+  const int warps = size * (ROUTE_THREADS / 32);
+  for (int e = rank * (ROUTE_THREADS / 32) + warp; e < args.E; e += 2 * warps) {
+    const bool two = e + warps < args.E;
+    const T* const w0 = static_cast<const T*>(args.w) + static_cast<long long>(e) * args.K;
+    const T* const w1 = two ? w0 + static_cast<long long>(warps) * args.K : w0;
+    double s0 = 0.0, s1 = 0.0;
+#pragma unroll 4
     for (int k = lane * 8; k < args.K; k += 256) {
-      float a[8], b[8];
+      float a[8], b[8], c[8];
       load8(x + k, a);
-      load8(w + k, b);
-      float s = a[0] * b[0];
+      load8(w0 + k, b);
+      load8(w1 + k, c);
+      float p = a[0] * b[0], q = a[0] * c[0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) s = fmaf(a[i], b[i], s);
-      sum += static_cast<double>(s);
+      for (int i = 1; i < 8; ++i) {
+        p = fmaf(a[i], b[i], p);
+        q = fmaf(a[i], c[i], q);
+      }
+      s0 += static_cast<double>(p);
+      s1 += static_cast<double>(q);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0)
-      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst0 + 8u * e), "d"(sum) : "memory");
+    for (int o = 16; o > 0; o >>= 1) {
+      s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+    }
+    if (lane == 0) {
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst0 + 8u * e), "d"(s0) : "memory");
+      if (two) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst0 + 8u * (e + warps)), "d"(s1) : "memory");
+    }
   }
   __syncwarp();
   cluster_sync_all();
   if (rank != 0 || warp != 0) return;
-  constexpr int PER = MOE_MAX_EXPERTS / 32;
   unsigned long long key[PER];
   float ex[PER];
   double top = -INFINITY;
@@ -375,7 +384,7 @@ moe_route_kernel(const RouteArgs args) {
   for (int i = 0; i < PER; ++i) {
     const int e = i * 32 + lane;
     const double l = e < args.E ? logits[e] : 0.0;
-    key[i] = e < args.E ? sort_key(l) : 0ull;
+    key[i] = e < args.E ? sort_key(l, e) : 0ull;
     if (e < args.E && !(l <= top)) top = l;  // a NaN becomes the maximum and makes every weight of the token NaN
   }
 #pragma unroll
@@ -395,31 +404,26 @@ moe_route_kernel(const RouteArgs args) {
   float mine = 0.f, chosen = 0.f;  // lane j keeps choice j
   int id = 0;
   for (int j = 0; j < args.top_k; ++j) {
-    unsigned long long best = 0ull;
-    int at = 0;
+    unsigned long long best = key[0];
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (key[i] > best) {  // ascending index inside a lane: the first of equals stays
-        best = key[i];
-        at = i;
-      }
-    const uint32_t hi = static_cast<uint32_t>(best >> 32), lo = static_cast<uint32_t>(best);
+    for (int i = 1; i < PER; ++i) best = key[i] > best ? key[i] : best;
+    const uint32_t hi = static_cast<uint32_t>(best >> 32);
     const uint32_t mhi = __reduce_max_sync(0xffffffffu, hi);
-    const uint32_t mlo = __reduce_max_sync(0xffffffffu, hi == mhi ? lo : 0u);
-    const uint32_t e = __reduce_min_sync(
-        0xffffffffu, (hi == mhi && lo == mlo) ? static_cast<uint32_t>(at * 32 + lane) : 0xffffffffu);
+    const uint32_t mlo = __reduce_max_sync(0xffffffffu, hi == mhi ? static_cast<uint32_t>(best) : 0u);
+    const unsigned long long win = (static_cast<unsigned long long>(mhi) << 32) | mlo;
+    const int e = 511 - static_cast<int>(mlo & 511u);
     float w = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (static_cast<uint32_t>(i * 32 + lane) == e) {
+      if (key[i] == win) {  // no two keys are equal: the index is in them
         w = ex[i];
         key[i] = 0ull;
       }
-    w = __shfl_sync(0xffffffffu, w, e & 31u);
+    w = __shfl_sync(0xffffffffu, w, e & 31);
     chosen += w;
     if (lane == j) {
       mine = w;
-      id = static_cast<int>(e);
+      id = e;
     }
   }
   if (lane < args.top_k) {

@@ -53,6 +53,7 @@ namespace gmlp {
 constexpr int W4_TILE_BYTES = 16384;  // 128 rows x 128 bytes: 256 columns
 constexpr int W4_UNIT_COLS = 256;
 constexpr int W4_HALF_COLS = 128;
+constexpr int W4_UNIT_CLOCKS = 1400;  // of one CTA, alone or not
 
 // Terms per activation.
 template <typename T>
@@ -463,7 +464,9 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   // Units: DUAL: tile = (expert, row tile), kbt units each. Else: tile = row tile, units = (expert, kb).
   const int row_tiles = (args.rows + ROWS - 1) / ROWS;
   const int per_tile = DUAL ? args.kbt : moe.n * args.kbt;
-  const Cut cut = is_moe ? make_cut(per_tile * (DUAL ? moe.n * row_tiles : row_tiles), gridDim.x) : args.cut;
+  const Cut cut = is_moe ? make_cut(per_tile * (DUAL ? moe.n * row_tiles : row_tiles),
+                                           cut_grain(per_tile, W4_UNIT_CLOCKS), gridDim.x)
+                                : args.cut;
   const int u_begin = cut_start(cut, blockIdx.x), u_end = cut_start(cut, blockIdx.x + 1);
   const int units = u_end - u_begin;
 
@@ -884,7 +887,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
           named_bar_sync(1, EPI);
         }
         T* const oa = out + static_cast<long long>(a) * args.M * ld;
-        finish_tile<2, true, MT, EPI>(begin, first, last, sp, ep_tid,
+        finish_tile<2, true, MT, EPI, 1>(begin, first, last, sp, ep_tid,
                                       [&](int, int r, int i, const float4& gate, const float4& up) {
           const int wr = row0 + r;
           if (wr < args.rows)
@@ -893,7 +896,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
         });
       } else {
         const T* const res = static_cast<const T*>(args.residual);
-        finish_tile<2, false, MT, EPI>(begin, first, last, sp, ep_tid,
+        finish_tile<2, false, MT, EPI, 1>(begin, first, last, sp, ep_tid,
                                        [&](int t, int r, int i, const float4& v, const float4&) {
           const int wr = tile * ROWS + t * 128 + r;
           if (wr < args.rows)
