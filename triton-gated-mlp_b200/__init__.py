@@ -8,8 +8,9 @@ for `from triton_gated_mlp.gated_mlp import FusedGatedMLP`.
 """
 from . import _lib, build, host_pipeline, parallel  # noqa: F401
 from .gated_mlp import FusedGatedMLP, FusedGatedMLPFunction, mlp_hidden_states_bwd, mlp_hidden_states_fwd  # noqa: F401
+from .moe import FusedMoEGatedMLP  # noqa: F401
 
 __all__ = [
-    "FusedGatedMLP", "FusedGatedMLPFunction", "mlp_hidden_states_fwd", "mlp_hidden_states_bwd",
+    "FusedGatedMLP", "FusedGatedMLPFunction", "FusedMoEGatedMLP", "mlp_hidden_states_fwd", "mlp_hidden_states_bwd",
     "parallel", "build", "host_pipeline",
 ]

@@ -54,8 +54,8 @@ __device__ __forceinline__ void moe_collect(const MoeTable& t, int M, MoeShared&
   for (int i = tid; i < FEW_MAX_TOKENS; i += blockDim.x) top[i] = 0u;
   __syncthreads();
   for (int i = tid; i < M * t.top_k; i += blockDim.x) {  // all entries at once: a token's own would be a chain of loads
-    const int e = t.ids[i];
-    const uint32_t w = __float_as_uint(t.weights[i]) & 0x7fffffffu;
+    const int e = __ldcg(t.ids + i);  // (past L1: the kernel may have started before this SM saw the table last)
+    const uint32_t w = __float_as_uint(__ldcg(t.weights + i)) & 0x7fffffffu;
     if (static_cast<unsigned>(e) < static_cast<unsigned>(t.experts)) {
       atomicOr(&s.seen[e >> 5], 1u << (e & 31));
       atomicMax(&top[i / t.top_k], w);  // a NaN belongs in the token's output
@@ -86,8 +86,8 @@ __device__ __forceinline__ void moe_factors(const MoeTable& t, int M, int e, int
   int hit = 0;
 #pragma unroll 8
   for (int j = 0; j < t.top_k; ++j) {
-    const float x = t.weights[ep_tid * t.top_k + j];
-    if (t.ids[ep_tid * t.top_k + j] == e) {
+    const float x = __ldcg(t.weights + ep_tid * t.top_k + j);
+    if (__ldcg(t.ids + ep_tid * t.top_k + j) == e) {
       w += x;  // the same expert twice in a token adds
       hit = 1;
     }

@@ -240,7 +240,7 @@ class FusedGatedMLP(nn.Module):
     are taken in tf32 (tcgen05.mma.kind::tf32, 10-bit mantissa, fp32 accumulation; the
     tolerance class of the reference's GPU tests, atol 1e-3) through the K-major kernels,
     with transposed copies where the backward pass needs them: a compatibility path, not
-    a fast one (no decode kernels, no input norm, no 8-bit weights). A CPU tensor raises
+    a fast one (no decode kernels, no input norm, no 8-bit or 4-bit weights). A CPU tensor raises
     GmlpError.
 
     Extra keyword-only arguments (all default to the single-GPU reference behaviour):
@@ -327,6 +327,7 @@ class FusedGatedMLP(nn.Module):
         self.input_norm_eps = 1e-6
         self._folded = None
         self._fp8 = None
+        self._w4 = None
         self._decode_weight_versions = None
 
     def attach_input_norm(self, weight: Tensor, eps: float = 1e-6) -> None:
@@ -345,21 +346,32 @@ class FusedGatedMLP(nn.Module):
         self.input_norm_eps = float(eps)
         self._folded = None
 
-    def quantize_decode_weights(self, enable: bool = True) -> None:
-        """Prepare (or drop) e4m3 copies of the three weight matrices, one scale per weight row, for the
-        decode path: inference with at most 64 tokens then streams half the weight bytes (activations
-        are quantised per token on the fly; everything else stays 16-bit). Call again after the weights
-        change. Needs hidden and intermediate sizes that are multiples of 128; not combined with an
-        attached input norm or tensor parallelism."""
+    def quantize_decode_weights(self, enable: bool = True, bits: int = 8, group_size: int = 128) -> None:
+        """Prepare (or drop) narrow copies of the three weight matrices for the decode path (inference with at most
+        64 tokens). bits=8: e4m3 with one scale per weight row, half the weight bytes (activations are quantised per
+        token on the fly); needs hidden and intermediate sizes that are multiples of 128. bits=4: nibbles with one
+        scale and zero point per `group_size` (32, 64 or 128) columns, about a quarter of the bytes (activations keep
+        their 16-bit accuracy); needs hidden and intermediate sizes that are multiples of the group size. Everything
+        else stays 16-bit. Call again after the weights change. Not combined with an attached input norm or tensor
+        parallelism."""
+        if bits not in (4, 8):
+            raise NotImplementedError(f"{bits}-bit decode weights: 4 and 8 bits are supported")
         if not enable:
-            self._fp8 = None
+            self._fp8 = self._w4 = None
             return
         if self.input_norm_weight is not None or self.parallel_mode == "tp":
-            raise NotImplementedError("8-bit decode weights are not combined with an input norm or tensor parallelism")
-        if self.hidden_size % 128 or self.intermediate_size % 128:
-            raise ValueError("8-bit decode weights need hidden_size and intermediate_size multiples of 128")
-        q = kernels.quantize_weight_rows_e4m3
-        self._fp8 = (q(self.gate_proj.weight), q(self.up_proj.weight), q(self.down_proj.weight))
+            raise NotImplementedError(f"{bits}-bit decode weights are not combined with an input norm or tensor parallelism")
+        weights = (self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight)
+        if bits == 4:
+            if (group_size not in kernels.INT4_GROUPS or self.hidden_size % group_size
+                    or self.intermediate_size % group_size):
+                raise ValueError(f"4-bit decode weights need a group size in {kernels.INT4_GROUPS} that divides "
+                                 f"hidden_size and intermediate_size; got {group_size}")
+            self._w4, self._fp8 = tuple(kernels.quantize_weight_int4(w, group_size) for w in weights), None
+        else:
+            if self.hidden_size % 128 or self.intermediate_size % 128:
+                raise ValueError("8-bit decode weights need hidden_size and intermediate_size multiples of 128")
+            self._fp8, self._w4 = tuple(kernels.quantize_weight_rows_e4m3(w) for w in weights), None
         self._decode_weight_versions = None     # the next decode call follows the kernels that wrote the copies
 
     def _folded_weights(self):
@@ -385,18 +397,22 @@ class FusedGatedMLP(nn.Module):
 
     def _decode_forward(self, x: Tensor, tp_group, residual: Optional[Tensor]) -> Tensor:
         """Inference with at most 64 tokens: the weight-streaming kernels (HBM-bound)."""
-        # A kernel that gave up a wait may have left counters in the scratch non-zero: a
-        # non-zero status read (anywhere in the process) starts a new scratch epoch.
-        key = (x.device, x.dtype, _lib.scratch_epoch())
-        if self._decode_scratch is None or self._decode_scratch[0] != key:
-            self._decode_scratch = (key, kernels.decode_scratch(
-                x.shape[0], self.hidden_size, self.intermediate_size, x.dtype, x.device))
         # The decode kernels begin to stream weights while the kernel ahead of them on the stream is still
         # running. If a parameter has been modified in place since the last decode call (an optimiser step, a
         # weight merge), that kernel may be the writer: this one call starts as an ordinary launch.
         versions = (self.gate_proj.weight._version, self.up_proj.weight._version, self.down_proj.weight._version)
         ordinary = versions != self._decode_weight_versions
         self._decode_weight_versions = versions
+        if self._w4 is not None and tp_group is None:   # (scratch: the call's own, one per stream and capture)
+            wg4, wu4, wd4 = self._w4
+            return kernels.decode_fwd_w4(x, wg4, self.gate_proj.bias, wu4, self.up_proj.bias, wd4, self.down_proj.bias,
+                                         act=self.act_fn, residual=residual, ordinary_launch=ordinary)
+        # A kernel that gave up a wait may have left counters in the scratch non-zero: a
+        # non-zero status read (anywhere in the process) starts a new scratch epoch.
+        key = (x.device, x.dtype, _lib.scratch_epoch())
+        if self._decode_scratch is None or self._decode_scratch[0] != key:
+            self._decode_scratch = (key, kernels.decode_scratch(
+                x.shape[0], self.hidden_size, self.intermediate_size, x.dtype, x.device))
         if self._fp8 is not None and tp_group is None:
             (wg8, wgs), (wu8, wus), (wd8, wds) = self._fp8
             return kernels.decode_fwd_fp8(x, wg8, wgs, self.gate_proj.bias, wu8, wus, self.up_proj.bias, wd8, wds,
