@@ -470,3 +470,46 @@ def test_a_decoder_step_of_all_of_them(pkg, cuda_dev, M):
             graph.replay()
             for got, want in zip(out, step(x)):
                 assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M", [1, 5, 64])
+def test_while_another_kernel_holds_most_sms(pkg, cuda_dev, M):
+    """A long GEMM holds 100 SMs, so that only some blocks of a call are there at a time: those leave their shares of the
+    cut tiles to the ones that come later, and the results keep their bits."""
+    K_ = pkg.ops.kernels
+    lib = pkg._lib.load()
+    g = _gen(cuda_dev, M)
+    K, N, E, k = 2048, 4096, 8, 2
+    x, xl = _rnd(g, M, K), _rnd(g, M, 8192)
+    wl = _w4(pkg, g, 2048, 8192)
+    dense = [_w4(pkg, g, *s) for s in ((N, K), (N, K), (K, N))]
+    experts = [_rnd(g, E, *s, std=s[1] ** -0.5) for s in ((N, K), (N, K), (K, N))]
+    experts4 = [K_.quantize_weight_int4(w, 128) for w in experts]
+    ids, wts = _choices(g, M, E, k)
+    calls = [lambda: K_.linear_w4(xl, wl), lambda: K_.decode_fwd_w4(x, dense[0], None, dense[1], None, dense[2], None),
+             lambda: K_.moe_decode_fwd(x, ids, wts, *experts), lambda: K_.moe_decode_fwd_w4(x, ids, wts, *experts4)]
+    want = [c() for c in calls]
+    a = _rnd(g, 16384, 16384)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    before = lib.gmlp_set_sm_limit(100)
+    try:
+        with torch.cuda.stream(side):
+            K_.gemm(a, a)
+            torch.cuda.synchronize()
+            started, done = torch.cuda.Event(), torch.cuda.Event()
+            started.record()
+            for _ in range(4):
+                K_.gemm(a, a)
+            done.record()
+    finally:
+        lib.gmlp_set_sm_limit(before)
+    started.synchronize()
+    got = [c() for _ in range(5) for c in calls]
+    mine = torch.cuda.Event()
+    mine.record()
+    mine.synchronize()
+    assert not done.query()                           # the GEMMs outlast the calls
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % len(calls)]), i

@@ -152,18 +152,24 @@ __device__ __forceinline__ Segment segment_at(int u, int u_end, int per_tile) {
 // each publishes its part as soon as it has it, and when it is through with its units it waits (bounded) for the
 // others' parts and finishes an equal share of the tile's rows and tokens, adding the parts in CTA order (the result does
 // not depend on arrival). (With one owner per tile that fetched all parts, 64 tokens and 9 CTAs per tile, the owner
-// alone took 26,000 clocks.) A CTA waits only after it has published everything it owes, for CTAs that come to
-// their last unit when it does; one that has not started yet waits for an SM that some other kernel or a CTA that
-// will not wait for it still holds.
+// alone took 26,000 clocks.) A CTA waits only after it has published everything it owes, and not for long: other CTAs
+// of the launch may not have an SM yet (another stream's kernel, or another launch of this one, may hold them), and two
+// launches whose CTAs kept their SMs until all of their own had come could stop one another. A CTA that has waited
+// GIVE_UP_CLOCKS leaves its share to those that come later; the last one to come never waits.
 // Only the float4 columns below M travel: with one token that is a quarter of a 16-column tile.
-// Counter word of a tile: parts published in the low half, CTAs that have seen all of them in the high half; the last of
-// those clears it.
+// Counter word of a tile, ten bits each: parts published, CTAs that gave up waiting (only while parts are missing), CTAs
+// that have seen all parts; the last of those clears it.
+constexpr int COUNT_LEFT = 1 << 10, COUNT_SEEN = 1 << 20, COUNT_MASK = (1 << 10) - 1;
+constexpr long long GIVE_UP_CLOCKS = 100000;  // 50 us; in an undisturbed call parts come within 10
+struct Join {
+  int first, last;   // CTAs that have parts of the tile
+  int mine, shares;  // this CTA finishes share `mine` of `shares`; none below 0
+};
 struct Split {
   Cut cut;
   int M;
   float4* slots;  // [2 * CTAs]: slot 2c holds CTA c's part of the tile it starts in the middle of, 2c + 1 any other
   int* counters;  // [row tiles]; zero before and after the launch
-  int* status;
   volatile int* abortp;
 };
 __device__ __forceinline__ int ld_acquire(const int* p) {
@@ -206,12 +212,12 @@ __device__ __forceinline__ float4 plus(const float4& a, const float4& b) {
 // This CTA's share of a tile whose parts are in the slots: emit(t, row, i, sums) for four tokens 4i .. 4i + 3 of a row, with
 // JOINT over both tiles at once (emit(0, row, i, gate, up)). ITEMS of a thread are worked on together.
 template <int NT, bool JOINT, int COLS_ALL, int THREADS, int ITEMS, typename Emit>
-__device__ __forceinline__ void finish_tile(int tile_begin, int first, int last, const Split& sp, int ep_tid, Emit emit) {
+__device__ __forceinline__ void finish_tile(int tile_begin, const Join& join, const Split& sp, int ep_tid, Emit emit) {
   constexpr int SLOT4 = NT * COLS_ALL / 4 * 128;
-  const int nq = (sp.M + 3) / 4, parts = last - first + 1, mine = blockIdx.x - first;
+  const int nq = (sp.M + 3) / 4, first = join.first, parts = join.last - first + 1;
   const int items = (JOINT ? 1 : NT) * nq * 128;
-  const int share = (items + parts - 1) / parts;
-  const int lo = share * mine, hi = lo + share < items ? lo + share : items;
+  const int share = (items + join.shares - 1) / join.shares;
+  const int lo = share * join.mine, hi = lo + share < items ? lo + share : items;
   const float4* const s0 = sp.slots + static_cast<long long>(slot_of(sp.cut, first, tile_begin)) * SLOT4;
   const float4* const s1 = sp.slots + (2LL * first + 2) * SLOT4;  // the others start in the middle of the tile
   const int per_t = nq * 128;
@@ -340,8 +346,8 @@ __device__ __forceinline__ void emit_product(T* po, const T* pr, long long ld, i
   }
 }
 
-// The end of a segment and of a CTA's units, shared by the stream kernels. `emit_tile(tile, tile_begin, first, last)` finishes
-// this CTA's share of a tile from the slots of CTAs first .. last.
+// The end of a segment and of a CTA's units, shared by the stream kernels. `emit_tile(tile, tile_begin, join)` finishes
+// this CTA's share of a tile from the slots.
 struct Pending {
   int tile[2];
   int n = 0;
@@ -353,7 +359,7 @@ __device__ __forceinline__ bool end_segment(const float (&v)[NT][COLS], const Se
   if (named_bar_or(1, THREADS, *sp.abortp != 0)) return false;
   publish_segment<NT, COLS, COLS_ALL, THREADS>(v, s, sp, col0, row, ep_tid);
   if (s.begin == s.tile_begin && s.end == s.tile_end)
-    emit_tile(s.tile, s.tile_begin, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.x));
+    emit_tile(s.tile, s.tile_begin, Join{static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.x), 0, 1});
   else
     pending.tile[pending.n++] = s.tile;
   return true;
@@ -361,6 +367,7 @@ __device__ __forceinline__ bool end_segment(const float (&v)[NT][COLS], const Se
 template <int THREADS, typename EmitTile>
 __device__ __forceinline__ void end_units(const Pending& pending, int per_tile, const Split& sp, int ep_tid,
                                           EmitTile emit_tile) {
+  __shared__ int shared_mine[2], shared_shares[2];
   if (pending.n == 0) return;
   int first[2], last[2];  // CTAs that have parts of the tile
 #pragma unroll
@@ -375,26 +382,43 @@ __device__ __forceinline__ void end_units(const Pending& pending, int per_tile, 
   // thread 0 waits for the parts of the first tile, thread 32 for those of the second
   const int k = ep_tid >> 5;
   const bool waiter = (ep_tid & 31) == 0 && k < pending.n;
-  const int my_tile = k == 0 ? pending.tile[0] : pending.tile[1];
-  const int my_parts = k == 0 ? last[0] - first[0] + 1 : last[1] - first[1] + 1;
+  int* const counter = sp.counters + (k == 0 ? pending.tile[0] : pending.tile[1]);
+  bool leave = false;  // this thread has still to count itself among those that have seen all parts
+  int shares = 0;
   if (waiter) {
+    const int my_first = k == 0 ? first[0] : first[1];
+    const int parts = (k == 0 ? last[0] : last[1]) - my_first + 1;
+    int mine = static_cast<int>(blockIdx.x) - my_first, v;
+    shares = parts;
     const long long t0 = clock64();
-    while ((ld_acquire(sp.counters + my_tile) & 0xffff) != my_parts) {
-      if (*sp.abortp != 0 || clock64() - t0 > WAIT_LIMIT_CYCLES) {
-        *sp.abortp = 1;
-        atomicCAS(sp.status, 0, GMLP_DEV_TIMEOUT_EPILOGUE);
+    while (((v = ld_acquire(counter)) & COUNT_MASK) != parts) {
+      // (the exchange fails when a part has come since)
+      if (*sp.abortp != 0 || (clock64() - t0 > GIVE_UP_CLOCKS && atomicCAS(counter, v, v + COUNT_LEFT) == v)) {
+        mine = -1;
         break;
       }
     }
+    if (mine >= 0) {
+      const int left = v / COUNT_LEFT & COUNT_MASK;
+      shares -= left;
+      leave = left == 0;
+      if (left > 0) {  // the shares go to those that are here, in the order in which they ask
+        mine = atomicAdd(counter, COUNT_SEEN) / COUNT_SEEN;
+        if (mine == shares - 1) *counter = 0;
+      }
+    }
+    shared_mine[k] = mine;
+    shared_shares[k] = shares;
   }
   if (named_bar_or(1, THREADS, *sp.abortp != 0)) return;
 #pragma unroll 1
   for (int p = 0; p < pending.n; ++p) {
     const int tile = p == 0 ? pending.tile[0] : pending.tile[1];
-    emit_tile(tile, tile * per_tile, p == 0 ? first[0] : first[1], p == 0 ? last[0] : last[1]);
+    const Join join{p == 0 ? first[0] : first[1], p == 0 ? last[0] : last[1], shared_mine[p], shared_shares[p]};
+    if (join.mine >= 0) emit_tile(tile, tile * per_tile, join);
   }
   // the last CTA to have seen all parts leaves the counter ready for the next call
-  if (waiter && (atomicAdd(sp.counters + my_tile, 0x10000) >> 16) == my_parts - 1) sp.counters[my_tile] = 0;
+  if (leave && atomicAdd(counter, COUNT_SEEN) / COUNT_SEEN == shares - 1) *counter = 0;
 }
 
 // Bounded wait that looks at no abort flag: a thread that gives up uses it to see its own copies in flight land

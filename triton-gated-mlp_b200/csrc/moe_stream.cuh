@@ -241,19 +241,19 @@ moe_stream_kernel(const __grid_constant__ MoeMaps maps, const MoeArgs args) {
       for (long long i = blockIdx.x * 128LL + ep_tid; i < all; i += gridDim.x * 128LL)
         out[i] = res ? res[i] : static_cast<T>(0.f);
     }
-    const Split sp{cut, args.M, reinterpret_cast<float4*>(args.slots), args.counters, args.status, abortp};
-    auto emit_tile = [&](int tile, int begin, int first, int last) {
+    const Split sp{cut, args.M, reinterpret_cast<float4*>(args.slots), args.counters, abortp};
+    auto emit_tile = [&](int tile, int begin, const Join& join) {
       if (DUAL) {
         const int a = tile / row_tiles, row0 = (tile - a * row_tiles) * 128;
         moe_factors(args.moe, args.M, moe.list[a], ep_tid, moe);
         named_bar_sync(1, 128);
         T* const oa = out + static_cast<long long>(a) * args.M * ld;
-        finish_tile<NACC, true, MPAD, 128, (MPAD > 16 ? 4 : 1)>(begin, first, last, sp, ep_tid,
+        finish_tile<NACC, true, MPAD, 128, (MPAD > 16 ? 4 : 1)>(begin, join, sp, ep_tid,
                                            [&](int, int r, int i, const float4& gate, const float4& up) {
           if (row0 + r < args.rows) emit_hidden(oa + row0 + r, ld, args.M, i, gate, up, nullptr, 0.f, 0.f, args.act, &moe);
         });
       } else {
-        finish_tile<NACC, false, MPAD, 128, (MPAD > 16 ? 4 : 1)>(begin, first, last, sp, ep_tid,
+        finish_tile<NACC, false, MPAD, 128, (MPAD > 16 ? 4 : 1)>(begin, join, sp, ep_tid,
                                             [&](int, int r, int i, const float4& v, const float4&) {
           const int wr = tile * 128 + r;
           if (wr < args.rows) emit_product(out + wr, res ? res + wr : nullptr, ld, args.M, i, v, nullptr, 0.f, &moe);

@@ -873,8 +873,8 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
             args.residual ? static_cast<const T*>(args.residual)[i] : static_cast<T>(0.f);
     }
     const MoeShared* const mp = is_moe ? &moe : nullptr;
-    const Split sp{cut, args.M, reinterpret_cast<float4*>(args.slots), args.counters, args.status, abortp};
-    auto emit_tile = [&](int tile, int begin, int first, int last) {
+    const Split sp{cut, args.M, reinterpret_cast<float4*>(args.slots), args.counters, abortp};
+    auto emit_tile = [&](int tile, int begin, const Join& join) {
       T* const out = static_cast<T*>(args.out);
       const T* const b0 = static_cast<const T*>(args.bias0);
       const float* const rs = FUSED ? nullptr : args.rowscale;
@@ -887,7 +887,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
           named_bar_sync(1, EPI);
         }
         T* const oa = out + static_cast<long long>(a) * args.M * ld;
-        finish_tile<2, true, MT, EPI, 1>(begin, first, last, sp, ep_tid,
+        finish_tile<2, true, MT, EPI, 1>(begin, join, sp, ep_tid,
                                       [&](int, int r, int i, const float4& gate, const float4& up) {
           const int wr = row0 + r;
           if (wr < args.rows)
@@ -896,7 +896,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
         });
       } else {
         const T* const res = static_cast<const T*>(args.residual);
-        finish_tile<2, false, MT, EPI, 1>(begin, first, last, sp, ep_tid,
+        finish_tile<2, false, MT, EPI, 1>(begin, join, sp, ep_tid,
                                        [&](int t, int r, int i, const float4& v, const float4&) {
           const int wr = tile * ROWS + t * 128 + r;
           if (wr < args.rows)
