@@ -130,6 +130,24 @@ __host__ __device__ __forceinline__ int cut_grain(int per_tile, int unit_clocks)
   return per_tile > 0 && per_tile * unit_clocks <= JOIN_CLOCKS ? per_tile : 1;
 }
 
+// A warp's 32 lanes (rows) of COLS 32-bit columns.
+template <int COLS>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t* r) {
+  if constexpr (COLS == 4) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int c = 0; c < COLS; c += 8)
+      asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r[c]), "=r"(r[c + 1]), "=r"(r[c + 2]), "=r"(r[c + 3]), "=r"(r[c + 4]), "=r"(r[c + 5]),
+                     "=r"(r[c + 6]), "=r"(r[c + 7])
+                   : "r"(taddr + c)
+                   : "memory");
+  }
+}
 struct Segment {
   int tile, begin, end;  // row tile, and this CTA's units of it
   int tile_begin, tile_end;
