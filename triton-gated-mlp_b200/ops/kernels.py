@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 from dataclasses import dataclass
 from typing import NamedTuple
 
@@ -655,12 +656,18 @@ def _few_buffers(scratch: Tensor | None, K: int, N: int, experts: int, work: int
     return scratch.data_ptr(), scratch.numel() * scratch.element_size(), own.data_ptr(), own
 
 
+@functools.lru_cache(maxsize=1024)
 def _w4_work_bytes(M: int, K: int, N: int, experts: int, group: int, dt: torch.dtype) -> int:
     return load().gmlp_w4_work_bytes(M, K, N, experts, group, 0 if dt is torch.bfloat16 else 1)
 
 
 def _raw_stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _few_problem(M: int, K: int, N: int, dt: torch.dtype, act: str, tuning: int = 0) -> Problem:
+    """_problem of a call without dropout and shards, by position (a third of the time of the keywords)."""
+    return Problem(M, K, N, dtype_code(dt), 0.0, 0, 0, 0, 0, 0, act_code(act), tuning)
 
 
 def _rows_of(x: Tensor) -> Tensor:
@@ -753,7 +760,7 @@ def decode_fwd_w4(x: Tensor, w_gate: Int4Weight, b_gate: Tensor | None, w_up: In
     if M == 0:
         return y
     x = _rows_of(x)
-    prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act, (1 << 26) if ordinary_launch else 0)
+    prob = _few_problem(M, K, N, dt, act, (1 << 26) if ordinary_launch else 0)
     with _on(dev):
         stream = _raw_stream(dev)
         sc, sc_bytes, work, keep = _few_buffers(scratch, K, N, 1, nbytes := _w4_work_bytes(M, K, N, 1, group, dt), dev,
@@ -841,7 +848,7 @@ def moe_decode_fwd(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Tensor, w_up
         raise ValueError(f"the mixture-of-experts decode path needs K and N multiples of 64; got K={K} N={N}")
     x, w_gate, w_up, w_down = _rows_of(x), _c(w_gate), _c(w_up), _c(w_down)
     active = min(E, M * k)
-    prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act)
+    prob = _few_problem(M, K, N, dt, act)
     with _on(dev):
         stream = _raw_stream(dev)
         sc, sc_bytes, h, keep = _few_buffers(scratch, K, N, active, 2 * active * M * N, dev, stream)
@@ -874,7 +881,7 @@ def moe_decode_fwd_w4(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Int4Weigh
         return y
     x = _rows_of(x)
     active = min(E, M * k)
-    prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act)
+    prob = _few_problem(M, K, N, dt, act)
     with _on(dev):
         stream = _raw_stream(dev)
         sc, sc_bytes, work, keep = _few_buffers(scratch, K, N, active,
