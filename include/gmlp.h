@@ -319,11 +319,15 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
  * or 128, cols a multiple of it.
  *   w4     rows of cols / 2 bytes: little-endian 32-bit words, word j holding columns 8j .. 8j+7, column 8j + c at
  *          bit (0, 16, 4, 20, 8, 24, 12, 28)[c]; 16-byte aligned
- *   scale  [cols / group, rows];  zero [cols / group, rows], or NULL for zero = 8 everywhere
+ *   scale  [cols / group, rows];  zero [cols / group, rows], or NULL for zero = 8 everywhere; both 4-byte aligned and
+ *          fastest where they are 16-byte aligned and rows is a multiple of 16. They are read in whole 16-byte
+ *          blocks: up to 15 bytes before and behind an array may be read (never used), within its blocks.
  * The weights are never rounded: a group's products with the integers q are summed in fp32 and then take zero and scale.
- * Activations enter as sums of two (bf16) or three (fp16) e4m3 numbers under a power of two per token and group,
- * which is off by at most 2^-17 of the group's largest activation, and not at all for those within 2^-9 (bf16) or
- * 2^-6 (fp16) of it. A NaN or infinite activation makes its token's outputs NaN, and no other token's.
+ * Activations enter as sums of two (bf16) or three (fp16) e4m3 numbers under a power of two, which are off by at most
+ * 2^-17 of the largest activation that shares the power: up to 4 tokens that of its token and group of columns, from 5
+ * tokens on that of its token (in the down product of a mixture: of the token's hidden values of all experts). Those
+ * within 2^-9 (bf16) or 2^-6 (fp16) of the largest are exact. A NaN or infinite activation makes its token's outputs NaN,
+ * and no other token's. Scales have to be finite. Gate and up matrices both have zeros or both have none.
  *
  * gmlp_w4_linear: y[m,r] = sum_c x[m,c] w[r,c] (+ bias[r]) (+ residual[m,r]) for 1 <= M <= 64 and any rows >= 1; x
  *   has row pitch ldx (a multiple of 8), y and residual [M, rows] are contiguous.

@@ -513,3 +513,21 @@ def test_while_another_kernel_holds_most_sms(pkg, cuda_dev, M):
     torch.cuda.synchronize()
     for i, y in enumerate(got):
         assert torch.equal(y, want[i % len(calls)]), i
+
+
+@pytest.mark.parametrize("M", [2, 9, 50])
+@pytest.mark.parametrize("shift", [2, 6, 12])
+def test_scales_and_zeros_on_any_four_byte_boundary(pkg, cuda_dev, M, shift):
+    """Views that start inside a 16-byte block, with and without zeros: the same bits as aligned copies."""
+    K_ = pkg.ops.kernels
+    g = _gen(cuda_dev, M)
+    for rows in (256, 333):
+        for symmetric in (False, True):
+            w = _w4(pkg, g, rows, 512, group=64, symmetric=symmetric)
+            x = _rnd(g, M, 512)
+            s = torch.empty(w.scale.numel() + shift, dtype=BF, device=cuda_dev)[shift:].view(w.scale.shape).copy_(w.scale)
+            z = None if symmetric else torch.empty(w.zero.numel() + 2 * shift, dtype=torch.uint8,
+                                                   device=cuda_dev)[2 * shift:].view(w.zero.shape).copy_(w.zero)
+            y = K_.linear_w4(x, K_.Int4Weight(w.w4, s, z))
+            assert torch.equal(y, K_.linear_w4(x, w))
+            ft.check(y, *ft.linear(x, ft.unpack(*w), None, None, BF, 64), "shifted scales")

@@ -124,7 +124,8 @@ __device__ __forceinline__ int cut_owner(const Cut& c, int unit) {  // the CTA t
   return unit < big ? unit / (c.each + 1) : c.odd + (unit - big) / c.each;
 }
 // Joining the parts of a tile takes some 6,000 clocks after its last unit (publish, see the others' parts, fetch them). Where
-// one CTA streams the whole tile in less, tiles stay whole.
+// one CTA streams the whole tile in less, tiles stay whole (device time with and without that rule: 4-bit MLP, 3 tokens,
+// K=512, N=896, 10.4 against 13.1 us; 18 experts of 576 x 320, 5 tokens, top 3, with the router, 23.5 against 25.6).
 constexpr int JOIN_CLOCKS = 6000;
 __host__ __device__ __forceinline__ int cut_grain(int per_tile, int unit_clocks) {
   return per_tile > 0 && per_tile * unit_clocks <= JOIN_CLOCKS ? per_tile : 1;

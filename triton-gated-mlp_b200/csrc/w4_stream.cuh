@@ -34,7 +34,7 @@
 // Kernels of a product: w4_stream_kernel; from 5 tokens on w4_split_kernel before it (terms, powers of two and group sums of
 // the activations, a few microseconds of latency that hide behind the weight stream's start).
 // Warps of w4_stream_kernel: 0 streams weights (TMA), 1 issues MMA, 2 streams activation terms, scales and zeros (TMA), 3
-// packs scales and zeros, and copies those whose rows are not aligned (cp.async), 4..11 expand (four per tile, thread = row), 12..19 take the sums
+// packs scales and zeros, 4..11 expand (four per tile, thread = row), 12..19 take the sums
 // and run the epilogue (thread = a row of both tiles; up to 4 tokens 12..15, and 16..19 make activation terms; up to 32 tokens
 // four warps per half of the tokens, 64 tokens four per quarter). Everything between two roles is a ring with full / empty barriers, and
 // every ring turns once a unit (65,536 weights, 1,400 clocks at the copy bandwidth): a role that is one thread or one warp
@@ -236,8 +236,9 @@ struct W4Args {
   MoeTable moe;
 };
 
-// Scales and zeros of a unit in shared memory. Copied by TMA: [2 tiles][groups][128] scales, then zeros alike. Copied by
-// words (rows that are not aligned start up to 3 bytes into a word): 416 bytes per (tile, group), zeros from byte 272.
+// Scales and zeros of a unit in shared memory. As TMA boxes (W4Args::wide): [2 tiles][groups][128] scales, then zeros alike.
+// As rows: per (tile, group) the 16-byte blocks that the 128 scales lie in (up to 17), from byte 272 on those of the zeros (up
+// to 9).
 constexpr int W4_META_ROW = 416;
 constexpr int W4_META_ZERO = 272;
 
@@ -318,14 +319,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
       : "memory");
-}
-// `bytes` (1..4) of a 4-byte word, the rest zero.
-__device__ __forceinline__ void cp_async_word(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-// Arrives on `bar` when this thread's cp.asyncs so far have landed (the barrier counts the thread from the start).
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared_u4(uint32_t a) {
   uint4 v;
@@ -419,7 +412,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     const uint32_t bar = wfull + 8 * threadIdx.x;
     int count = 1;  // wfull (TMA), aempty and cfull (MMA), sfull (warp 3), drain
     if (bar >= wempty && bar < xfull) count = 8;                               // expanding warps
-    if (bar >= xfull && bar < xempty) count = 1 + (args.wide ? 0 : 32) + (FUSED ? args.M : 0);  // TMA, copying lanes, tokens
+    if (bar >= xfull && bar < xempty) count = 1 + (FUSED ? args.M : 0);  // TMA, tokens
     if (bar >= xempty && bar < afull) count = 1 + C::EPI / 32;                 // MMA, accumulating warps
     if (bar >= afull && bar < aempty) count = 8;
     if (bar >= cempty && bar < sfull) count = C::EPI / 32;
@@ -535,11 +528,28 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       const int a = DUAL ? 0 : w.a;
       const uint32_t dst = x_base + r.at * C::X_STAGE, fb = xfull + 8 * r.at;
       constexpr uint32_t META_BYTES = GPU * MT * 4;
+      const uint32_t md = m_base + r.at * C::M_STAGE;
+      uint32_t sz_bytes = args.wide ? 2 * GPU * 128 * (2 + (args.zero0 != nullptr ? 1 : 0)) : 0;
+      uint64_t src = 0;  // this lane's copy
+      uint32_t len = 0;
+      if (!args.wide) {
+        const int t = lane >> 1 >= GPU ? 1 : 0, g = (lane >> 1) - t * GPU;  // even lanes: scales, odd ones: zeros
+        const int skip = DUAL ? 0 : t * 128, left = args.rows - w.row0 - skip;
+        const long long e0 = (static_cast<long long>(moe.list[w.a]) * args.groups + w.kb * GPU + g) * args.rows + w.row0 + skip;
+        const uint32_t nrow = static_cast<uint32_t>(left < 128 ? left : 128);
+        const uint64_t base = reinterpret_cast<uint64_t>(
+            lane & 1 ? static_cast<const void*>(DUAL && t == 1 ? args.zero1 : args.zero0)
+                     : static_cast<const void*>(DUAL && t == 1 ? args.scale1 : args.scale0));
+        const int sh = 1 - (lane & 1);  // bytes of an element, as a shift
+        src = base + (static_cast<uint64_t>(e0) << sh);
+        if (base != 0 && left > 0 && lane < 4 * GPU && g < groups_in(w.kb))
+          len = ((static_cast<uint32_t>(src) & 15u) + (nrow << sh) + 15u) & ~15u;
+        src &= ~15ull;
+        sz_bytes = __reduce_add_sync(0xffffffffu, len);
+      }
       if (elect_one()) {
-        const uint32_t sz_bytes = args.wide ? 2 * GPU * 128 * (2 + (args.zero0 != nullptr ? 1 : 0)) : 0;
         mbar_expect_tx(fb, (FUSED ? 0 : 2 * TERMS * MT * 128 + META_BYTES) + sz_bytes);
         if (args.wide) {
-          const uint32_t md = m_base + r.at * C::M_STAGE;
           const int gy = moe.list[w.a] * args.groups + w.kb * GPU;
           tma_load_2d_hint(md, &maps.s0, fb, w.row0, gy, pol_w);
           tma_load_2d_hint(md + GPU * 256, DUAL ? &maps.s1 : &maps.s0, fb, w.row0 + (DUAL ? 0 : 128), gy, pol_w);
@@ -559,6 +569,8 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
         }
       }
       __syncwarp();
+      if (len != 0)
+        bulk_load(md + (lane >> 1) * W4_META_ROW + (lane & 1) * W4_META_ZERO, reinterpret_cast<const void*>(src), len, fb);
       step(w);
       r.next(NX);
     }
@@ -571,55 +583,15 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   } else if (warp == 3) {
     // --------------------------------------------------- scales and zeros --
     if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    // One word per row, tile and group for all the accumulating threads: scale << 16 | zero. Where the rows of scales and zeros
-    // are not aligned (any number of weight rows is allowed) this warp copies them too, up to 65 + 33 words of 4 bytes per
-    // (tile, group), of which the last one only as far as the rows go, and runs as many units ahead with that as there
-    // are stages.
+    // One word per row, tile and group for all the accumulating threads: scale << 16 | zero.
     const bool zeros = args.zero0 != nullptr;
-    uint8_t* const m_stages = smem + NW * 2 * W4_TILE_BYTES + NX * C::X_STAGE;
-    uint8_t* const s_stages = m_stages + NX * C::M_STAGE;
-    const int ahead = args.wide ? 0 : NX - 1;
-    W4Walk wc, w;  // positions of the unit being copied and of the unit being packed
-    start(wc);
+    const uint8_t* const m_stages = smem + NW * 2 * W4_TILE_BYTES + NX * C::X_STAGE;
+    uint8_t* const s_stages = smem + NW * 2 * W4_TILE_BYTES + NX * (C::X_STAGE + C::M_STAGE);
+    W4Walk w;
     start(w);
-    Ring rc, r;
+    Ring r;
     bool ok = true;
-    for (int u = 0; u < units + ahead && ok; ++u) {
-      if (!args.wide && u < units) {
-        if (!(ok = quick_wait(xempty + 8 * rc.at, rc.phase ^ 1u, abortp))) break;
-        const int ng = groups_in(wc.kb);
-        const long long unit0 = (static_cast<long long>(moe.list[wc.a]) * args.groups + wc.kb * GPU) * args.rows + wc.row0;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint16_t* const sc = (DUAL && t == 1) ? args.scale1 : args.scale0;
-          const uint8_t* const ze = (DUAL && t == 1) ? args.zero1 : args.zero0;
-          const int skip = DUAL ? 0 : t * 128;
-          const int left = args.rows - wc.row0 - skip;
-          const int nrow = left < 128 ? left : 128;
-#pragma unroll 1
-          for (int i = 0; i < ng && nrow > 0; ++i) {
-            const long long e0 = unit0 + skip + static_cast<long long>(i) * args.rows;
-            const uint32_t dst = m_base + rc.at * C::M_STAGE + (t * GPU + i) * W4_META_ROW + lane * 4;
-            const int head = static_cast<int>(e0 & 1) * 2, bytes = head + 2 * nrow - lane * 4;
-            const char* const s0 = reinterpret_cast<const char*>(sc + e0) - head + lane * 4;
-#pragma unroll
-            for (int k = 0; k < 3; ++k)
-              if (bytes > k * 128) cp_async_word(dst + k * 128, s0 + k * 128, bytes - k * 128 < 4 ? bytes - k * 128 : 4);
-            if (ze != nullptr) {
-              const int zhead = static_cast<int>(e0 & 3), zbytes = zhead + nrow - lane * 4;
-              const uint8_t* const z0 = ze + e0 - zhead + lane * 4;
-#pragma unroll
-              for (int k = 0; k < 2; ++k)
-                if (zbytes > k * 128)
-                  cp_async_word(dst + W4_META_ZERO + k * 128, z0 + k * 128, zbytes - k * 128 < 4 ? zbytes - k * 128 : 4);
-            }
-          }
-        }
-        cp_async_arrive(xfull + 8 * rc.at);
-        step(wc);
-        rc.next(NX);
-      }
-      if (u < ahead) continue;
+    for (int u = 0; u < units && ok; ++u) {
       if (!(ok = quick_wait(xfull + 8 * r.at, r.phase, abortp))) break;
       const int ng = groups_in(w.kb);
       const uint8_t* const mm = m_stages + r.at * C::M_STAGE;
@@ -635,14 +607,16 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
             s23 = q.y;
             if (zeros) z = *reinterpret_cast<const uint32_t*>(mm + 2 * GPU * 256 + (t * GPU + g) * 128 + lane * 4);
           } else {
-            // where the rows start inside the copied words: low bits of the first one's index
+            // where the rows start inside the copied blocks of 16 bytes: low bits of the first one's address
             const uint32_t e = (static_cast<uint32_t>(moe.list[w.a]) * args.groups + w.kb * GPU + g) *
                                    static_cast<uint32_t>(args.rows) + w.row0 + (DUAL ? 0 : t * 128);
+            const uint32_t s_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(DUAL && t == 1 ? args.scale1 : args.scale0));
+            const uint32_t z_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(DUAL && t == 1 ? args.zero1 : args.zero0));
             const uint8_t* const mr = mm + (t * GPU + g) * W4_META_ROW;
-            const uint16_t* const sp = reinterpret_cast<const uint16_t*>(mr + (e & 1u) * 2) + lane * 4;
+            const uint16_t* const sp = reinterpret_cast<const uint16_t*>(mr + ((s_at + 2 * e) & 15u)) + lane * 4;
             s01 = sp[0] | (static_cast<uint32_t>(sp[1]) << 16);
             s23 = sp[2] | (static_cast<uint32_t>(sp[3]) << 16);
-            const uint8_t* const zp = mr + W4_META_ZERO + (e & 3u) + lane * 4;
+            const uint8_t* const zp = mr + W4_META_ZERO + ((z_at + e) & 15u) + lane * 4;
             if (zeros) z = zp[0] | (zp[1] << 8) | (zp[2] << 16) | (static_cast<uint32_t>(zp[3]) << 24);
           }
           uint4 o = make_uint4((s01 << 16) | (z & 15u), (s01 & 0xFFFF0000u) | ((z >> 8) & 15u),
@@ -659,7 +633,6 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       abort_flag = 1;
       atomicCAS(args.status, 0, GMLP_DEV_TIMEOUT_PRODUCER);
     }
-    cp_async_wait_all();
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA --
     if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
