@@ -5,6 +5,9 @@
 //   DUAL   units = (active expert, row tile of N, 64 columns of K), two tiles (gate, up) a unit; all M tokens are
 //          multiplied (the tensor pipe has the time, see MPAD there) and the epilogue keeps the chosen ones
 //   !DUAL  units = (row tile of the hidden size, (active expert, 64 columns of N)): one accumulator for all experts
+// Measured (one B200, with the router): 8 experts of 4096 x 14336, one token, top 2: 129 us for 705 MB of chosen weights = 5.4
+// TB/s; 64 experts of 2048 x 1408, 64 tokens, top 6: 204 us for 1107 MB = 5.4 TB/s (copy rate 6.56; with 64 tokens an SM also
+// takes 8 KB of activations from L2 for every 32 KB of weights).
 #pragma once
 #include "few_token.cuh"
 
@@ -314,7 +317,7 @@ moe_stream_kernel(const __grid_constant__ MoeMaps maps, const MoeArgs args) {
 // a pass, products exact in fp32, eight of them summed in fp32 and added to an fp64 sum, so that the order of the
 // logits (a choice next to a border) is that of the exact sums but for a relative 1e-7. The logits go to the first
 // block's shared memory (distributed shared memory), whose first warp selects. Latency-bound: C spreads the 2 E K bytes
-// of a token over SMs.
+// of a token over SMs. Measured: 8 experts x 4096, one token 4.4 us; 64 x 2048, 64 tokens 5.2; 512 x 4096, 64 tokens 32.
 constexpr int ROUTE_THREADS = 256;
 struct RouteArgs {
   const void* x;

@@ -43,6 +43,13 @@
 // issues the MMAs was itself the bound, at 3,000 clocks per 32,768 weights.)
 //
 // Work split: stream-K over units of (two row tiles, 256 columns) as in few_token.cuh.
+//
+// Measured (one B200, replayed from a graph, G = 128): gated MLP K=8192, N=28672 of one token 70 us = 5.3 TB/s of the packed
+// bytes (the copy rate is 6.56), 16 tokens 94, 32 tokens 113, 64 tokens 158 (G = 64: 227, G = 32: 438); product 131072 x 4096,
+// 8 tokens 56 us; 4096 x 4096, one token 8.5 us, of which 7 are the life of a block from its start to its join. Up to 8
+// tokens HBM bounds it. Above, the accumulating warps do: two instructions per two (row, token) sums of a group, and the
+// trip of the sums through tensor memory (at 64 tokens 55 % of the issue slots, 40 % of the tensor pipe, 29 % of
+// HBM). Fetching a group's sums while those of the group before are worked on was slower (64 tokens: 164 us).
 #pragma once
 #include <cuda_fp8.h>
 
@@ -53,7 +60,7 @@ namespace gmlp {
 constexpr int W4_TILE_BYTES = 16384;  // 128 rows x 128 bytes: 256 columns
 constexpr int W4_UNIT_COLS = 256;
 constexpr int W4_HALF_COLS = 128;
-constexpr int W4_UNIT_CLOCKS = 1400;  // of one CTA, alone or not
+constexpr int W4_UNIT_CLOCKS = 1400;  // of one CTA, whether or not the others stream
 
 // Terms per activation.
 template <typename T>
@@ -114,7 +121,9 @@ __device__ __forceinline__ float nan_max(float a, float b) { return (b > a || b 
 // x [active][M][cols] (row pitch ldx) -> t8 [TERMS][R][cols] e4m3 bytes, meta [active][groups][MT] floats 2^-9 sum_g x 2^e with
 // the groups of a row padded to whole units of 256 columns (zeros there), and per token 512 2^-e (NaN where the token holds
 // a NaN or an infinity). A cluster of blocks per token: each takes a share of the token's half units (128 columns, 16
-// lanes of 8; a group is 4, 8 or 16 lanes), finds their largest value, and goes over them again with the token's.
+// lanes of 8; a group is 4, 8 or 16 lanes), finds their largest value, and goes over them again with the token's. Bound by
+// latency (launch, two passes, the cluster's barrier): 7 us for 8 or 16 tokens, 8 to 10 for 64, cold and alone; as the
+// predecessor of a stream kernel about 5, since that one starts meanwhile.
 struct W4SplitArgs {
   const void* x;
   long long ldx;
