@@ -326,7 +326,8 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
  * Activations enter as sums of two (bf16) or three (fp16) e4m3 numbers under a power of two, which are off by at most
  * 2^-17 of the largest activation that shares the power: up to 4 tokens that of its token and group of columns, from 5
  * tokens on that of its token (in the down product of a mixture: of the token's hidden values of all experts). Those
- * within 2^-9 (bf16) or 2^-6 (fp16) of the largest are exact. A NaN or infinite activation makes its token's outputs NaN,
+ * within 2^-9 (bf16) or 2^-6 (fp16) of the largest are exact. (Where the largest is below 2^-113, which only bf16
+ * reaches, they are off by up to 2^-130.) A NaN or infinite activation makes its token's outputs NaN,
  * and no other token's. Scales have to be finite. Gate and up matrices both have zeros or both have none.
  *
  * gmlp_w4_linear: y[m,r] = sum_c x[m,c] w[r,c] (+ bias[r]) (+ residual[m,r]) for 1 <= M <= 64 and any rows >= 1; x

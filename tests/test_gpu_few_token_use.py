@@ -531,3 +531,50 @@ def test_scales_and_zeros_on_any_four_byte_boundary(pkg, cuda_dev, M, shift):
             y = K_.linear_w4(x, K_.Int4Weight(w.w4, s, z))
             assert torch.equal(y, K_.linear_w4(x, w))
             ft.check(y, *ft.linear(x, ft.unpack(*w), None, None, BF, 64), "shifted scales")
+
+
+@pytest.mark.parametrize("M", [1, 4, 8, 64])
+@pytest.mark.parametrize("largest", [3e38, 1e30, 1e-33])
+def test_ends_of_bfloat16(pkg, cuda_dev, M, largest):
+    """Activations next to the type's largest number whose products with the weights are finite, and tiny ones."""
+    K_ = pkg.ops.kernels
+    g = _gen(cuda_dev, M)
+    w = _w4(pkg, g, 300, 256, group=64)
+    w = w._replace(scale=(w.scale.float() * 2.0 ** -6).to(BF))
+    x = ((torch.rand((M, 256), generator=g, device=cuda_dev) * 2 - 1) * largest).to(BF)
+    y = K_.linear_w4(x, w)
+    assert torch.isfinite(y).all()
+    ft.check(y, *ft.linear(x, ft.unpack(*w), None, None, BF, 64), f"M={M} largest={largest}")
+
+
+@pytest.mark.parametrize("M", [2, 12])
+def test_dense_module_with_sizes_only_four_bits_take(pkg, cuda_dev, M):
+    torch.manual_seed(M)
+    m = pkg.FusedGatedMLP(96, 160, bias=False).to(cuda_dev, BF)
+    m.quantize_decode_weights(bits=4, group_size=32)
+    x = _rnd(_gen(cuda_dev, M), M, 96)
+    q = [ft.unpack(*w) for w in m._w4]
+    with torch.no_grad():
+        ft.check(m(x), *ft.mlp(x, q[0], None, q[1], None, q[2], None, None, BF, "silu", 32), "96 x 160")
+
+
+def test_two_host_threads_on_one_stream(pkg, cuda_dev):
+    """Their kernels interleave on the stream: each thread has work buffers of its own."""
+    import threading
+
+    sets = [_calls(pkg, cuda_dev, M, seed=3 * M) for M in (5, 40)]
+    want = [{n: c() for n, c in s.items()} for s in sets]
+    bad = []
+
+    def run(calls, expected):
+        for _ in range(100):
+            for n, c in calls.items():
+                if not torch.equal(c(), expected[n]):
+                    bad.append(n)
+
+    threads = [threading.Thread(target=run, args=a) for a in zip(sets, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -183,6 +183,8 @@ def test_module_quantize_arguments(pkg):
         m.quantize_decode_weights()
     m.quantize_decode_weights(bits=4, group_size=64)
     assert m._w4[0].w4.shape == (384, 96) and m._w4[2].scale.shape == (6, 192) and m._fp8 is None
+    with pytest.raises(NotImplementedError, match="input norm"):
+        m.attach_input_norm(torch.ones(192))
     m.quantize_decode_weights(False)
     assert m._w4 is None
     m.attach_input_norm(torch.ones(192))

@@ -18,7 +18,7 @@
 //    least 16, and the weights of one arrive every 89).
 //    The block: up to 4 tokens, a token and group (terms made inside the kernel, unit by unit); above, a whole token.
 // Per row r, token m:
-//   y[r][m] = 512 sum_g s[r][g] * ( acc[r][m]  -  z[r][g] * sx[m][g] ) * 2^-e,
+//   y[r][m] = sum_g 512 s[r][g] * ( acc[r][m]  -  z[r][g] * sx[m][g] ) * 2^-e,
 //   acc = sum_i sum_{c in g} (q[r][c] 2^-9) t_i[c][m],   sx = 2^-9 sum_{c in g} x[m][c] 2^e
 // with the scale, the zero point and the power of two applied in 32 bits when a group's sums leave tensor memory:
 // neither weights nor activations are rounded (but for the bound above), and that work is per token and group, not per
@@ -119,7 +119,7 @@ __device__ __forceinline__ float amax8(const float (&v)[8]) {
 __device__ __forceinline__ float nan_max(float a, float b) { return (b > a || b != b) ? b : a; }
 
 // x [active][M][cols] (row pitch ldx) -> t8 [TERMS][R][cols] e4m3 bytes, meta [active][groups][MT] floats 2^-9 sum_g x 2^e with
-// the groups of a row padded to whole units of 256 columns (zeros there), and per token 512 2^-e (NaN where the token holds
+// the groups of a row padded to whole units of 256 columns (zeros there), and per token 2^-e (NaN where the token holds
 // a NaN or an infinity). A cluster of blocks per token: each takes a share of the token's half units (128 columns, 16
 // lanes of 8; a group is 4, 8 or 16 lanes), finds their largest value, and goes over them again with the token's. Bound by
 // latency (launch, two passes, the cluster's barrier): 7 us for 8 or 16 tokens, 8 to 10 for 64, cold and alone; as the
@@ -188,7 +188,7 @@ w4_split_kernel(const W4SplitArgs args) {
   for (int i = 1; i < W4_SPLIT_CLUSTER; ++i) amax = nan_max(amax, block_max[i]);
   const bool bad = amax != amax;
   const int ex = bad ? 0 : split_exponent(amax);
-  if (rank == 0 && tid == 0) args.rowscale[m] = bad ? amax : 512.0f * power_of_two(-ex);
+  if (rank == 0 && tid == 0) args.rowscale[m] = bad ? amax : power_of_two(-ex);
   const int width = 4 << args.gshift;  // lanes per group
   for (int first = lo; first < hi; first += W4_SPLIT_THREADS / 16) {
     const int item = first + (tid >> 4);
@@ -227,7 +227,7 @@ struct W4Args {
   int cols;
   int* status;
   const float* meta;       // not FUSED: [experts in h or 1][kbt * groups per unit][MT] sx
-  const float* rowscale;   // not FUSED: [M] 512 2^-e
+  const float* rowscale;   // not FUSED: [M] 2^-e
   const uint16_t* scale0;  // [experts][groups][rows], T
   const uint16_t* scale1;  // DUAL: the up matrix's
   const uint8_t* zero0;    // [experts][groups][rows] or null (8)
@@ -897,7 +897,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
 #pragma unroll
           for (int b = 0; b < BUF_PAIRS; ++b) {
             const uint32_t sz = ss[((b & 1) * GPU + g0 + (b >> 1)) * 128];
-            sc[b] = (FUSED ? 512.0f : 1.0f) * Pack2<T>::unpack(sz >> 16).x;
+            sc[b] = 512.0f * Pack2<T>::unpack(sz >> 16).x;
             // an integer below 2^23 in a float's fraction: 2^23 - (2^23 + z)
             nz[b] = 8388608.0f - __uint_as_float(0x4B000000u | (sz & 15u));
           }
@@ -932,10 +932,12 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
                       const float sx[4] = {q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
                       for (int j = 0; j < 4; j += 2) {
-                        const float y0 = tok[j] * fmaf(nz[b0 + b], sx[j], __uint_as_float(x[b][k + j]));
-                        const float y1 = tok[j + 1] * fmaf(nz[b0 + b], sx[j + 1], __uint_as_float(x[b][k + j + 1]));
-                        v[t][(c + k + j) / 2] =
-                            f2_fma(f2_pack(sc[b0 + b], sc[b0 + b]), f2_pack(y0, y1), v[t][(c + k + j) / 2]);
+                        // (scale and power of two first: their product with the sum is the group's share of the output and
+                        // overflows only where that does)
+                        const f32x2 f = f2_pack(sc[b0 + b] * tok[j], sc[b0 + b] * tok[j + 1]);
+                        const f32x2 y = f2_pack(fmaf(nz[b0 + b], sx[j], __uint_as_float(x[b][k + j])),
+                                                fmaf(nz[b0 + b], sx[j + 1], __uint_as_float(x[b][k + j + 1])));
+                        v[t][(c + k + j) / 2] = f2_fma(f, y, v[t][(c + k + j) / 2]);
                       }
                     } else {
                       // two tokens an instruction: what bounds many tokens is issue slots

@@ -341,6 +341,8 @@ class FusedGatedMLP(nn.Module):
         row-wise kernel of its own."""
         if weight.shape != (self.hidden_size,):
             raise ValueError(f"norm weight must have shape ({self.hidden_size},), got {tuple(weight.shape)}")
+        if self._w4 is not None:
+            raise NotImplementedError("4-bit decode weights are not combined with an input norm")
         self.input_norm_weight = nn.Parameter(weight.detach().clone().to(self.gate_proj.weight.device,
                                                                           self.gate_proj.weight.dtype))
         self.input_norm_eps = float(eps)
@@ -492,7 +494,8 @@ class FusedGatedMLP(nn.Module):
         if x.dtype == torch.float32 and self.input_norm_weight is not None:
             raise NotImplementedError("the input norm is not available for float32 modules")
         if (not needs_grad and p == 0.0 and x.is_cuda and x.dtype != torch.float32
-                and kernels.decode_supported(x.shape[0], self.hidden_size, self.intermediate_size)):
+                and (kernels.decode_supported(x.shape[0], self.hidden_size, self.intermediate_size)
+                     or (self._w4 is not None and 0 < x.shape[0] <= kernels.DECODE_MAX_TOKENS))):
             y = self._decode_forward(x, tp_group, residual)
             return y.view(shapes) if len(shapes) > 2 else y
         if self.input_norm_weight is not None:

@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import threading
 from dataclasses import dataclass
 from typing import NamedTuple
 
@@ -619,7 +620,8 @@ def few_scratch(K: int, N: int, experts: int, device: torch.device) -> Tensor:
 
 def _scratch_for(counters: int, work: int, dev: torch.device, stream: int):
     """(scratch address, bytes, work address) of calls without buffers of their own: one pair of buffers per (device,
-    stream), since calls on a stream are ordered, and one per graph capture, cleared inside the graph: no two graphs, and
+    stream, host thread), since a thread's calls on a stream are ordered (two threads' kernels may interleave), and
+    one per graph capture, cleared inside the graph: no two graphs, and
     no graph and an eager call, ever share counters. New ones are made when a kernel has given up a wait since
     (its counters may be dirty). A work buffer above 64 MB is the call's own (it must live until the call has enqueued
     its kernels: the third entry keeps it)."""
@@ -628,7 +630,7 @@ def _scratch_for(counters: int, work: int, dev: torch.device, stream: int):
         v = C.c_uint64(0)
         check(load().gmlp_capture_id(stream, C.byref(v)))
         cap = v.value
-    key = (dev.index, stream, cap != 0)
+    key = (dev.index, stream, threading.get_ident(), cap != 0)
     tag = (cap, _lib.scratch_epoch())
     have = _few_scratch.get(key)
     if have is None or have[0] != tag or have[1] < counters:
