@@ -240,6 +240,13 @@ def test_refusals(pkg, cuda_dev):
                  lambda: K_.moe_decode_fwd(x.float(), ids, wts, *(full.float(),) * 3)):
         with pytest.raises(NotImplementedError):
             call()
+    cpu = K_.Int4Weight(*(t.cpu() for t in w))
+    for call in (lambda: K_.linear_w4(x, cpu), lambda: K_.linear_w4(x, w._replace(scale=cpu.scale)),
+                 lambda: K_.linear_w4(x, w._replace(zero=cpu.zero)),
+                 lambda: K_.decode_fwd_w4(x, w, None, w, None, cpu, None),
+                 lambda: K_.moe_decode_fwd(x, ids.cpu(), wts, full, full, full)):
+        with pytest.raises(pkg._lib.GmlpError, match="no CPU path"):
+            call()
     # a router row of 100 columns is no multiple of 8; 4-bit words have to start on 16 bytes
     with pytest.raises(pkg._lib.GmlpError, match="multiple of 8"):
         K_.moe_route(_rnd(g, 2, 100), _rnd(g, 4, 100), 1)

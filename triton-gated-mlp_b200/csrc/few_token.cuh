@@ -128,7 +128,7 @@ __device__ __forceinline__ int cut_owner(const Cut& c, int unit) {  // the CTA t
 // K=512, N=896, 10.4 against 13.1 us; 18 experts of 576 x 320, 5 tokens, top 3, with the router, 23.5 against 25.6).
 constexpr int JOIN_CLOCKS = 6000;
 __host__ __device__ __forceinline__ int cut_grain(int per_tile, int unit_clocks) {
-  return per_tile > 0 && per_tile * unit_clocks <= JOIN_CLOCKS ? per_tile : 1;
+  return per_tile > 0 && per_tile <= JOIN_CLOCKS / unit_clocks ? per_tile : 1;
 }
 
 // A warp's 32 lanes (rows) of COLS 32-bit columns.

@@ -586,15 +586,17 @@ def dequantize_weight_int4(w: Int4Weight) -> Tensor:
 def _int4_group(w: Int4Weight, lead: tuple, rows: int, cols: int, dt: torch.dtype, dev: torch.device) -> int:
     """Checks a 4-bit weight against the shape it must have; returns its group size."""
     q, s, z = w
-    sh = s.shape
+    sh, idx = s.shape, dev.index
     groups = sh[-2] if len(sh) >= 2 else 0
     group = cols // groups if groups else 0
     want = (*lead, groups, rows)
     if (group in INT4_GROUPS and groups * group == cols and q.dtype is torch.uint8 and q.shape == (*lead, rows, cols // 2)
-            and s.dtype is dt and sh == want and q.is_contiguous() and s.is_contiguous() and q.device == dev
-            and s.device == dev
-            and (z is None or (z.dtype is torch.uint8 and z.shape == want and z.is_contiguous() and z.device == dev))):
+            and s.dtype is dt and sh == want and q.is_contiguous() and s.is_contiguous() and q.get_device() == idx
+            and s.get_device() == idx
+            and (z is None or (z.dtype is torch.uint8 and z.shape == sh and z.is_contiguous() and z.get_device() == idx))):
         return group
+    if require_cuda(q, s, z) != dev:
+        raise _lib.GmlpError(f"tensors on different devices: {dev} and {q.device}")
     if q.dtype is not torch.uint8 or q.shape != (*lead, rows, cols // 2) or q.device != dev or not q.is_contiguous():
         raise ValueError(f"4-bit weights must be contiguous uint8 of shape {(*lead, rows, cols // 2)} on {dev}; got "
                          f"{q.dtype} {tuple(q.shape)} on {q.device}")
@@ -709,7 +711,7 @@ def linear_w4(x: Tensor, w: Int4Weight, bias: Tensor | None = None, residual: Te
     [rows, cols]; any number of rows). The kernel normally starts streaming weights while the preceding kernel on the
     stream is still running; ordinary_launch=True makes it wait first (for the call that follows a kernel which
     writes the weights)."""
-    dev = require_cuda(x, w[0], w[1], w[2], bias, residual)
+    dev = require_cuda(x, bias, residual)
     dt = _same_dtype(x, bias, residual)
     _few_common(x, dt, "linear_w4")
     M, K = x.shape
@@ -746,7 +748,7 @@ def decode_fwd_w4(x: Tensor, w_gate: Int4Weight, b_gate: Tensor | None, w_up: In
     """decode_fwd on 4-bit weights with group scales (quantize_weight_int4); x, biases, residual and the result stay
     16-bit, the hidden state is rounded to 16 bits between the two kernels as in decode_fwd. All three matrices share
     one group size."""
-    dev = require_cuda(x, *w_gate, b_gate, *w_up, b_up, *w_down, b_down, residual)
+    dev = require_cuda(x, b_gate, b_up, b_down, residual)
     dt = _same_dtype(x, b_gate, b_up, b_down, residual)
     _few_common(x, dt, "decode_fwd_w4")
     M, K = x.shape
@@ -864,7 +866,7 @@ def moe_decode_fwd_w4(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Int4Weigh
                       w_down: Int4Weight, act: str = "silu", residual: Tensor | None = None,
                       scratch: Tensor | None = None) -> Tensor:
     """moe_decode_fwd on 4-bit experts: Int4Weight matrices with a leading [experts] dimension, one group size."""
-    dev = require_cuda(x, ids, weights, *w_gate, *w_up, *w_down, residual)
+    dev = require_cuda(x, ids, weights, residual)
     dt = _same_dtype(x, residual)
     _few_common(x, dt, "moe_decode_fwd_w4")
     M, K = x.shape
