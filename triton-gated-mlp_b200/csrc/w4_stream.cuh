@@ -45,10 +45,11 @@
 // Work split: stream-K over units of (two row tiles, 256 columns) as in few_token.cuh.
 //
 // Measured (one B200, replayed from a graph, G = 128): gated MLP K=8192, N=28672 of one token 70 us = 5.3 TB/s of the packed
-// bytes (the copy rate is 6.56), 16 tokens 94, 32 tokens 113, 64 tokens 158 (G = 64: 227, G = 32: 438); product 131072 x 4096,
-// 8 tokens 56 us; 4096 x 4096, one token 8.5 us, of which 7 are the life of a block from its start to its join. Up to 8
-// tokens HBM bounds it. Above, the accumulating warps do: two instructions per two (row, token) sums of a group, and the
-// trip of the sums through tensor memory (at 64 tokens 55 % of the issue slots, 40 % of the tensor pipe, 29 % of
+// bytes (the copy rate is 6.56), 8 tokens 81, 16 tokens 89, 32 tokens 109, 64 tokens 159 (G = 64: 227, G = 32: 438);
+// product 131072 x 4096, 8 tokens 56 us; 4096 x 4096, one token 8.5 us, of which 7 are the life of a block from its start to
+// its join. Of an MLP's time 16 us (one token) to 37 (32 tokens) do not grow with N: starts, joins and the terms. Up to 16
+// tokens HBM bounds the rest. Above, the accumulating warps do: two instructions per two (row, token) sums of a group,
+// and the trip of the sums through tensor memory (at 64 tokens 55 % of the issue slots, 40 % of the tensor pipe, 29 % of
 // HBM). Fetching a group's sums while those of the group before are worked on was slower (64 tokens: 164 us).
 #pragma once
 #include <cuda_fp8.h>
@@ -122,8 +123,7 @@ __device__ __forceinline__ float nan_max(float a, float b) { return (b > a || b 
 // the groups of a row padded to whole units of 256 columns (zeros there), and per token 2^-e (NaN where the token holds
 // a NaN or an infinity). A cluster of blocks per token: each takes a share of the token's half units (128 columns, 16
 // lanes of 8; a group is 4, 8 or 16 lanes), finds their largest value, and goes over them again with the token's. Bound by
-// latency (launch, two passes, the cluster's barrier): 7 us for 8 or 16 tokens, 8 to 10 for 64, cold and alone; as the
-// predecessor of a stream kernel about 5, since that one starts meanwhile.
+// latency (launch, two passes, the cluster's barrier), about 5 us before a stream kernel, which starts meanwhile.
 struct W4SplitArgs {
   const void* x;
   long long ldx;
@@ -135,7 +135,9 @@ struct W4SplitArgs {
   int dependent;
   MoeTable moe;
 };
-constexpr int W4_SPLIT_THREADS = 256;
+// 8 blocks of 512 threads: a thread's eight columns mostly are its only ones and stay in registers (MLP K=8192, N=28672,
+// 8 / 16 / 32 tokens: 81 / 89 / 109 us; blocks of 256 threads 85 / 93 / 113, of 1024 threads 81 / 88 / 117).
+constexpr int W4_SPLIT_THREADS = 512;
 constexpr int W4_SPLIT_CLUSTER = 8;
 
 template <typename T>
@@ -164,8 +166,10 @@ w4_split_kernel(const W4SplitArgs args) {
     if (live) load8(static_cast<const T*>(args.x) + (static_cast<long long>(a) * args.M + m) * args.ldx + col, v);
     return live;
   };
-  float amax = 0.f;
-  for (int item = lo + (tid >> 4); item < hi; item += W4_SPLIT_THREADS / 16) {
+  float kept[8];  // the first item's columns, mostly the only ones
+  const bool kept_live = load(lo + (tid >> 4), kept);
+  float amax = amax8(kept);
+  for (int item = lo + (tid >> 4) + W4_SPLIT_THREADS / 16; item < hi; item += W4_SPLIT_THREADS / 16) {
     float v[8];
     load(item, v);
     amax = nan_max(amax, amax8(v));
@@ -193,7 +197,13 @@ w4_split_kernel(const W4SplitArgs args) {
   for (int first = lo; first < hi; first += W4_SPLIT_THREADS / 16) {
     const int item = first + (tid >> 4);
     float v[8];
-    const bool live = load(item, v);
+    bool live = kept_live;
+    if (first == lo) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = kept[i];
+    } else {
+      live = load(item, v);
+    }
     uint2 code[TERMS];
     float sum = split_terms<TERMS>(v, ex, code);
     for (int o = 1; o < width; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
