@@ -967,6 +967,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
           rc.next(NC);
         }
         if (!ok) break;
+        __syncwarp();  // all lanes have read the unit's factors, scales and zeros
         if (lane == 0) mbar_arrive(xempty + 8 * rx.at);
         rx.next(NX);
         step(w);
