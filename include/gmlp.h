@@ -323,11 +323,10 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
  *          fastest where they are 16-byte aligned and rows is a multiple of 16. They are read in whole 16-byte
  *          blocks: up to 15 bytes before and behind an array may be read (never used), within its blocks.
  * The weights are never rounded: a group's products with the integers q are summed in fp32 and then take zero and scale.
- * Activations enter as sums of two (bf16) or three (fp16) e4m3 numbers under a power of two, which are off by at most
- * 2^-17 of the largest activation that shares the power: up to 4 tokens that of its token and group of columns, from 5
- * tokens on that of its token (in the down product of a mixture: of the token's hidden values of all experts). Those
- * within 2^-9 (bf16) or 2^-6 (fp16) of the largest are exact. (Where the largest is below 2^-113, which only bf16
- * reaches, they are off by up to 2^-130.) A NaN or infinite activation makes its token's outputs NaN,
+ * Activations enter as sums of three e5m2 numbers under a power of two. Those within 2^-23 (bf16) or 2^-20 (fp16) of the
+ * largest activation that shares the power are exact, smaller ones off by at most 2^-31 of it, which is less than sums in
+ * fp32 keep; it is shared by a token's group of columns up to 4 tokens and by a token from 5 on (in the down product of
+ * a mixture by the token's hidden values of all experts). A NaN or infinite activation makes its token's outputs NaN,
  * and no other token's. Scales have to be finite. Gate and up matrices both have zeros or both have none.
  *
  * gmlp_w4_linear: y[m,r] = sum_c x[m,c] w[r,c] (+ bias[r]) (+ residual[m,r]) for 1 <= M <= 64 and any rows >= 1; x

@@ -8,7 +8,7 @@ The bounds count, term by term,
   * 32-bit sums: each addition is off by at most 2^-23 of the sum of magnitudes S = sum |w| |x| so far (the tensor
     core may truncate, hence 2^-23 and not 2^-24); a sum of n columns in groups of G takes at most n / 16 steps of the
     matrix instruction (16 columns each, counted as 2 additions) and n / G of the group sums, and at most 32 joins;
-  * 4-bit products only: an activation enters as a sum of e4m3 numbers that is off by at most 2^-17 of the largest
+  * 4-bit products only: an activation enters as a sum of three e5m2 numbers that is off by at most 2^-31 of the largest
     activation of its token and group (up to 4 tokens), or of its token (a token's rows of all experts in the down
     projection of a mixture);
   * the gate activation in 32 bits: 2^-19 relative (exp and division of the fast kind, each below 2^-21), and
@@ -20,6 +20,7 @@ import torch
 from torch import Tensor
 
 SHIFTS = (0, 16, 4, 20, 8, 24, 12, 28)
+TERM_FLOOR = 2.0 ** -31
 
 
 def unpack(w4: Tensor, scale: Tensor, zero: Tensor | None) -> Tensor:
@@ -61,7 +62,7 @@ def product(x: Tensor, w: Tensor, group: int = 0, largest: Tensor | None = None)
         return v, (x.abs() @ w.abs().transpose(-1, -2)) * (steps * 2.0 ** -23)
     size = 4 * _largest(w, group)
     return v, (x.abs() @ size.transpose(-1, -2)) * (steps * 2.0 ** -23) + \
-        ((_block_largest(x, group) if largest is None else largest) @ w.abs().transpose(-1, -2)) * 2.0 ** -17
+        ((_block_largest(x, group) if largest is None else largest) @ size.transpose(-1, -2)) * TERM_FLOOR
 
 
 _ACTS = {
@@ -159,3 +160,60 @@ def check(got: Tensor, want: Tensor, bound: Tensor, what: str) -> None:
     worst = float(torch.nan_to_num(off, nan=float("inf")).max()) if off.numel() else 0.0
     assert worst <= 1.0, f"{what}: {worst:.3g} times the bound at {int(off.argmax())} ({float(got.flatten()[off.argmax()])} " \
                          f"for {float(want.flatten()[off.argmax()])})"
+
+
+# ------------------------------------------------------------------------------- root-mean-square error of 4-bit products --
+# The bounds above are worst cases and grow with the square of the columns: over thousands of columns they hide a product
+# of the wrong precision. These limits are for the root-mean-square error over a token's outputs and grow like the root.
+#
+# The output's own rounding is taken out of the way by a residual: with residual = -round(y) the kernel returns
+# y - round(y), whose rounding is off by eps / 2 of at most eps / 2 of y.
+def as_terms(x: Tensor, group: int, terms: int = 3) -> Tensor:
+    """The float64 values that stand for x in a 4-bit product: per block (see _block_largest) a power of two brings the
+    largest magnitude to [2^14, 2^15), and each term is the e5m2 rounding of what is left. CPU."""
+    block = _largest(x, group) if x.shape[0] <= 4 else x.abs().amax(-1, keepdim=True).expand_as(x)
+    e = 14 - torch.frexp(block)[1] + 1
+    up = torch.ldexp(torch.ones_like(x), torch.where(block > 0, e, torch.zeros_like(e)).clamp_max(120))
+    rest, total = x * up, torch.zeros_like(x)
+    for _ in range(terms):
+        t = rest.float().to(torch.float8_e5m2).double()
+        rest, total = rest - t, total + t
+    return total / up
+
+
+def rms(v: Tensor) -> Tensor:
+    """Of every token's (row's) values."""
+    return v.double().pow(2).mean(-1).sqrt()
+
+
+def product_rms_limit(x: Tensor, scale: Tensor, y: Tensor, extra: float = 0.0) -> Tensor:
+    """Largest root-mean-square error over a token's outputs y = x w^T (float64 x [M, cols], scale [groups, rows]).
+
+    A group's sum is made by up to 12 steps of the matrix instruction (128 columns, 32 a step, three terms), each off by at
+    most 2^-23 of the sum so far, all perhaps to the same side (a tensor core that truncates); the integers q are at most
+    15, and over inputs without a pattern the sum of q x is at most 15 |x_g| in the mean, |x_g| the length of the
+    group's activations. sx is a sum of up to 13 rounded steps (eight columns, five exchanges) times at most 15, and two
+    roundings apply it: 12 + 13 / 2 + 1 < 20 such steps, 300 * 2^-23 of scale |x_g|. Errors of different groups have nothing
+    to do with each other and add up like a root, and so do the roundings of the sums over groups: at most cols / group
+    + 34 of them, half of 2^-23 of y each. The terms are off by TERM_FLOOR of the largest activation, times 15 scale."""
+    groups, cols = scale.shape[-2], x.shape[-1]
+    s2 = scale.double().pow(2)
+    lengths = x.unflatten(-1, (groups, -1)).pow(2).sum(-1)
+    inner = 300 * 2.0 ** -23 * (lengths @ s2).mean(-1).sqrt()
+    floor = TERM_FLOOR * 15 * x.abs().amax(-1) * (s2.sum(0).mean() * (cols // groups)).sqrt()
+    return inner + floor + rms(y) * (2.0 ** -24 * (groups + 34) ** 0.5 + extra)
+
+
+def cancelling_residual(y: Tensor, dt: torch.dtype) -> Tensor:
+    return (-y).to(dt)
+
+
+def check_rms(got: Tensor, y: Tensor, residual: Tensor, limit: Tensor, dt: torch.dtype, what: str,
+              rows: Tensor | None = None) -> None:
+    """`got` = y + residual in `dt`, residual = cancelling_residual(y): root-mean-square error of every token (over the
+    outputs `rows`) against its limit and the rounding of what is left of y, eps / 2 of eps / 2 of it."""
+    left = y + residual.double()
+    err, y = got.double() - left, y if rows is None else y[:, rows]
+    off = rms(err if rows is None else err[:, rows]) / (limit + rms(y) * (torch.finfo(dt).eps ** 2 / 4))
+    worst = float(torch.nan_to_num(off, nan=float("inf")).max())
+    assert worst <= 1.0, f"{what}: root-mean-square error {worst:.3g} times its limit at token {int(off.argmax())}"

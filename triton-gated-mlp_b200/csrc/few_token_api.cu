@@ -52,16 +52,14 @@ static int check_group(int32_t group, int64_t cols) {
 struct W4Work {
   size_t t8_off, meta_off, row_off, total;
 };
-static size_t w4_t8_bytes(int64_t rows, int64_t cols, int dtype) {
-  return static_cast<size_t>(dtype == GMLP_BF16 ? w4_terms<__nv_bfloat16>() : w4_terms<__half>()) * rows * cols;
-}
+static size_t w4_t8_bytes(int64_t rows, int64_t cols) { return static_cast<size_t>(W4_TERMS) * rows * cols; }
 // K columns of x (M rows); N columns of h (active * M rows), N = 0 for a plain product
-static W4Work w4_work(int64_t M, int64_t K, int64_t N, int64_t active, int group, int dtype) {
+static W4Work w4_work(int64_t M, int64_t K, int64_t N, int64_t active, int group) {
   W4Work w;
   w.t8_off = align_up(static_cast<size_t>(active * M * N) * 2, 256);
   w.meta_off = w.row_off = w.total = std::max<size_t>(w.t8_off, 16);
   if (M <= W4_FUSED_TOKENS) return w;
-  w.meta_off = w.t8_off + align_up(std::max(w4_t8_bytes(M, K, dtype), w4_t8_bytes(active * M, N, dtype)), 256);
+  w.meta_off = w.t8_off + align_up(std::max(w4_t8_bytes(M, K), w4_t8_bytes(active * M, N)), 256);
   const int64_t k_units = (K + W4_UNIT_COLS - 1) / W4_UNIT_COLS, n_units = (N + W4_UNIT_COLS - 1) / W4_UNIT_COLS;
   w.row_off = w.meta_off + static_cast<size_t>(std::max(k_units, active * n_units)) * (W4_UNIT_COLS / group) * w4_mt(M) *
                                sizeof(float);
@@ -69,7 +67,7 @@ static W4Work w4_work(int64_t M, int64_t K, int64_t N, int64_t active, int group
   return w;
 }
 
-// Activations as e4m3 terms (see w4_stream.cuh).
+// Activations as e5m2 terms (see w4_stream.cuh).
 static int launch_split(int64_t M, int64_t R, int64_t cols, int64_t ldx, int group, int dtype, const void* x, char* work,
                         const W4Work& w, const MoeTable& moe, bool dependent, cudaStream_t stream) {
   W4SplitArgs a;
@@ -204,7 +202,7 @@ int gmlp_capture_id(void* stream, uint64_t* id) {
 size_t gmlp_w4_work_bytes(int64_t M, int64_t K, int64_t N, int32_t experts, int32_t group, int32_t dtype) {
   if (M <= 0 || M > FEW_MAX_TOKENS || K <= 0 || N < 0 || experts <= 0 || (group != 32 && group != 64 && group != 128))
     return 0;
-  return w4_work(M, K, N, experts, group, dtype).total;
+  return w4_work(M, K, N, experts, group).total;
 }
 
 int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t dtype, const void* x, int64_t ldx,
@@ -228,7 +226,7 @@ int gmlp_w4_linear(int64_t M, int64_t rows, int64_t cols, int32_t group, int32_t
   const FewLayout l = few_layout(rows, rows, 1, dev->sm_count);
   if (scratch_bytes < l.total)
     return fail(GMLP_ERR_SCRATCH, "scratch holds %zu bytes, %zu needed", scratch_bytes, l.total);
-  const W4Work ww = w4_work(M, cols, 0, 1, group, dtype);
+  const W4Work ww = w4_work(M, cols, 0, 1, group);
   if (work_bytes < ww.total) return fail(GMLP_ERR_SCRATCH, "work holds %zu bytes, %zu needed", work_bytes, ww.total);
   char* const wk = static_cast<char*>(work);
   char* const sc = static_cast<char*>(scratch);
@@ -281,7 +279,7 @@ static int mlp_w4(const gmlp_problem_t* p, int32_t group, int64_t experts, const
   const FewLayout l = few_layout(p->K, p->N, active, dev->sm_count);
   if (scratch_bytes < l.total)
     return fail(GMLP_ERR_SCRATCH, "scratch holds %zu bytes, %zu needed", scratch_bytes, l.total);
-  const W4Work ww = w4_work(p->M, p->K, p->N, active, group, p->dtype);
+  const W4Work ww = w4_work(p->M, p->K, p->N, active, group);
   if (work_bytes < ww.total) return fail(GMLP_ERR_SCRATCH, "work holds %zu bytes, %zu needed", work_bytes, ww.total);
   char* const wk = static_cast<char*>(work);
   char* const sc = static_cast<char*>(scratch);

@@ -82,7 +82,7 @@ struct W4Call {
 
 template <int MT, bool DUAL, typename T, int GSHIFT, bool FUSED>
 int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
-  using Conf = W4Conf<MT, w4_terms<T>(), GSHIFT, FUSED>;
+  using Conf = W4Conf<MT, GSHIFT, FUSED>;
   if (c.max_units > 0x7fffffffLL) return fail(GMLP_ERR_SHAPE, "the call has more than 2^31 units of work");
   W4Maps m;
   int rc;
@@ -90,7 +90,7 @@ int launch_w4_t(const DeviceInfo* dev, const W4Call& c) {
   m.w1 = m.w0;
   if (DUAL && (rc = encode_map(&m.w1, c.w1.q, c.cols / 2, c.experts * c.rows, c.cols / 2, 128, 128, DTYPE_U8))) return rc;
   m.x = m.w0;
-  if (!FUSED && (rc = encode_map(&m.x, c.t8, c.cols, w4_terms<T>() * c.R, c.cols, 128, MT, DTYPE_U8))) return rc;
+  if (!FUSED && (rc = encode_map(&m.x, c.t8, c.cols, W4_TERMS * c.R, c.cols, 128, MT, DTYPE_U8))) return rc;
   // Scales and zeros as TMA boxes of the unit's groups where their rows are aligned, else row by row in 16-byte blocks, one copy
   // for each (tile, group) and array. Device time, boxes against rows: 131072 x 4096, 8 tokens 56 against 61 us; K=8192,
   // N=28672 MLP of one token 70 against 72, of 64 tokens 164 against 175.

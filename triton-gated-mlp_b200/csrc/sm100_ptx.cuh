@@ -339,10 +339,10 @@ __host__ __device__ constexpr uint32_t make_idesc_tf32(int m, int n) {
   return (1u << 4) | (2u << 7) | (2u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
-// The same layout for tcgen05.mma.kind::f8f6f4 with both operands e4m3 (format code 0),
-// K-major, fp32 accumulate.
-__host__ __device__ constexpr uint32_t make_idesc_f8(int m, int n) {
-  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+// The same layout for tcgen05.mma.kind::f8f6f4, K-major, fp32 accumulate: A e4m3 (format code 0), B the given format.
+constexpr uint32_t FORMAT_E4M3 = 0, FORMAT_E5M2 = 1;
+__host__ __device__ constexpr uint32_t make_idesc_f8(int m, int n, uint32_t b_format = FORMAT_E4M3) {
+  return (1u << 4) | (b_format << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
 }  // namespace gmlp

@@ -8,18 +8,20 @@
 // 1. A nibble is an 8-bit float. The e4m3 codes 0..15 stand for 0, 1, .., 15 times 2^-9 (0..7 are the subnormals,
 //    8..15 the first binade, with the same spacing). So a packed word needs two masks and a shift to become eight
 //    operands of tcgen05.mma.kind::f8f6f4, exactly:  q 2^-9.
-// 2. An activation is a short sum of 8-bit floats. e4m3 has 4 significant bits, bf16 8, fp16 11: with a power of
-//    two that brings the largest value of a block of activations to [128, 256),
-//      x 2^e = t_1 + t_2 (bf16)   or   t_1 + t_2 + t_3 (fp16),   t_i the e4m3 rounding of what is left.
-//    That is exact for values within 2^-9 (bf16) or 2^-6 (fp16) of the block's largest; below, the error is at most
-//    2^-10 (half the spacing of e4m3's subnormals) where the largest is at least 2^7: 2^-17 of the block's largest
-//    value, 256 (bf16) or 32 (fp16) times less than that value's own half step.
+// 2. An activation is a short sum of 8-bit floats. e5m2 has 3 significant bits and each rounding to the nearest saves one
+//    more: three terms carry 3 + 4 + 4 = 11, as many as fp16 has (bf16: 8). With a power of two that brings the largest
+//    value of a block of activations to [2^14, 2^15),
+//      x 2^e = t_1 + t_2 + t_3,   t_i the e5m2 rounding of what is left.
+//    That is exact for values within 2^-23 (bf16) or 2^-20 (fp16) of the block's largest; below, the error is at most
+//    2^-17 (half the spacing of e5m2's subnormals) where the largest is at least 2^14: 2^-31 of the block's largest
+//    value, below what 32-bit sums keep. (e4m3 terms, two of them for bf16, have a floor of 2^-17 of the largest: with an
+//    activation of 16384 among normal ones, outputs that it does not reach were off by 8e-2.)
 //    The terms are MMAs into one accumulator (the tensor pipe has the time: an MMA of N <= 64 columns takes N / 2 clocks, at
 //    least 16, and the weights of one arrive every 89).
 //    The block: up to 4 tokens, a token and group (terms made inside the kernel, unit by unit); above, a whole token.
 // Per row r, token m:
 //   y[r][m] = sum_g 512 s[r][g] * ( acc[r][m]  -  z[r][g] * sx[m][g] ) * 2^-e,
-//   acc = sum_i sum_{c in g} (q[r][c] 2^-9) t_i[c][m],   sx = 2^-9 sum_{c in g} x[m][c] 2^e
+//   acc = sum_i sum_{c in g} (q[r][c] 2^-9) t_i[c][m],   sx = 2^-9 sum_{c in g} sum_i t_i[c][m]
 // with the scale, the zero point and the power of two applied in 32 bits when a group's sums leave tensor memory:
 // neither weights nor activations are rounded (but for the bound above), and that work is per token and group, not per
 // weight: three operations per token and group while 2^-e belongs to the group, two when it belongs to the token. That
@@ -63,40 +65,34 @@ constexpr int W4_UNIT_COLS = 256;
 constexpr int W4_HALF_COLS = 128;
 constexpr int W4_UNIT_CLOCKS = 1400;  // of one CTA, whether or not the others stream
 
-// Terms per activation.
-template <typename T>
-__host__ __device__ constexpr int w4_terms() {
-  return 2;
-}
-template <>
-__host__ __device__ constexpr int w4_terms<__half>() {
-  return 3;
-}
+constexpr int W4_TERMS = 3;  // per activation
 
 // ---- activations -> terms ----
-// The power of two, as an exponent, that brings `amax` to [128, 256); limited so that it and its inverse are normal numbers.
+// The power of two, as an exponent, that brings `amax` to [2^14, 2^15); limited so that it and its inverse are normal numbers.
 __device__ __forceinline__ int split_exponent(float amax) {
-  const int ex = 7 - (static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127);
+  const int ex = 14 - (static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127);
   return ex > 120 ? 120 : ex;
 }
+// What takes the power off again, 2^-e, is applied as 2^(13 - e) and the scales' 512 as 512 * 2^-13: both are then normal
+// numbers for every e, and sums of scale * acc stay finite for scales up to 2^106 over 2^16 columns.
+constexpr int W4_LIFT = 13;
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 // Eight columns of a lane times 2^ex: the terms' codes (bytes in the order in which the expanders' masks deliver a word's
 // nibbles: columns 0 4 1 5 | 2 6 3 7); returns the sum of the terms.
-template <int TERMS>
-__device__ __forceinline__ float split_terms(const float (&v)[8], int ex, uint2 (&codes)[TERMS]) {
+__device__ __forceinline__ float split_terms(const float (&v)[8], int ex, uint2 (&codes)[W4_TERMS]) {
   constexpr int PERM[8] = {0, 4, 1, 5, 2, 6, 3, 7};
   const float up = power_of_two(ex);
   float rest[8], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) rest[i] = v[i] * up;
 #pragma unroll
-  for (int t = 0; t < TERMS; ++t) {
+  for (int t = 0; t < W4_TERMS; ++t) {
     uint32_t pair[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int a = PERM[2 * i], b = PERM[2 * i + 1];
-      const __nv_fp8x2_storage_t c = __nv_cvt_float2_to_fp8x2(make_float2(rest[a], rest[b]), __NV_SATFINITE, __NV_E4M3);
-      const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(c, __NV_E4M3)));
+      const __nv_fp8x2_storage_t c = __nv_cvt_float2_to_fp8x2(make_float2(rest[a], rest[b]), __NV_SATFINITE, __NV_E5M2);
+      const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(c, __NV_E5M2)));
       rest[a] -= back.x;
       rest[b] -= back.y;
       sum += back.x + back.y;
@@ -119,9 +115,9 @@ __device__ __forceinline__ float amax8(const float (&v)[8]) {
 }
 __device__ __forceinline__ float nan_max(float a, float b) { return (b > a || b != b) ? b : a; }
 
-// x [active][M][cols] (row pitch ldx) -> t8 [TERMS][R][cols] e4m3 bytes, meta [active][groups][MT] floats 2^-9 sum_g x 2^e with
-// the groups of a row padded to whole units of 256 columns (zeros there), and per token 2^-e (NaN where the token holds
-// a NaN or an infinity). A cluster of blocks per token: each takes a share of the token's half units (128 columns, 16
+// x [active][M][cols] (row pitch ldx) -> t8 [W4_TERMS][R][cols] e5m2 bytes, meta [active][groups][MT] floats sx with
+// the groups of a row padded to whole units of 256 columns (zeros there), and per token 2^(13 - e) (NaN where the token
+// holds a NaN or an infinity). A cluster of blocks per token: each takes a share of the token's half units (128 columns, 16
 // lanes of 8; a group is 4, 8 or 16 lanes), finds their largest value, and goes over them again with the token's. Bound by
 // latency (launch, two passes, the cluster's barrier), about 5 us before a stream kernel, which starts meanwhile.
 struct W4SplitArgs {
@@ -143,7 +139,6 @@ constexpr int W4_SPLIT_CLUSTER = 8;
 template <typename T>
 __global__ void __launch_bounds__(W4_SPLIT_THREADS)
 w4_split_kernel(const W4SplitArgs args) {
-  constexpr int TERMS = w4_terms<T>();
   __shared__ MoeShared moe;
   __shared__ float warp_max[W4_SPLIT_THREADS / 32];
   __shared__ float block_max[W4_SPLIT_CLUSTER];
@@ -192,7 +187,7 @@ w4_split_kernel(const W4SplitArgs args) {
   for (int i = 1; i < W4_SPLIT_CLUSTER; ++i) amax = nan_max(amax, block_max[i]);
   const bool bad = amax != amax;
   const int ex = bad ? 0 : split_exponent(amax);
-  if (rank == 0 && tid == 0) args.rowscale[m] = bad ? amax : power_of_two(-ex);
+  if (rank == 0 && tid == 0) args.rowscale[m] = bad ? amax : power_of_two(W4_LIFT - ex);
   const int width = 4 << args.gshift;  // lanes per group
   for (int first = lo; first < hi; first += W4_SPLIT_THREADS / 16) {
     const int item = first + (tid >> 4);
@@ -204,15 +199,15 @@ w4_split_kernel(const W4SplitArgs args) {
     } else {
       live = load(item, v);
     }
-    uint2 code[TERMS];
-    float sum = split_terms<TERMS>(v, ex, code);
+    uint2 code[W4_TERMS];
+    float sum = split_terms(v, ex, code);
     for (int o = 1; o < width; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (item >= hi) continue;
     const int a = item / blocks, col = (item - a * blocks) * W4_HALF_COLS + sub * 8;
     if (live) {
       uint8_t* const p = args.t8 + (static_cast<long long>(a) * args.M + m) * args.cols + col;
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t) *reinterpret_cast<uint2*>(p + t * args.R * args.cols) = code[t];
+      for (int t = 0; t < W4_TERMS; ++t) *reinterpret_cast<uint2*>(p + t * args.R * args.cols) = code[t];
     }
     if ((sub & (width - 1)) == 0) {
       const long long g = static_cast<long long>(a) * (blocks * (4 >> args.gshift)) + (col >> (5 + args.gshift));
@@ -237,7 +232,7 @@ struct W4Args {
   int cols;
   int* status;
   const float* meta;       // not FUSED: [experts in h or 1][kbt * groups per unit][MT] sx
-  const float* rowscale;   // not FUSED: [M] 2^-e
+  const float* rowscale;   // not FUSED: [M] 2^(13 - e)
   const uint16_t* scale0;  // [experts][groups][rows], T
   const uint16_t* scale1;  // DUAL: the up matrix's
   const uint8_t* zero0;    // [experts][groups][rows] or null (8)
@@ -265,10 +260,14 @@ constexpr int W4_META_ZERO = 272;
 // token) pair in turn; a pair takes about 800 clocks, a unit's weights 1,400 to arrive, which carries four tokens (8
 // tokens, 28672 x 8192: 85 us, 73 with six such warps, against 50 with the terms made beforehand).
 constexpr int W4_FUSED_TOKENS = 4;
-template <int MT, int TERMS, int GSHIFT, bool FUSED>
+template <int MT, int GSHIFT, bool FUSED>
 struct W4Conf {
   static_assert(!FUSED || MT == 8, "one instantiation of each fused form");
-  static constexpr int N = MT < 16 ? 16 : MT;      // columns of the MMA; those behind MT hold nothing of use
+  // Up to 8 tokens the terms are columns of one MMA, which costs the same 16 clocks with 32 columns as with 16, and the
+  // accumulating warps add them up; above they are MMAs into one accumulator.
+  static constexpr bool STACKED = MT == 8;
+  static constexpr int TOK = FUSED ? W4_FUSED_TOKENS : MT;  // rows of a term
+  static constexpr int N = STACKED ? (W4_TERMS * TOK + 15) / 16 * 16 : MT;  // columns of the MMA
   // accumulating threads: four warps per share of the tokens; 64 tokens take sixteen warps (with eight, 64 sums a thread)
   static constexpr int SHARES = FUSED ? 1 : (MT == 64 ? 4 : 2);
   static constexpr int EPI = 128 * SHARES;
@@ -277,10 +276,12 @@ struct W4Conf {
   static constexpr int GPH = 4 >> GSHIFT;          // groups per half unit (128 columns)
   static constexpr int GPU = 2 * GPH;              // groups per unit
   static constexpr int FACTORS = FUSED ? 2 : 1;    // per token and group: 2^-e (FUSED) and sx
-  // activation terms of a unit: [two halves][TERMS] of N rows x 128 columns, then [GPU][FACTORS][MT] factors
-  static constexpr int X_TERM = N * 128;
-  static constexpr int X_HALF = TERMS * X_TERM;
+  // activation terms of a unit: [two halves][W4_TERMS] of TOK rows x 128 columns, then [GPU][FACTORS][MT] factors. (Columns
+  // of the MMA behind the last term are whatever lies there.)
+  static constexpr int X_TERM = TOK * 128;
+  static constexpr int X_HALF = (W4_TERMS * X_TERM + 1023) / 1024 * 1024;
   static constexpr int X_STAGE = (2 * X_HALF + GPU * FACTORS * MT * 4 + 1023) / 1024 * 1024;
+  static_assert(X_STAGE >= X_HALF + N * 128, "the MMA reads N rows of the second half");
   static constexpr int M_STAGE = 2 * GPU * W4_META_ROW;  // scales and zeros of a unit as they lie in memory
   static constexpr int S_STAGE = 2 * GPU * 128 * 4;      // and as a word per row: scale << 16 | zero
   static constexpr int SIDE = X_STAGE + M_STAGE + S_STAGE;
@@ -320,7 +321,7 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// D[tmem] (+)= A[tmem] * B[smem], e4m3: A is 128 lanes x 8 columns, four elements a column (32 of the reduction).
+// D[tmem] (+)= A[tmem] * B[smem], 8-bit floats: A is 128 lanes x 8 columns, four elements a column (32 of the reduction).
 __device__ __forceinline__ void umma_f8_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
                                            uint32_t accumulate) {
   asm volatile(
@@ -400,10 +401,10 @@ struct W4Walk {
 };
 
 template <int MT, bool DUAL, typename T, int GSHIFT, bool FUSED>
-__global__ void __launch_bounds__(W4Conf<MT, w4_terms<T>(), GSHIFT, FUSED>::THREADS, 1)
+__global__ void __launch_bounds__(W4Conf<MT, GSHIFT, FUSED>::THREADS, 1)
 w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
-  constexpr int TERMS = w4_terms<T>();
-  using C = W4Conf<MT, TERMS, GSHIFT, FUSED>;
+  constexpr int TERMS = W4_TERMS;
+  using C = W4Conf<MT, GSHIFT, FUSED>;
   constexpr int N = C::N;
   constexpr int NW = C::W_STAGES, NX = C::X_STAGES, NA = C::A_BUFS, NC = C::C_BUFS;
   constexpr int GPH = C::GPH, GPU = C::GPU, PAIRS = C::PAIRS, BUF_PAIRS = C::BUF_PAIRS;
@@ -581,7 +582,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
         if (!FUSED) {
 #pragma unroll
           for (int i = 0; i < 2 * TERMS; ++i)  // a half behind the last column arrives as zeros
-            tma_load_2d_hint(dst + i * C::X_TERM, &maps.x, fb, w.kb * W4_UNIT_COLS + (i / TERMS) * W4_HALF_COLS,
+            tma_load_2d_hint(dst + i / TERMS * C::X_HALF + i % TERMS * C::X_TERM, &maps.x, fb, w.kb * W4_UNIT_COLS + (i / TERMS) * W4_HALF_COLS,
                              static_cast<int>((i % TERMS) * args.R) + a * args.M, pol);
           bulk_load(dst + 2 * C::X_HALF, args.meta + (static_cast<long long>(a) * args.kbt + w.kb) * (GPU * MT),
                     META_BYTES, fb);
@@ -655,7 +656,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA --
     if (MT == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    constexpr uint32_t IDESC = make_idesc_f8(128, N);
+    constexpr uint32_t IDESC = make_idesc_f8(128, N, FORMAT_E5M2);
     const uint64_t x0 = make_smem_desc(x_base, 16, 1024);
     Ring rx, ra, rc;
     bool ok = true;
@@ -678,9 +679,9 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
             for (int k = 0; k < KSTEPS; ++k) {
               const int kk = g * KSTEPS + k;  // 32-column step inside the half
 #pragma unroll
-              for (int i = 0; i < TERMS; ++i)
+              for (int i = 0; i < (C::STACKED ? 1 : TERMS); ++i)
                 umma_f8_ts(d + (p - p0) * N, a0 + t * 64 + h * 32 + kk * 8,
-                           xd + static_cast<uint64_t>(((h * TERMS + i) * C::X_TERM >> 4) + 2 * kk), IDESC,
+                           xd + static_cast<uint64_t>(((h * C::X_HALF + i * C::X_TERM) >> 4) + 2 * kk), IDESC,
                            k + i > 0 ? 1u : 0u);
             }
           }
@@ -801,17 +802,19 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
       for (int o = 1; o < WIDTH; o <<= 1) amax = nan_max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       const int ex = amax != amax ? 0 : split_exponent(amax);
       uint2 code[TERMS];
-      float sum = split_terms<TERMS>(v, ex, code);
+      float sum = split_terms(v, ex, code);
 #pragma unroll
       for (int o = 1; o < WIDTH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float down = amax != amax ? amax : power_of_two(-ex);
+      const float down = amax != amax ? amax : power_of_two(W4_LIFT - ex);
       ok = quick_wait(xempty + 8 * r.at, r.phase ^ 1u, abortp);
       if (!ok) break;
       uint8_t* const xs = smem + NW * 2 * W4_TILE_BYTES + r.at * C::X_STAGE;
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t)
-        *reinterpret_cast<uint2*>(xs + (half * TERMS + t) * C::X_TERM + m * 128 + (((sub >> 1) ^ (m & 7)) << 4) +
-                                  (sub & 1) * 8) = code[t];
+      for (int t = 0; t < TERMS; ++t) {
+        const int xr = t * C::TOK + m;
+        *reinterpret_cast<uint2*>(xs + half * C::X_HALF + xr * 128 + (((sub >> 1) ^ (xr & 7)) << 4) + (sub & 1) * 8) =
+            code[t];
+      }
       if ((sub & (WIDTH - 1)) == 0) {
         float* const mt = reinterpret_cast<float*>(xs + 2 * C::X_HALF) + (half * GPH + sub / WIDTH) * 2 * MT + m;
         mt[0] = down;
@@ -832,7 +835,8 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
     constexpr int CH = COLS < 16 ? COLS : 16;  // token columns per round of tensor-memory loads
     constexpr int GROUPS = BUF_PAIRS / 2;      // groups in a buffer, both tiles' sums each
     // sums in flight at a time: as many as 32 registers hold
-    constexpr int BATCH = BUF_PAIRS * CH <= 32 ? BUF_PAIRS : 32 / CH;
+    constexpr int LOADS = C::STACKED ? TERMS : 1;
+    constexpr int BATCH = BUF_PAIRS * CH * LOADS <= 32 ? BUF_PAIRS : 32 / (CH * LOADS);
     const int quarter = warp & 3;
     const int col0 = ((warp - 12) >> 2) * COLS;
     const bool idle = col0 >= args.M;  // no tokens in these columns
@@ -907,7 +911,7 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
 #pragma unroll
           for (int b = 0; b < BUF_PAIRS; ++b) {
             const uint32_t sz = ss[((b & 1) * GPU + g0 + (b >> 1)) * 128];
-            sc[b] = 512.0f * Pack2<T>::unpack(sz >> 16).x;
+            sc[b] = (512.0f / (1 << W4_LIFT)) * Pack2<T>::unpack(sz >> 16).x;
             // an integer below 2^23 in a float's fraction: 2^23 - (2^23 + z)
             nz[b] = 8388608.0f - __uint_as_float(0x4B000000u | (sz & 15u));
           }
@@ -918,10 +922,14 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
           for (int b0 = 0; b0 < BUF_PAIRS; b0 += BATCH) {
 #pragma unroll
             for (int c = 0; c < COLS; c += CH) {
-              uint32_t x[BATCH][CH];
+              uint32_t x[BATCH][CH], more[BATCH][LOADS][CH];
               if (!idle) {
 #pragma unroll
-                for (int b = 0; b < BATCH; ++b) tmem_ld_cols<CH>(src + (b0 + b) * N + c, x[b]);
+                for (int b = 0; b < BATCH; ++b) {
+                  tmem_ld_cols<CH>(src + (b0 + b) * N + c, x[b]);
+#pragma unroll
+                  for (int i = 1; i < LOADS; ++i) tmem_ld_cols<CH>(src + (b0 + b) * N + i * C::TOK + c, more[b][i]);
+                }
                 tmem_ld_wait();
               }
               if (b0 + BATCH == BUF_PAIRS && c + CH == COLS) {  // the last sums are in registers
@@ -930,6 +938,17 @@ w4_stream_kernel(const __grid_constant__ W4Maps maps, const W4Args args) {
                 if (lane == 0) mbar_arrive(cempty + 8 * rc.at);
               }
               if (!idle) {
+                if constexpr (C::STACKED) {  // the terms' sums, the smallest first
+#pragma unroll
+                  for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+                    for (int k = 0; k < CH; ++k) {
+                      float sum = __uint_as_float(more[b][LOADS - 1][k]);
+#pragma unroll
+                      for (int i = LOADS - 2; i > 0; --i) sum += __uint_as_float(more[b][i][k]);
+                      x[b][k] = __float_as_uint(__uint_as_float(x[b][k]) + sum);
+                    }
+                }
 #pragma unroll
                 for (int k = 0; k < CH; k += 4) {
 #pragma unroll

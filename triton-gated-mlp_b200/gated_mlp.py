@@ -352,8 +352,8 @@ class FusedGatedMLP(nn.Module):
         """Prepare (or drop) narrow copies of the three weight matrices for the decode path (inference with at most
         64 tokens). bits=8: e4m3 with one scale per weight row, half the weight bytes (activations are quantised per
         token on the fly); needs hidden and intermediate sizes that are multiples of 128. bits=4: nibbles with one
-        scale and zero point per `group_size` (32, 64 or 128) columns, about a quarter of the bytes (activations keep
-        their 16-bit accuracy); needs hidden and intermediate sizes that are multiples of the group size. Everything
+        scale and zero point per `group_size` (32, 64 or 128) columns, about a quarter of the bytes (activations enter
+        exactly, or off by 2^-31 of the largest of their token); needs hidden and intermediate sizes that are multiples of the group size. Everything
         else stays 16-bit. Call again after the weights change. Not combined with an attached input norm or tensor
         parallelism."""
         if bits not in (4, 8):
