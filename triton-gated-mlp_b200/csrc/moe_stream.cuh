@@ -393,7 +393,7 @@ moe_route_kernel(const RouteArgs args) {
     const int e = i * 32 + lane;
     const double l = e < args.E ? logits[e] : 0.0;
     key[i] = e < args.E ? sort_key(l, e) : 0ull;
-    if (e < args.E && !(l <= top)) top = l;  // a NaN becomes the maximum and makes every weight of the token NaN
+    if (e < args.E && (l > top || l != l)) top = l;  // a NaN stays the maximum and makes every weight of the token NaN
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
