@@ -335,8 +335,8 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
  * Both start streaming weights before the preceding kernel on the stream has finished, with the precondition and
  * the GMLP_TUNE_ORDINARY_LAUNCH way out of gmlp_decode_fwd.
  *
- * gmlp_moe_route: the router. logits = x w_router^T ([experts, K]); per token ids[M, top_k] = the experts of the top_k
- *   largest logits in descending order (equal ones: lower index first; a NaN ranks below every number, so the ids
+ * gmlp_moe_route: the router. logits = x w_router^T ([experts, K]), exact products summed in fp64; per token ids[M, top_k] = the experts of the top_k
+ *   largest logits in descending order (equal ones, to within 2^-43 of them: lower index first; a NaN ranks below every number, so the ids
  *   are valid and distinct whatever x holds), weights[M, top_k] = softmax over all experts at those ids,
  *   divided by their sum if `renormalize`. experts <= 512, top_k <= min(32, experts), any M.
  * gmlp_moe_decode_fwd: y[t] = sum_j weights[t,j] * MLP_{ids[t,j]}(x[t]) (+ residual[t]) with

@@ -140,11 +140,12 @@ static int launch_moe(int mpad, int dtype, const DeviceInfo* dev, Args... args) 
             : launch_moe_t<64, DUAL, __half>(dev, dtype, args...);
 }
 
-template <typename T>
-static int launch_route(const RouteArgs& a, unsigned grid, int cluster, cudaStream_t st) {
-  if (a.E <= 32) return launch_few(moe_route_kernel<T, 1>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
-  if (a.E <= 128) return launch_few(moe_route_kernel<T, 4>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
-  return launch_few(moe_route_kernel<T, 16>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
+template <typename T, int TOKENS>
+static int launch_route(const RouteArgs& a, int cluster, cudaStream_t st) {
+  const unsigned grid = static_cast<unsigned>((a.M + TOKENS - 1) / TOKENS * cluster);
+  if (a.E <= 32) return launch_few(moe_route_kernel<T, 1, TOKENS>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
+  if (a.E <= 128) return launch_few(moe_route_kernel<T, 4, TOKENS>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
+  return launch_few(moe_route_kernel<T, 16, TOKENS>, grid, ROUTE_THREADS, 0, true, st, a, cluster);
 }
 
 static int check_few(const gmlp_problem_t* p, const char* what) {
@@ -415,18 +416,26 @@ int gmlp_moe_route(int64_t M, int64_t K, int32_t experts, int32_t top_k, int32_t
   a.x = x;
   a.w = w_router;
   a.ldx = ldx;
+  a.M = static_cast<int>(M);
   a.K = static_cast<int>(K);
   a.E = experts;
   a.top_k = top_k;
   a.renormalize = renormalize ? 1 : 0;
   a.ids = ids;
   a.weights = weights;
-  // a warp takes two experts at a time; up to eight blocks a token
+  // A warp takes two experts at a time, or one where there are SMs for it (32 experts x 4096, 32 tokens: 6.7 us against 7.4);
+  // up to eight blocks a token.
   int cluster = 1;
-  while (cluster < 8 && cluster * 2 * (ROUTE_THREADS / 32) < experts) cluster *= 2;
-  const unsigned grid = static_cast<unsigned>(M * cluster);
+  while (cluster < 8 && (cluster * 2 * (ROUTE_THREADS / 32) < experts ||
+                         (cluster * (ROUTE_THREADS / 32) < experts && M * cluster * 2 <= dev->sm_count)))
+    cluster *= 2;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == GMLP_BF16 ? launch_route<__nv_bfloat16>(a, grid, cluster, st) : launch_route<__half>(a, grid, cluster, st);
+  const bool bf = dtype == GMLP_BF16;
+  // Two tokens a cluster where there are enough blocks either way (2048 tokens, 128 x 2048: 175 us against 229 with one; 64
+  // tokens, 512 x 4096, three to four blocks an SM: 74 against 57).
+  if (M * cluster > 8 * dev->sm_count)
+    return bf ? launch_route<__nv_bfloat16, 2>(a, cluster, st) : launch_route<__half, 2>(a, cluster, st);
+  return bf ? launch_route<__nv_bfloat16, 1>(a, cluster, st) : launch_route<__half, 1>(a, cluster, st);
 }
 
 }  // extern "C"

@@ -314,16 +314,20 @@ moe_stream_kernel(const __grid_constant__ MoeMaps maps, const MoeArgs args) {
 // ---- router ----
 // logits l[t][e] = x_t . Wr_e; p = softmax(l); the top_k largest (equal ones: lowest index first; NaN ranks lowest) with
 // weights p, or p divided by their sum. A cluster of C blocks per token: each warp takes two experts
-// a pass, products exact in fp32, eight of them summed in fp32 and added to an fp64 sum, so that the order of the
-// logits (a choice next to a border) is that of the exact sums but for a relative 1e-7. The logits go to the first
-// block's shared memory (distributed shared memory), whose first warp selects. Latency-bound: C spreads the 2 E K bytes
-// of a token over SMs. Measured: 8 experts x 4096, one token 4.4 us; 64 x 2048, 64 tokens 5.2; 512 x 4096, 64 tokens 32.
+// a pass, products exact and summed in fp64: a logit is off by at most K 2^-53 of sum |x_k w_k|, however much of it
+// cancels, so that a choice next to a border is that of the exact sums. (Eight products summed in fp32 at a time are off by
+// some 2^-24 of sum |x_k w_k|: four channels of 3e4 that cancel turned choices over and moved weights by 6e-3. That took
+// 4.4, 5.2 and 32 us for the cases below; products converted one by one instead of widened: 6.0, 8.6 and 62.) The
+// logits go to the first block's shared memory (distributed shared memory), whose first warp selects. Latency-bound where
+// tokens are few: C spreads the 2 E K bytes of a token over SMs.
+// Measured: 8 experts x 4096, one token 4.2 us; 64 x 2048, 64 tokens 7.5; 512 x 4096, 64 tokens 57; 128 x 2048,
+// 2048 tokens 174.
 constexpr int ROUTE_THREADS = 256;
 struct RouteArgs {
   const void* x;
   const void* w;
   long long ldx;
-  int K, E, top_k, renormalize;
+  int M, K, E, top_k, renormalize;
   int* ids;
   float* weights;
 };
@@ -335,56 +339,128 @@ __device__ __forceinline__ unsigned long long sort_key(double v, int e) {
   if (v != v) b = 0x0008000000000000ull;  // below the key of -inf, above that of a removed entry (0)
   return (b & ~511ull) | static_cast<unsigned long long>(511 - e);
 }
-// PER: experts per lane of the selecting warp.
-template <typename T, int PER>
+// A 16-bit value (as the float it was converted to) times 2^-896, exactly, subnormals too: its exponent and fraction bits moved to
+// a double's place, with the exponent's bias left as it is. Not for infinities and NaNs.
+constexpr double WIDENED = 0x1p896;
+__device__ __forceinline__ double widened(float v) {
+  return __hiloint2double((__float_as_int(v) >> 3) & static_cast<int>(0x8fffffffu), 0);
+}
+// A lane's columns of TOKENS x EXPERTS dot products in CHAINS sums each. FAST: the weights widened; `finite` is
+// 0 times every weight, a NaN if one is not finite.
+template <bool FAST, int CHAINS, int TOKENS, int EXPERTS, typename T>
+__device__ __forceinline__ void route_columns(const T* const (&x)[TOKENS], const T* const (&w)[EXPERTS], int K, int lane,
+                                              double (&s)[TOKENS][EXPERTS], f32x2& finite) {
+  double t[CHAINS][TOKENS][EXPERTS];
+#pragma unroll
+  for (int c = 0; c < CHAINS; ++c)
+#pragma unroll
+    for (int m = 0; m < TOKENS; ++m)
+#pragma unroll
+      for (int e = 0; e < EXPERTS; ++e) t[c][m][e] = 0.0;
+  constexpr int UNROLL = !FAST ? 1 : TOKENS == 1 ? 4 : 2;
+#pragma unroll UNROLL
+  for (int k = lane * 8; k < K; k += 256) {
+    float a[TOKENS][8], b[EXPERTS][8];
+#pragma unroll
+    for (int m = 0; m < TOKENS; ++m) load8(x[m] + k, a[m]);
+#pragma unroll
+    for (int e = 0; e < EXPERTS; ++e) load8(w[e] + k, b[e]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < EXPERTS; ++e) {
+        const double u = FAST ? widened(b[e][i]) : b[e][i];
+#pragma unroll
+        for (int m = 0; m < TOKENS; ++m) t[i % CHAINS][m][e] = fma(static_cast<double>(a[m][i]), u, t[i % CHAINS][m][e]);
+        if (FAST && i % 2 == 0) finite = f2_fma(f2_pack(b[e][i], b[e][i + 1]), 0ull, finite);
+      }
+  }
+#pragma unroll
+  for (int m = 0; m < TOKENS; ++m)
+#pragma unroll
+    for (int e = 0; e < EXPERTS; ++e) {
+      double v = t[0][m][e] + t[1][m][e];
+      if (CHAINS == 4) v += t[CHAINS - 2][m][e] + t[CHAINS - 1][m][e];
+      s[m][e] = FAST ? v * WIDENED : v;
+    }
+}
+// Widened products underflow below 2^-178, and infinities and NaNs cannot be widened: a sum that this can have touched (by
+// more than 2^-47 of it) is made again with converted weights. The same additions in the same order: equal rows have
+// equal sums.
+template <int CHAINS, int TOKENS, int EXPERTS, typename T>
+__device__ __forceinline__ void route_dots(const T* const (&x)[TOKENS], const T* const (&w)[EXPERTS], int K, int lane,
+                                           double (&s)[TOKENS][EXPERTS]) {
+  f32x2 finite = 0ull;
+  route_columns<true, CHAINS, TOKENS, EXPERTS>(x, w, K, lane, s, finite);
+  float z0, z1;
+  f2_unpack(finite, z0, z1);
+  bool again = z0 + z1 != 0.f;
+#pragma unroll
+  for (int m = 0; m < TOKENS; ++m) {
+    bool small = false;
+#pragma unroll
+    for (int e = 0; e < EXPERTS; ++e) small |= fabs(s[m][e]) < 0x1p-100;
+    if (small)  // unless x is zero there: a row of padding
+      for (int k = lane * 8; k < K && !again; k += 256) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x[m] + k);
+        again = ((v.x | v.y | v.z | v.w) & 0x7fff7fffu) != 0u;
+      }
+  }
+  if (__any_sync(0xffffffffu, again)) route_columns<false, CHAINS, TOKENS, EXPERTS>(x, w, K, lane, s, finite);
+}
+// PER: experts per lane of the selecting warp. TOKENS: tokens of a cluster, which share the loads and the widening of the
+// router's rows.
+// Four sums a product where latency counts, two where more blocks per SM do (64 tokens: 64 x 2048 7.4 us with four, 8.2
+// with two; 512 x 4096 73 and 57).
+template <typename T, int PER, int TOKENS>
 __global__ void __launch_bounds__(ROUTE_THREADS)
 moe_route_kernel(const RouteArgs args) {
-  __shared__ double logits[32 * PER];
+  constexpr int CHAINS = TOKENS == 1 && PER <= 4 ? 4 : 2;
+  __shared__ double shared_logits[TOKENS][32 * PER];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t rank, size;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
-  const unsigned token = blockIdx.x / size;
+  const int first = static_cast<int>(blockIdx.x / size) * TOKENS;
   pdl_launch_dependents();
   cluster_sync_all();  // the first block's shared memory is written below: it has to be there
   pdl_wait();
-  const T* const x = static_cast<const T*>(args.x) + token * args.ldx;
-  const uint32_t dst0 = mapa_shared(smem_u32(logits), 0);
+  const T* x[TOKENS];
+#pragma unroll
+  for (int m = 0; m < TOKENS; ++m)  // (a token behind the last one is the last one again)
+    x[m] = static_cast<const T*>(args.x) + (first + m < args.M ? first + m : args.M - 1) * args.ldx;
+  const uint32_t dst0 = mapa_shared(smem_u32(shared_logits), 0);
   // experts warp-major over the cluster, two at a time: they share the loads of x
   const int warps = size * (ROUTE_THREADS / 32);
+  auto put = [&](double v, int m, int e) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst0 + 8u * (m * 32 * PER + e)), "d"(v) : "memory");
+  };
   for (int e = rank * (ROUTE_THREADS / 32) + warp; e < args.E; e += 2 * warps) {
-    const bool two = e + warps < args.E;
     const T* const w0 = static_cast<const T*>(args.w) + static_cast<long long>(e) * args.K;
-    const T* const w1 = two ? w0 + static_cast<long long>(warps) * args.K : w0;
-    double s0 = 0.0, s1 = 0.0;
-#pragma unroll 4
-    for (int k = lane * 8; k < args.K; k += 256) {
-      float a[8], b[8], c[8];
-      load8(x + k, a);
-      load8(w0 + k, b);
-      load8(w1 + k, c);
-      float p = a[0] * b[0], q = a[0] * c[0];
+    if (e + warps < args.E) {
+      const T* const w[2] = {w0, w0 + static_cast<long long>(warps) * args.K};
+      double s[TOKENS][2];
+      route_dots<CHAINS, TOKENS, 2>(x, w, args.K, lane, s);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) {
-        p = fmaf(a[i], b[i], p);
-        q = fmaf(a[i], c[i], q);
+      for (int m = 0; m < TOKENS; ++m) {
+        put(s[m][0], m, e);
+        put(s[m][1], m, e + warps);
       }
-      s0 += static_cast<double>(p);
-      s1 += static_cast<double>(q);
-    }
+    } else {
+      const T* const w[1] = {w0};
+      double s[TOKENS][1];
+      route_dots<CHAINS, TOKENS, 1>(x, w, args.K, lane, s);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-    }
-    if (lane == 0) {
-      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst0 + 8u * e), "d"(s0) : "memory");
-      if (two) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst0 + 8u * (e + warps)), "d"(s1) : "memory");
+      for (int m = 0; m < TOKENS; ++m) put(s[m][0], m, e);
     }
   }
   __syncwarp();
   cluster_sync_all();
-  if (rank != 0 || warp != 0) return;
+  const int token = first + warp;  // of the first block, a warp for each token
+  if (rank != 0 || warp >= TOKENS || token >= args.M) return;
+  const double* const logits = shared_logits[warp];
   unsigned long long key[PER];
   float ex[PER];
   double top = -INFINITY;
