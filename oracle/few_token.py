@@ -168,10 +168,10 @@ def check(got: Tensor, want: Tensor, bound: Tensor, what: str) -> None:
 #
 # The output's own rounding is taken out of the way by a residual: with residual = -round(y) the kernel returns
 # y - round(y), whose rounding is off by eps / 2 of at most eps / 2 of y.
-def as_terms(x: Tensor, group: int, terms: int = 3) -> Tensor:
-    """The float64 values that stand for x in a 4-bit product: per block (see _block_largest) a power of two brings the
-    largest magnitude to [2^14, 2^15), and each term is the e5m2 rounding of what is left. CPU."""
-    block = _largest(x, group) if x.shape[0] <= 4 else x.abs().amax(-1, keepdim=True).expand_as(x)
+def as_terms(x: Tensor, group: int, terms: int = 3, largest: Tensor | None = None) -> Tensor:
+    """The float64 values that stand for x in a 4-bit product: per block (see _block_largest; `largest` where it is wider)
+    a power of two brings the largest magnitude to [2^14, 2^15), and each term is the e5m2 rounding of what is left. CPU."""
+    block = _block_largest(x, group) if largest is None else largest.expand_as(x)
     e = 14 - torch.frexp(block)[1] + 1
     up = torch.ldexp(torch.ones_like(x), torch.where(block > 0, e, torch.zeros_like(e)).clamp_max(120))
     rest, total = x * up, torch.zeros_like(x)
@@ -202,6 +202,55 @@ def product_rms_limit(x: Tensor, scale: Tensor, y: Tensor, extra: float = 0.0) -
     inner = 300 * 2.0 ** -23 * (lengths @ s2).mean(-1).sqrt()
     floor = TERM_FLOOR * 15 * x.abs().amax(-1) * (s2.sum(0).mean() * (cols // groups)).sqrt()
     return inner + floor + rms(y) * (2.0 ** -24 * (groups + 34) ** 0.5 + extra)
+
+
+def hidden_rounded(x: Tensor, wg: Tensor, sg: Tensor, bg, wu: Tensor, su: Tensor, bu, act: str, dt: torch.dtype,
+                   f: Tensor | None = None):
+    """The hidden state of a 4-bit MLP as the kernel rounds it between its halves (times f), and the variance of what the
+    errors d before that rounding make of it: a value changes its rounding with a probability of at most d / step, by a
+    step (and by d where that is larger): d (step + d). d: the products' root-mean-square limits through the activation
+    (slope at most 1.13), and 2^-18 of the value for the activation itself and the products around it."""
+    g, u = x @ wg.t(), x @ wu.t()
+    dg, du = product_rms_limit(x, sg, g)[:, None], product_rms_limit(x, su, u)[:, None]
+    g = g if bg is None else g + bg.double()
+    u = u if bu is None else u + bu.double()
+    a = _ACTS[act](g)
+    h = a * u
+    d = 1.13 * dg * u.abs() + a.abs() * du + h.abs() * 2.0 ** -18
+    if f is not None:
+        h, d = h * f, d * f.abs()
+    info = torch.finfo(dt)
+    return h.to(dt).double(), d * (h.abs() * info.eps + info.smallest_normal * info.eps + d)
+
+
+def mlp_rms(x, wg, sg, bg, wu, su, bu, wd, sd, bd, dt, act="silu"):
+    """(y, limit) of decode_fwd_w4 without a residual: weights in float64, scales as they are stored."""
+    h, var = hidden_rounded(x.double(), wg, sg, bg, wu, su, bu, act, dt)
+    y = h @ wd.t()
+    limit = product_rms_limit(h, sd, y) + (var @ wd.pow(2).t()).mean(-1).sqrt()
+    return (y if bd is None else y + bd.double()), limit + (0 if bd is None else rms(bd[None]) * 2.0 ** -23)
+
+
+def moe_rms(x, ids, weights, wg, sg, wu, su, wd, sd, dt, act="silu"):
+    """(y, limit) of moe_decode_fwd_w4 without a residual, every id valid and once in its token."""
+    x, weights, T, E = x.double(), weights.double(), x.shape[0], wg.shape[0]
+    top = weights.abs().amax(1, keepdim=True)
+    parts, largest = [], torch.zeros((T, 1), dtype=torch.float64, device=x.device)
+    for e in range(E):
+        t, place = torch.nonzero(ids == e, as_tuple=True)
+        if len(t):
+            h, var = hidden_rounded(x[t], wg[e], sg[e], None, wu[e], su[e], None, act, dt, weights[t, place][:, None] / top[t])
+            largest[t] = torch.maximum(largest[t], h.abs().amax(1, keepdim=True))
+            parts.append((e, t, h, var))
+    y, square = torch.zeros_like(x), torch.zeros(T, dtype=torch.float64, device=x.device)
+    for e, t, h, var in parts:   # errors of different experts add up like a root; the floor is that of the token's largest
+        part = h @ wd[e].t()
+        y[t] += top[t] * part
+        widest = TERM_FLOOR * 15 * largest[t, 0] * (sd[e].double().pow(2).sum(0).mean() * (h.shape[1] // sd.shape[-2])).sqrt()
+        own = product_rms_limit(h, sd[e], part) + widest
+        square[t] += top[t, 0].pow(2) * (own.pow(2) + (var @ wd[e].pow(2).t()).mean(-1))
+    groups = len(parts) * sd.shape[-2]
+    return y, square.sqrt() + rms(y) * 2.0 ** -24 * (groups + 34) ** 0.5
 
 
 def cancelling_residual(y: Tensor, dt: torch.dtype) -> Tensor:

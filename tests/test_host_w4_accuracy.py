@@ -50,3 +50,54 @@ def test_limits_tell_three_terms_from_two(pkg, M, dt, group, outlier):
         elif outlier <= 1024:
             with pytest.raises(AssertionError, match="root-mean-square"):
                 ft.check_rms(got, y, res, limit, dt, "two terms", rows)
+
+
+def _restated_mlp(x, wg, wu, wd, act, dt, group, terms):
+    """decode_fwd_w4 with sums in 64 bits and activations of so many terms."""
+    a = ft.as_terms(x, group, terms)
+    h = (ft._ACTS[act](a @ wg.t()) * (a @ wu.t())).to(dt).double()
+    return ft.as_terms(h, group, terms) @ wd.t()
+
+
+@pytest.mark.parametrize("M,dt,group", [(3, BF, 128), (17, FP, 32), (64, BF, 64), (9, FP, 128)])
+def test_mlp_limits_tell_three_terms_from_two(pkg, M, dt, group):
+    g = torch.Generator().manual_seed(M)
+    K, N = 512, 896
+    (qg, wg), (qu, wu), (qd, wd) = (_w4(pkg, g, *s, group, dt) for s in ((N, K), (N, K), (K, N)))
+    x = torch.randn((M, K), generator=g).to(dt).double()
+    y, limit = ft.mlp_rms(x, wg, qg.scale, None, wu, qu.scale, None, wd, qd.scale, None, dt)
+    res = ft.cancelling_residual(y, dt)
+    ft.check_rms((_restated_mlp(x, wg, wu, wd, "silu", dt, group, 3) + res.double()).to(dt), y, res, limit, dt, "three")
+    with pytest.raises(AssertionError, match="root-mean-square"):
+        ft.check_rms((_restated_mlp(x, wg, wu, wd, "silu", dt, group, 2) + res.double()).to(dt), y, res, limit, dt, "two")
+
+
+@pytest.mark.parametrize("T,dt,group", [(4, BF, 64), (20, FP, 64)])
+def test_moe_limits_tell_three_terms_from_two(pkg, T, dt, group):
+    g = torch.Generator().manual_seed(T)
+    E, k, K, N = 6, 2, 256, 320
+    packed = [pkg.ops.kernels.quantize_weight_int4((torch.randn((E, r, c), generator=g) * c ** -0.5).to(dt), group)
+              for r, c in ((N, K), (N, K), (K, N))]
+    wg, wu, wd = (ft.unpack(*q) for q in packed)
+    x = torch.randn((T, K), generator=g).to(dt).double()
+    ids = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)])
+    wts = torch.rand((T, k), generator=g) + 0.1
+    y, limit = ft.moe_rms(x, ids, wts, wg, packed[0].scale, wu, packed[1].scale, wd, packed[2].scale, dt)
+    res = ft.cancelling_residual(y, dt)
+    for terms in (3, 2):
+        top = wts.double().amax(1, keepdim=True)
+        hs = torch.zeros((T, E, N), dtype=torch.float64)
+        a = ft.as_terms(x, group, terms)
+        for t in range(T):
+            for j in range(k):
+                e = int(ids[t, j])
+                h = torch.nn.functional.silu(a[t] @ wg[e].t()) * (a[t] @ wu[e].t())
+                hs[t, e] = (h * wts[t, j].double() / top[t]).to(dt).double()
+        largest = None if T <= 4 else hs.abs().amax((1, 2), keepdim=True).flatten(1)
+        got = top * ft.as_terms(hs.flatten(1), group, terms, largest) @ wd.transpose(0, 1).flatten(1).t()
+        got = (got + res.double()).to(dt)
+        if terms == 3:
+            ft.check_rms(got, y, res, limit, dt, "three")
+        else:
+            with pytest.raises(AssertionError, match="root-mean-square"):
+                ft.check_rms(got, y, res, limit, dt, "two")
