@@ -431,6 +431,13 @@ def decode_scratch(M: int, K: int, N: int, dt: torch.dtype, device: torch.device
     return torch.zeros(((nbytes + 3) // 4,), dtype=torch.int32, device=device)
 
 
+def _check_scratch(scratch: Tensor, dev: torch.device) -> None:
+    """A caller's scratch is an address to the kernels: it has to be one piece of `dev`'s memory."""
+    if scratch.device != dev or not scratch.is_contiguous():
+        raise ValueError(f"scratch must be a contiguous tensor on {dev}; got one of strides {scratch.stride()} on "
+                         f"{scratch.device}")
+
+
 def decode_fwd(x: Tensor, w_gate: Tensor, b_gate: Tensor | None, w_up: Tensor, b_up: Tensor | None,
                w_down: Tensor, b_down: Tensor | None, scratch: Tensor | None = None, act: str = "silu",
                residual: Tensor | None = None, out: Tensor | None = None, row_scale: Tensor | None = None,
@@ -451,6 +458,7 @@ def decode_fwd(x: Tensor, w_gate: Tensor, b_gate: Tensor | None, w_up: Tensor, b
         raise ValueError(f"decode path needs 1 <= M <= 64 and K, N multiples of 64; got M={M} K={K} N={N}")
     if scratch is None:
         scratch = decode_scratch(M, K, N, dt, dev)
+    _check_scratch(scratch, dev)
     h = torch.empty((M, N), dtype=dt, device=dev)
     y = _out_buffer(out, (M, K), dt, dev)
     prob = _problem(M, K, N, dt, NO_DROPOUT, NO_SHARD, act, _lib.tune_word(ordinary_launch=ordinary_launch))
@@ -515,6 +523,7 @@ def decode_fwd_fp8(x: Tensor, w_gate8: Tensor, w_gate_scale: Tensor, b_gate: Ten
         raise ValueError(f"8-bit decode path needs 1 <= M <= 64 and K, N multiples of 128; got M={M} K={K} N={N}")
     if scratch is None:
         scratch = decode_scratch(M, K, N, dt, dev)
+    _check_scratch(scratch, dev)
     x8 = torch.empty((M, K), dtype=torch.uint8, device=dev)
     xs = torch.empty((M,), dtype=torch.float32, device=dev)
     h = torch.empty((M, N), dtype=dt, device=dev)
@@ -656,6 +665,7 @@ def _few_buffers(scratch: Tensor | None, K: int, N: int, experts: int, work: int
     """Addresses of scratch and work buffer, and what has to stay alive until the call has been made."""
     if scratch is None:
         return _scratch_for((-(-N // 128)) * experts * 4 + (-(-K // 128)) * 4 + 512, work, dev, stream)
+    _check_scratch(scratch, dev)
     own = torch.empty((work,), dtype=torch.uint8, device=dev)
     return scratch.data_ptr(), scratch.numel() * scratch.element_size(), own.data_ptr(), own
 
