@@ -568,12 +568,13 @@ def quantize_weight_int4(w: Tensor, group: int = 128, symmetric: bool = False) -
     if w.dtype not in (torch.bfloat16, torch.float16):
         raise NotImplementedError(f"4-bit weights are made from bfloat16 or float16 matrices, got {w.dtype}")
     v = w.detach().float().unflatten(-1, (-1, group))
+    least = 2.0 ** -24 if w.dtype is torch.float16 else 2.0 ** -126   # a group of zeros; fp16's smallest number
     if symmetric:
-        scale = (v.abs().amax(-1) / 7.5).clamp_min(2.0 ** -24).to(w.dtype)
+        scale = (v.abs().amax(-1) / 7.5).clamp_min(least).to(w.dtype)
         zero = None
     else:
         lo, hi = v.amin(-1).clamp_max(0), v.amax(-1).clamp_min(0)
-        scale = ((hi - lo) / 15).clamp_min(2.0 ** -24).to(w.dtype)
+        scale = ((hi - lo) / 15).clamp_min(least).to(w.dtype)
         zero = (-lo / scale.float()).round().clamp(0, 15)
     q = (v / scale.float()[..., None]).round()
     q = (q + (8 if zero is None else zero[..., None])).clamp_(0, 15).to(torch.int32).flatten(-2)
