@@ -327,7 +327,8 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
  * largest activation that shares the power are exact, smaller ones off by at most 2^-31 of it, which is less than sums in
  * fp32 keep; it is shared by a token's group of columns up to 4 tokens and by a token from 5 on (in the down product of
  * a mixture by the token's hidden values of all experts). A NaN or infinite activation makes its token's outputs NaN,
- * and no other token's. Scales have to be finite. Gate and up matrices both have zeros or both have none.
+ * and no other token's; so does a hidden value that rounds to infinity in the 16-bit type (fp16: from 65520 on), where
+ * gmlp_decode_fwd goes on with the infinity. Scales have to be finite. Gate and up matrices both have zeros or both have none.
  *
  * gmlp_w4_linear: y[m,r] = sum_c x[m,c] w[r,c] (+ bias[r]) (+ residual[m,r]) for 1 <= M <= 64 and any rows >= 1; x
  *   has row pitch ldx (a multiple of 8), y and residual [M, rows] are contiguous.

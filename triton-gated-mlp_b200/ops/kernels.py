@@ -757,8 +757,8 @@ def decode_fwd_w4(x: Tensor, w_gate: Int4Weight, b_gate: Tensor | None, w_up: In
                   w_down: Int4Weight, b_down: Tensor | None, scratch: Tensor | None = None, act: str = "silu",
                   residual: Tensor | None = None, ordinary_launch: bool = False) -> Tensor:
     """decode_fwd on 4-bit weights with group scales (quantize_weight_int4); x, biases, residual and the result stay
-    16-bit, the hidden state is rounded to 16 bits between the two kernels as in decode_fwd. All three matrices share
-    one group size."""
+    16-bit, the hidden state is rounded to 16 bits between the two kernels as in decode_fwd (a value that overflows there
+    makes its token's outputs NaN). All three matrices share one group size."""
     dev = require_cuda(x, b_gate, b_up, b_down, residual)
     dt = _same_dtype(x, b_gate, b_up, b_down, residual)
     _few_common(x, dt, "decode_fwd_w4")
@@ -843,7 +843,8 @@ def moe_decode_fwd(x: Tensor, ids: Tensor, weights: Tensor, w_gate: Tensor, w_up
     """y[t] = sum_j weights[t, j] * MLP_e(x[t]) (+ residual[t]), e = ids[t, j], for at most 64 tokens, with
     MLP_e(x) = (act(x w_gate[e]^T) * (x w_up[e]^T)) w_down[e]^T; w_gate / w_up [experts, N, K], w_down [experts, K, N].
     ids and weights come from moe_route or from a router of the caller's: an id outside [0, experts) is skipped (-1
-    marks padding), a repeated one adds. Only the experts that some token chose are read."""
+    marks padding), a repeated one adds. Only the experts that some token chose are read. Weights that are not contiguous
+    (a transposed stack) are copied whole by every call."""
     dev = require_cuda(x, ids, weights, w_gate, w_up, w_down, residual)
     dt = _same_dtype(x, w_gate, w_up, w_down, residual)
     _few_common(x, dt, "moe_decode_fwd")
