@@ -26,3 +26,14 @@ def test_views_give_what_copies_give(pkg, view):
     w = torch.randn((40, 96), generator=torch.Generator().manual_seed(2)).to(BF)
     for a, b in zip(K_.quantize_weight_int4(view(w), 32), K_.quantize_weight_int4(w, 32)):
         assert a.is_contiguous() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_group_size_of_a_weight_and_what_the_decode_path_takes(pkg, group):
+    K_ = pkg.ops.kernels
+    w = K_.quantize_weight_int4(torch.zeros(2, 40, 256, dtype=BF), group)
+    assert w.group == group and K_.Int4Weight(*(t[0] for t in w)).group == group
+    assert K_.decode_w4_supported(1, 256, 384, group) and K_.decode_w4_supported(64, 256, 384, group)
+    for M, K, N, G in ((0, 256, 256, group), (65, 256, 256, group), (1, 256 + 16, 256, group), (1, 256, 16, group),
+                       (1, 256, 256, 48)):
+        assert not K_.decode_w4_supported(M, K, N, G)

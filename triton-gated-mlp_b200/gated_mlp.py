@@ -495,7 +495,8 @@ class FusedGatedMLP(nn.Module):
             raise NotImplementedError("the input norm is not available for float32 modules")
         if (not needs_grad and p == 0.0 and x.is_cuda and x.dtype != torch.float32
                 and (kernels.decode_supported(x.shape[0], self.hidden_size, self.intermediate_size)
-                     or (self._w4 is not None and 0 < x.shape[0] <= kernels.DECODE_MAX_TOKENS))):
+                     or (self._w4 is not None and kernels.decode_w4_supported(
+                         x.shape[0], self.hidden_size, self.intermediate_size, self._w4[0].group)))):
             y = self._decode_forward(x, tp_group, residual)
             return y.view(shapes) if len(shapes) > 2 else y
         if self.input_norm_weight is not None:

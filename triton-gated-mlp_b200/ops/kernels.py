@@ -556,6 +556,11 @@ class Int4Weight(NamedTuple):
     scale: Tensor
     zero: Tensor | None = None
 
+    @property
+    def group(self) -> int:
+        """Columns that share a scale."""
+        return 2 * self.w4.shape[-1] // self.scale.shape[-2]
+
 
 def quantize_weight_int4(w: Tensor, group: int = 128, symmetric: bool = False) -> Int4Weight:
     """One-off preparation of a 16-bit weight matrix [.., rows, cols] for the 4-bit paths: per row and group of `group`
