@@ -263,11 +263,13 @@ constexpr int W4_FUSED_TOKENS = 4;
 template <int MT, int GSHIFT, bool FUSED>
 struct W4Conf {
   static_assert(!FUSED || MT == 8, "one instantiation of each fused form");
-  // Up to 8 tokens the terms are columns of one MMA, which costs the same 16 clocks with 32 columns as with 16, and the
-  // accumulating warps add them up; above they are MMAs into one accumulator.
-  static constexpr bool STACKED = MT == 8;
-  static constexpr int TOK = FUSED ? W4_FUSED_TOKENS : MT;  // rows of a term
-  static constexpr int N = STACKED ? (W4_TERMS * TOK + 15) / 16 * 16 : MT;  // columns of the MMA
+  // Up to 8 tokens and with groups of 128 the terms are columns of one MMA, which costs the same 16 clocks with 32 columns as
+  // with 16, and the accumulating warps add them up; else they are MMAs into one accumulator, since smaller groups have
+  // more sums to add up (K=8192, N=28672 MLP without pause, G = 128 / 64 / 32: one token 77 / 109 / 254 us stacked, 85 / 108
+  // / 236 not; 8 tokens 91 / 109 / 256 and 93 / 108 / 190).
+  static constexpr bool STACKED = MT == 8 && GSHIFT == 2;
+  static constexpr int TOK = STACKED && FUSED ? W4_FUSED_TOKENS : MT;  // rows of a term
+  static constexpr int N = STACKED ? (W4_TERMS * TOK + 15) / 16 * 16 : MT < 16 ? 16 : MT;  // columns of the MMA
   // accumulating threads: four warps per share of the tokens; 64 tokens take sixteen warps (with eight, 64 sums a thread)
   static constexpr int SHARES = FUSED ? 1 : (MT == 64 ? 4 : 2);
   static constexpr int EPI = 128 * SHARES;
@@ -281,7 +283,7 @@ struct W4Conf {
   static constexpr int X_TERM = TOK * 128;
   static constexpr int X_HALF = (W4_TERMS * X_TERM + 1023) / 1024 * 1024;
   static constexpr int X_STAGE = (2 * X_HALF + GPU * FACTORS * MT * 4 + 1023) / 1024 * 1024;
-  static_assert(X_STAGE >= X_HALF + N * 128, "the MMA reads N rows of the second half");
+  static_assert(X_STAGE >= X_HALF + (STACKED ? 0 : (W4_TERMS - 1) * X_TERM) + N * 128, "the MMA reads N rows");
   static constexpr int M_STAGE = 2 * GPU * W4_META_ROW;  // scales and zeros of a unit as they lie in memory
   static constexpr int S_STAGE = 2 * GPU * 128 * 4;      // and as a word per row: scale << 16 | zero
   static constexpr int SIDE = X_STAGE + M_STAGE + S_STAGE;
