@@ -339,7 +339,7 @@ int gmlp_decode_fwd_fp8(const gmlp_problem_t* p, const void* x, const void* w_ga
  * gmlp_moe_route: the router. logits = x w_router^T ([experts, K]), exact products summed in fp64; per token ids[M, top_k] = the experts of the top_k
  *   largest logits in descending order (equal ones, to within 2^-43 of them: lower index first; a NaN ranks below every number, so the ids
  *   are valid and distinct whatever x holds), weights[M, top_k] = softmax over all experts at those ids,
- *   divided by their sum if `renormalize`. experts <= 512, top_k <= min(32, experts), any M.
+ *   divided by their sum if `renormalize`. experts <= 512, top_k <= min(32, experts), M < 2^24, K a multiple of 8.
  * gmlp_moe_decode_fwd: y[t] = sum_j weights[t,j] * MLP_{ids[t,j]}(x[t]) (+ residual[t]) with
  *   MLP_e(x) = (act(x w_gate[e]^T) * (x w_up[e]^T)) w_down[e]^T; w_gate, w_up [experts, N, K], w_down [experts, K, N],
  *   K and N multiples of 64, M <= 64. Only experts that some token chose are read. An id outside [0, experts) is

@@ -46,13 +46,14 @@
 //
 // Work split: stream-K over units of (two row tiles, 256 columns) as in few_token.cuh.
 //
-// Measured (one B200, replayed from a graph, G = 128): gated MLP K=8192, N=28672 of one token 70 us = 5.3 TB/s of the packed
-// bytes (the copy rate is 6.56), 8 tokens 81, 16 tokens 89, 32 tokens 109, 64 tokens 159 (G = 64: 227, G = 32: 438);
-// product 131072 x 4096, 8 tokens 56 us; 4096 x 4096, one token 8.5 us, of which 7 are the life of a block from its start to
-// its join. Of an MLP's time 16 us (one token) to 37 (32 tokens) do not grow with N: starts, joins and the terms. Up to 16
+// Measured (one B200, replayed from a graph, G = 128): gated MLP K=8192, N=28672 of one token 71 us = 5.2 TB/s of the packed
+// bytes (the copy rate is 6.56), 8 tokens 83, 16 tokens 88, 32 tokens 111, 64 tokens 168 (G = 64: 235, G = 32: 463);
+// product 131072 x 4096, 8 tokens 60 us; 4096 x 4096, one token 8.7 us, of which 7 are the life of a block from its start to
+// its join. Of an MLP's time 16 us (one token) to 33 (64 tokens) do not grow with N: starts, joins and the terms. Up to 16
 // tokens HBM bounds the rest. Above, the accumulating warps do: two instructions per two (row, token) sums of a group,
-// and the trip of the sums through tensor memory (at 64 tokens 55 % of the issue slots, 40 % of the tensor pipe, 29 % of
-// HBM). Fetching a group's sums while those of the group before are worked on was slower (64 tokens: 164 us).
+// and the trip of the sums through tensor memory (at 64 tokens 55 % of the issue slots, 41 % of the tensor pipe, 29 % of
+// HBM). Fetching a group's sums while those of the group before are worked on was slower (64 tokens: 164 us against 158 with
+// two terms; that third term costs bf16 9 us at 64 tokens and nothing measurable up to 32).
 #pragma once
 #include <cuda_fp8.h>
 
@@ -63,7 +64,10 @@ namespace gmlp {
 constexpr int W4_TILE_BYTES = 16384;  // 128 rows x 128 bytes: 256 columns
 constexpr int W4_UNIT_COLS = 256;
 constexpr int W4_HALF_COLS = 128;
-constexpr int W4_UNIT_CLOCKS = 1400;  // of one CTA, whether or not the others stream
+// Of one CTA, whether or not the others stream: what its weights take to arrive. Measured at 3 and 5 tokens; many tokens take
+// longer to accumulate (64 tokens with G = 128 / 64 / 32: about 3,900 / 5,500 / 10,800 clocks, from the times above), so that
+// a short tile of theirs stays whole (see cut_grain) where cutting it would leave fewer SMs idle.
+constexpr int W4_UNIT_CLOCKS = 1400;
 
 constexpr int W4_TERMS = 3;  // per activation
 

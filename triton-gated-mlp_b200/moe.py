@@ -4,7 +4,8 @@ The layer that stands in FusedGatedMLP's place in a mixture-of-experts block:
   y[t] = sum_j weights[t, j] * MLP_{ids[t, j]}(x[t]) (+ residual[t])
 with ids and weights from a linear router (softmax over all experts, the top_k largest, optionally divided by their
 sum) and MLP_e the gated MLP of FusedGatedMLP without biases. Three launches for up to 64 tokens (router, gate/up of
-the chosen experts, their down projections); only the experts that some token chose are read. There is no counterpart
+the chosen experts, their down projections), five on 4-bit experts from 5 tokens on (before each of the two a kernel
+that makes the activations' terms); only the experts that some token chose are read. There is no counterpart
 in the reference, whose module has one MLP (src/triton_gated_mlp/gated_mlp.py:203-237).
 """
 from __future__ import annotations

@@ -799,7 +799,8 @@ MOE_MAX_TOP_K = 32
 def moe_route(x: Tensor, w_router: Tensor, top_k: int, renormalize: bool = True):
     """The router of a mixture of experts: (ids int32 [M, top_k], weights float32 [M, top_k]) with ids the experts of
     the top_k largest logits x w_router^T ([experts, K]) in descending order (equal ones: lower index first) and
-    weights their softmax probabilities, divided by their sum when `renormalize`. Any number of tokens."""
+    weights their softmax probabilities, divided by their sum when `renormalize`. Any number of tokens below 2^24; K a
+    multiple of 8."""
     dev = require_cuda(x, w_router)
     dt = _same_dtype(x, w_router)
     if x.dim() != 2 or w_router.dim() != 2 or x.shape[1] != w_router.shape[1]:
