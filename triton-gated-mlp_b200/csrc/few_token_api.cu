@@ -398,8 +398,9 @@ int gmlp_moe_route(int64_t M, int64_t K, int32_t experts, int32_t top_k, int32_t
                    const void* x, int64_t ldx, const void* w_router, int32_t* ids, float* weights, void* stream) {
   int rc;
   if (dtype != GMLP_BF16 && dtype != GMLP_FP16) return fail(GMLP_ERR_DTYPE, "the router takes bf16 or fp16");
-  if (M < 1 || M > 0xffffffLL || K < 1 || K > 0x7ffffff0LL || (K % 8) != 0)
-    return fail(GMLP_ERR_SHAPE, "the router needs 1 <= M < 2^24 and K a positive multiple of 8; got M=%lld K=%lld",
+  if (M < 1 || M > 0xffffffLL || K < 1 || K > 0x7ffffe00LL || (K % 8) != 0)
+    return fail(GMLP_ERR_SHAPE,
+                "the router needs 1 <= M < 2^24 and K a positive multiple of 8 below 2^31 - 511; got M=%lld K=%lld",
                 static_cast<long long>(M), static_cast<long long>(K));
   if (experts < 1 || experts > MOE_MAX_EXPERTS)
     return fail(GMLP_ERR_SHAPE, "%d experts: 1 to %d are supported", experts, MOE_MAX_EXPERTS);

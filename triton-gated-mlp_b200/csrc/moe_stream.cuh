@@ -339,8 +339,8 @@ __device__ __forceinline__ unsigned long long sort_key(double v, int e) {
   if (v != v) b = 0x0008000000000000ull;  // below the key of -inf, above that of a removed entry (0)
   return (b & ~511ull) | static_cast<unsigned long long>(511 - e);
 }
-// A 16-bit value (as the float it was converted to) times 2^-896, exactly, subnormals too: its exponent and fraction bits moved to
-// a double's place, with the exponent's bias left as it is. Not for infinities and NaNs.
+// A 16-bit value (as the float it was converted to) times 2^-896, exactly, subnormals too: its exponent and fraction bits
+// moved to a double's place, with the exponent's bias left as it is. Not for infinities and NaNs.
 constexpr double WIDENED = 0x1p896;
 __device__ __forceinline__ double widened(float v) {
   return __hiloint2double((__float_as_int(v) >> 3) & static_cast<int>(0x8fffffffu), 0);
